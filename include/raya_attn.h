@@ -74,6 +74,24 @@ typedef struct {
   float scale;      /* softmax scale applied to q.k */
 } raya_attn_desc;
 
+/* A learned relative position bias, added to the scaled score of query i and
+ * key j: table[head][bucket(j - i)].  `table` is a DEVICE array
+ * [heads][buckets] of floats; `buckets` is even, 4 to 128.  Half of the
+ * buckets hold j - i <= 0, the other half (buckets / 2 + k) j - i > 0.  In
+ * each half, with first = buckets / 4 and rest = buckets / 2 - first, bucket
+ * k < first holds the distance k alone, bucket first + k the distances from
+ * first * (max_distance / first)^(k / rest) up to where the next one begins,
+ * and the last one everything further.  The bounds are whole numbers, found
+ * exactly (raya_attn_bias_bounds).  max_distance: above first, below 2^29.
+ * An entry of -inf, or at or below -2^100 (such as the lowest float), masks
+ * its bucket: those keys get no weight, and a row that is left with no key
+ * is zero, as under a mask that allows none. */
+typedef struct {
+  const float* table;
+  int32_t buckets;
+  int32_t max_distance;
+} raya_attn_bias;
+
 /* Kernel selection for raya_attn_forward_ex (tests and benchmarks). */
 typedef enum {
   RAYA_KERNEL_AUTO = 0,     /* head_dim 64: the tensor-core kernel
@@ -223,6 +241,51 @@ raya_attn_status raya_attn_packed_workspace(const raya_attn_desc* desc, float ro
  * Arguments and results as raya_attn_forward_packed. */
 raya_attn_status raya_attn_forward_packed_noalloc(const raya_attn_desc* desc, const float* qkv, float* ctx,
                                                   const int32_t* valid_len, float rope_theta, void* stream);
+
+/* Training: the forward pass that leaves what the backward pass reads, with
+ * an optional relative position bias (`bias` NULL: none), and the backward
+ * pass.  No counterpart in the reference, which only runs inference.
+ *
+ * raya_attn_forward_bias computes raya_attn_forward's result with x_ij =
+ * scale * q_i . k_j + bias as the score, and, where `stats` is not NULL, the
+ * row statistics stats[row] = (m, l): the largest score m_i = max_j x_ij and
+ * l_i = sum_j exp(x_ij - m_i) over the allowed keys; (-inf, 0) for a row
+ * without keys.  `stats` is a DEVICE array of batch*heads*seq pairs of
+ * floats, and log(l) + m is the row's log-sum-exp.  The score accuracy is
+ * that of fp32 (3xFP16 products on the tensor cores for head_dim <= 128).
+ *
+ * raya_attn_backward takes q, k, v, out and stats of such a forward pass
+ * with the same descriptor, valid_len and bias, and dout, the gradient of
+ * out.  It recomputes p_ij = exp(x_ij - m_i) / l_i and writes dq, dk and dv,
+ * and with a bias (dtable not NULL) the gradient of its table,
+ * dtable[heads][buckets].  Rows at or beyond valid_len of q, k, v, out,
+ * stats and dout are not read; those of dq, dk and dv are written as +0.0f,
+ * and buckets that no allowed pair falls into get 0.  The outputs must not
+ * overlap the inputs or one another.
+ *
+ * Both are asynchronous on `stream`, allocate nothing, keep nothing between
+ * calls and sum in a fixed order, so that equal calls give equal bits.  They
+ * need a DEVICE workspace of raya_attn_train_workspace bytes (`backward`:
+ * which of the two; the bias's table is not read there), 16-byte aligned,
+ * that no other call uses while this one runs.  The valid lengths are read
+ * on the device and clamped into [0, seq] as by raya_attn_forward.
+ * head_dim <= 256; the kernels are chosen by head_dim alone. */
+raya_attn_status raya_attn_forward_bias(const raya_attn_desc* desc, const float* q, const float* k, const float* v,
+                                        float* out, float* stats, const int32_t* valid_len,
+                                        const raya_attn_bias* bias, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+
+raya_attn_status raya_attn_backward(const raya_attn_desc* desc, const float* q, const float* k, const float* v,
+                                    const float* out, const float* stats, const float* dout, float* dq, float* dk,
+                                    float* dv, const int32_t* valid_len, const raya_attn_bias* bias, float* dtable,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+raya_attn_status raya_attn_train_workspace(const raya_attn_desc* desc, const raya_attn_bias* bias, int backward,
+                                           size_t* bytes);
+
+/* The smallest distance |j - i| of each bucket of one half, into the HOST
+ * array bounds[buckets / 2] (bounds[0] = 0).  Host-only. */
+raya_attn_status raya_attn_bias_bounds(int32_t buckets, int32_t max_distance, int32_t* bounds);
 
 /* Stage timing, the counterpart of Tiled::attend_with_stages / StageTimes
  * (tiled/mod.rs:60-126, tiled/stages.rs:1-31): raya_attn_forward_ex whose

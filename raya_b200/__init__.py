@@ -17,9 +17,9 @@ import importlib
 
 _FROM_ATTENTION = (
     "BLOCK", "WINDOW", "AttentionKernel", "AttnParams", "AttnShape", "Cuda", "CudaConfig", "CudaError",
-    "DeviceTimeout", "KernelError", "LengthError", "Mask", "ShapeError", "UnsupportedError", "ErrorInfo",
-    "fill_normal", "ffma_peak", "kernel_for", "last_error_info", "make_desc", "multi_gpu", "shard", "stage_times",
-    "sync_status", "validate", "work",
+    "DeviceTimeout", "KernelError", "LengthError", "Mask", "RelativeBias", "ShapeError", "UnsupportedError",
+    "ErrorInfo", "fill_normal", "ffma_peak", "kernel_for", "last_error_info", "make_desc", "multi_gpu", "shard", "stage_times",
+    "sync_status", "train_workspace", "validate", "work",
 )
 _FROM_LIB = (
     "KERNEL_AUTO", "KERNEL_ROWWISE", "KERNEL_TC16_WS", "KERNEL_TC16_WS2", "KERNEL_TC32_WS", "KERNEL_TC32_WS2",

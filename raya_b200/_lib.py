@@ -29,7 +29,8 @@ EXPORTS = (
     "raya_attn_ffma_peak", "raya_attn_version", "raya_attn_forward_timed",
     "raya_attn_probe_timeout", "raya_attn_forward_packed", "raya_attn_packed_workspace",
     "raya_attn_forward_packed_noalloc", "raya_attn_kernel_for", "raya_attn_last_error_info",
-    "raya_attn_forward_multi_gpu",
+    "raya_attn_forward_multi_gpu", "raya_attn_forward_bias", "raya_attn_backward",
+    "raya_attn_train_workspace", "raya_attn_bias_bounds",
 )
 
 
@@ -47,6 +48,12 @@ class Desc(ctypes.Structure):
         ("window", ctypes.c_int64),
         ("scale", ctypes.c_float),
     ]
+
+
+class Bias(ctypes.Structure):
+    """raya_attn_bias."""
+
+    _fields_ = [("table", ctypes.c_void_p), ("buckets", ctypes.c_int32), ("max_distance", ctypes.c_int32)]
 
 
 def _load() -> ctypes.CDLL:
@@ -76,6 +83,15 @@ def _load() -> ctypes.CDLL:
     lib.raya_attn_packed_workspace.restype = st
     lib.raya_attn_forward_packed_noalloc.argtypes = [dp, vp, vp, vp, ctypes.c_float, vp]
     lib.raya_attn_forward_packed_noalloc.restype = st
+    bp = ctypes.POINTER(Bias)
+    lib.raya_attn_forward_bias.argtypes = [dp, vp, vp, vp, vp, vp, vp, bp, vp, sz, vp]
+    lib.raya_attn_forward_bias.restype = st
+    lib.raya_attn_backward.argtypes = [dp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, bp, vp, vp, sz, vp]
+    lib.raya_attn_backward.restype = st
+    lib.raya_attn_train_workspace.argtypes = [dp, bp, ctypes.c_int, ctypes.POINTER(sz)]
+    lib.raya_attn_train_workspace.restype = st
+    lib.raya_attn_bias_bounds.argtypes = [ctypes.c_int32, ctypes.c_int32, ip]
+    lib.raya_attn_bias_bounds.restype = st
     lib.raya_attn_probe_timeout.argtypes = [ctypes.c_int64, vp]
     lib.raya_attn_probe_timeout.restype = st
     lib.raya_attn_sync_status.argtypes = [vp]

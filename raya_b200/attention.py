@@ -21,6 +21,7 @@ CUDA library; there is no CPU path.
 from __future__ import annotations
 
 import abc
+import contextlib
 import ctypes
 from dataclasses import dataclass, field
 from typing import Sequence, Union
@@ -193,6 +194,36 @@ class AttnParams:
         if (v < -2**31).any() or (v > 2**31 - 1).any():
             raise ShapeError("invalid shape: valid_len out of int32 range")
         return np.ascontiguousarray(v.astype(np.int32))
+
+
+@dataclass(frozen=True, eq=False)
+class RelativeBias:
+    """A learned relative position bias (``raya_attn_bias``): ``table`` is a
+    CUDA float32 tensor [heads][buckets], the bias of every distance bucket;
+    query i and key j get ``table[head][bucket(j - i)]``.  buckets is even, 4
+    to 128; distances at or beyond ``max_distance`` share the last bucket of
+    their side.  An entry of -inf, or the type's lowest value, masks its
+    bucket."""
+
+    table: object
+    max_distance: int = 128
+
+    @property
+    def buckets(self) -> int:
+        return int(self.table.shape[-1])
+
+    def bounds(self) -> np.ndarray:
+        """The smallest distance of each bucket of one side (host-only)."""
+        n = self.buckets
+        out = np.zeros(max(n // 2, 1), dtype=np.int32)
+        _check(lib.raya_attn_bias_bounds(n, self.max_distance, _i32p(out)))
+        return out
+
+    def bucket(self, rel) -> np.ndarray:
+        """The bucket of rel = j - i, elementwise (host-only)."""
+        r = np.asarray(rel, dtype=np.int64)
+        near = np.searchsorted(self.bounds(), np.abs(r), side="right") - 1
+        return near + (r > 0) * (self.buckets // 2)
 
 
 def make_desc(shape: AttnShape, params: AttnParams) -> Desc:
@@ -386,6 +417,121 @@ class Cuda(AttentionKernel):
             workspace.record_stream(torch.cuda.ExternalStream(stream, device=qkv.device))
         if valid_len is None:  # keep the uploaded lengths alive until the kernel has run
             _sync(stream)
+
+
+    def attend_bias(self, shape: AttnShape, params: AttnParams, q, k, v, out, stats=None,
+                    bias: RelativeBias | None = None, valid_len=None, workspace=None, stream=None) -> None:
+        """attend_device with a relative position bias on the scores and, for
+        the backward pass, the row statistics (``raya_attn_forward_bias``):
+        ``stats`` [batch][heads][seq][2] gets each row's largest score and
+        the sum of exp(score - largest), (-inf, 0) for a row without keys.
+        Both are optional.  Contiguous CUDA float32 tensors on one device;
+        asynchronous on ``stream`` (the current one of that device if None),
+        except that uploading ``params.valid_len`` (``valid_len`` None, and
+        some sequence padded) waits for the call.  A caller's ``workspace``
+        (a CUDA tensor of at least train_workspace bytes) must not be used by
+        another call meanwhile; without one the call takes it from torch's
+        caching allocator."""
+        c = _TrainCall(shape, params, bias, valid_len, workspace, stream, {"q": q, "k": k, "v": v, "out": out}, stats)
+        with c.run(False) as ws:
+            _check(lib.raya_attn_forward_bias(c.desc, c.ptr["q"], c.ptr["k"], c.ptr["v"], c.ptr["out"],
+                                              c.ptr["stats"], c.valid, c.bias, *ws, c.stream))
+
+    def attend_backward(self, shape: AttnShape, params: AttnParams, q, k, v, out, stats, dout, dq, dk, dv,
+                        bias: RelativeBias | None = None, dtable=None, valid_len=None, workspace=None,
+                        stream=None) -> None:
+        """The gradients of attend_bias (``raya_attn_backward``): ``out`` and
+        ``stats`` are what it gave for the same shape, params, valid_len and
+        bias, ``dout`` is the gradient of out; writes ``dq``, ``dk``, ``dv``
+        and, with a bias, its table's gradient into ``dtable``
+        [heads][buckets] unless that is None.  The probabilities are
+        recomputed, every sum is taken in a fixed order.  Tensors, streams
+        and workspace as for attend_bias."""
+        if stats is None:
+            raise TypeError("attend_backward needs the stats of attend_bias")
+        c = _TrainCall(shape, params, bias, valid_len, workspace, stream,
+                       {"q": q, "k": k, "v": v, "out": out, "dout": dout, "dq": dq, "dk": dk, "dv": dv}, stats, dtable)
+        with c.run(True) as ws:
+            _check(lib.raya_attn_backward(c.desc, *(c.ptr[n] for n in ("q", "k", "v", "out", "stats", "dout", "dq", "dk", "dv")),
+                                          c.valid, c.bias, c.ptr["dtable"], *ws, c.stream))
+
+
+def train_workspace(shape: AttnShape, params: AttnParams, bias: RelativeBias | None = None,
+                    backward: bool = False) -> int:
+    """Workspace bytes of attend_bias, or of attend_backward (host-only)."""
+    d, need = make_desc(shape, params), ctypes.c_size_t()
+    b = None if bias is None else _lib.Bias(None, bias.buckets, bias.max_distance)
+    _check(lib.raya_attn_train_workspace(ctypes.byref(d), b, int(backward), ctypes.byref(need)))
+    return need.value
+
+
+class _TrainCall:
+    """The checked arguments of one training call: every tensor a contiguous
+    CUDA float32 tensor of its size, all on one device."""
+
+    def __init__(self, shape, params, bias, valid_len, workspace, stream, tensors, stats, dtable=None):
+        import torch
+
+        self.torch, self.device = torch, None
+        d = make_desc(shape, params)
+        self.desc, numel = ctypes.byref(d), shape.numel()
+        self.ptr = {n: self._take(n, x, numel) for n, x in tensors.items()}
+        self.ptr["stats"] = None if stats is None else self._take("stats", stats, 2 * shape.batch * shape.heads * shape.seq)
+        self.bias, self.ptr["dtable"] = None, None
+        if bias is not None:
+            entries = shape.heads * bias.buckets
+            self.bias = _lib.Bias(self._take("table", bias.table, entries), bias.buckets, bias.max_distance)
+            if dtable is not None:
+                self.ptr["dtable"] = self._take("dtable", dtable, entries)
+        elif dtable is not None:
+            raise TypeError("dtable without a bias")
+        self.keep = None
+        if valid_len is None:
+            host = params.valid_array(shape.batch)
+            if (host < 0).any() or (host > shape.seq).any():
+                raise ShapeError(f"invalid shape: valid_len outside [0, {shape.seq}]")
+            if (host != shape.seq).any():
+                self.keep = valid_len = torch.from_numpy(host).to(self.device)
+        self.valid = None if valid_len is None else self._take("valid_len", valid_len, shape.batch, torch.int32)
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        elif not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream), device=self.device)
+        if stream.device != self.device:
+            raise TypeError(f"the stream is on {stream.device}, the tensors are on {self.device}")
+        self.on, self.stream = stream, stream.cuda_stream
+        if workspace is not None and (not isinstance(workspace, torch.Tensor) or not workspace.is_contiguous()
+                                      or workspace.device != self.device):
+            raise TypeError("the workspace must be a contiguous CUDA tensor on the tensors' device")
+        self.workspace = workspace
+
+    def _take(self, name, x, numel, dtype=None):
+        dtype = dtype or self.torch.float32
+        if not isinstance(x, self.torch.Tensor) or not x.is_cuda or x.dtype != dtype or not x.is_contiguous():
+            raise TypeError(f"`{name}` must be a contiguous CUDA {dtype} tensor")
+        if self.device is None:
+            self.device = x.device
+        if x.device != self.device:
+            raise TypeError(f"`{name}` is on {x.device}, the other tensors are on {self.device}")
+        if x.numel() != numel:
+            raise LengthError(f"buffer `{name}` has length {x.numel()}, expected {numel}", name=name, got=x.numel(),
+                              expected=numel)
+        return x.data_ptr()
+
+    @contextlib.contextmanager
+    def run(self, backward: bool):
+        """Makes the tensors' device and the call's stream current and gives
+        the workspace's pointer and size.  Memory that is taken here is taken
+        on the call's stream, so the allocator orders its next use."""
+        with self.torch.cuda.stream(self.on):
+            ws = self.workspace
+            if ws is None:
+                need = ctypes.c_size_t()
+                _check(lib.raya_attn_train_workspace(self.desc, self.bias, int(backward), ctypes.byref(need)))
+                ws = self.torch.empty(need.value, dtype=self.torch.uint8, device=self.device)
+            yield (ws.data_ptr() or None, ws.numel() * ws.element_size())
+            if self.keep is not None:  # keep the uploaded lengths alive until the kernels have run
+                _sync(self.stream)
 
 
 STAGE_NAMES = ("qk", "softmax", "pv", "k_wait", "v_wait", "refill", "tiles", "total")

@@ -24,6 +24,8 @@
 #include "tc32_common.cuh"
 #include "tc32_ws.cuh"
 #include "tiled64.cuh"
+#include "train_common.cuh"
+#include "train_rowwise.cuh"
 
 namespace raya {
 namespace {
@@ -238,6 +240,10 @@ raya_attn_status ensure_ready(int dev, DeviceCtx** out) {
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(packed smem)");
       }
     }
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(train::rowwise_train_dq),
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             train::kMaxBuckets * train::kRowThreads * static_cast<int>(sizeof(float)));
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(rowwise_train_dq smem)");
     c.ready = true;
   }
   *out = &c;
@@ -842,6 +848,8 @@ raya_attn_status host_pipeline(int device, const HostJob& job) {
   return RAYA_ATTN_OK;
 }
 
+#include "train_host.cuh"
+
 }  // namespace
 }  // namespace raya
 
@@ -1040,6 +1048,58 @@ raya_attn_status raya_attn_forward_packed_noalloc(const raya_attn_desc* desc, co
     if (st != RAYA_ATTN_OK) return st;
   }
   return launch_packed(ctx_dev, desc, qkv, ctx, valid_len, rope ? reinterpret_cast<const float*>(table) : nullptr, s);
+}
+
+raya_attn_status raya_attn_bias_bounds(int32_t buckets, int32_t max_distance, int32_t* bounds) {
+  const raya_attn_status st = check_buckets(buckets, max_distance);
+  if (st != RAYA_ATTN_OK) return st;
+  if (!bounds) return fail(RAYA_ATTN_ERR_SHAPE, "invalid shape: null output");
+  const train::BucketBounds b = bucket_bounds(buckets, max_distance);
+  std::copy(b.at, b.at + buckets / 2, bounds);
+  return RAYA_ATTN_OK;
+}
+
+raya_attn_status raya_attn_train_workspace(const raya_attn_desc* desc, const raya_attn_bias* bias, int backward,
+                                           size_t* bytes) {
+  TrainPlan plan;
+  const raya_attn_status st = train_plan(desc, bias, backward != 0, &plan);
+  if (st != RAYA_ATTN_OK) return st;
+  if (!bytes) return fail(RAYA_ATTN_ERR_SHAPE, "invalid shape: null output");
+  *bytes = plan.bytes;
+  return RAYA_ATTN_OK;
+}
+
+raya_attn_status raya_attn_forward_bias(const raya_attn_desc* desc, const float* q, const float* k, const float* v,
+                                        float* out, float* stats, const int32_t* valid_len,
+                                        const raya_attn_bias* bias, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+  TrainIo io{};
+  io.q = q;
+  io.k = k;
+  io.v = v;
+  io.out_w = out;
+  io.stats_w = stats;
+  io.valid_len = valid_len;
+  return train_call(desc, io, bias, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), false);
+}
+
+raya_attn_status raya_attn_backward(const raya_attn_desc* desc, const float* q, const float* k, const float* v,
+                                    const float* out, const float* stats, const float* dout, float* dq, float* dk,
+                                    float* dv, const int32_t* valid_len, const raya_attn_bias* bias, float* dtable,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  TrainIo io{};
+  io.q = q;
+  io.k = k;
+  io.v = v;
+  io.out = out;
+  io.stats = stats;
+  io.dout = dout;
+  io.dq = dq;
+  io.dk = dk;
+  io.dv = dv;
+  io.dtable = dtable;
+  io.valid_len = valid_len;
+  return train_call(desc, io, bias, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), true);
 }
 
 raya_attn_status raya_attn_probe_timeout(int64_t timeout_cycles, void* stream) {

@@ -1,0 +1,214 @@
+// train_host.cuh — the host side of the training operators: argument checks,
+// the bias's bucket bounds, the workspace's layout and the launches.
+// Included by raya_attn.cu inside its anonymous namespace.
+
+constexpr int kMinBuckets = 4;
+constexpr int kMaxBucketPowers = train::kMaxBuckets / 4;
+constexpr long long kMaxDistance = 1ll << 29;
+
+raya_attn_status check_buckets(int32_t buckets, int32_t max_distance) {
+  if (buckets < kMinBuckets || buckets > train::kMaxBuckets || buckets % 2 != 0)
+    return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: %d bias buckets (an even number, %d to %d)", buckets,
+                kMinBuckets, train::kMaxBuckets);
+  if (max_distance <= buckets / 4 || max_distance >= kMaxDistance)
+    return fail(RAYA_ATTN_ERR_SHAPE, "invalid shape: max_distance %d (above %d, below %lld for %d buckets)",
+                max_distance, buckets / 4, kMaxDistance, buckets);
+  return RAYA_ATTN_OK;
+}
+
+// a^p * b^q as base-2^32 digits, least significant first (p + q <= 32
+// factors below 2^32, so 33 digits hold it).
+struct Digits {
+  uint32_t at[kMaxBucketPowers + 1];
+  int n;
+};
+Digits power_product(uint32_t a, int p, uint32_t b, int q) {
+  Digits x{{1}, 1};
+  for (int i = 0; i < p + q; ++i) {
+    const uint32_t factor = i < p ? a : b;
+    uint64_t carry = 0;
+    for (int k = 0; k < x.n; ++k) {
+      carry += static_cast<uint64_t>(x.at[k]) * factor;
+      x.at[k] = static_cast<uint32_t>(carry);
+      carry >>= 32;
+    }
+    if (carry) x.at[x.n++] = static_cast<uint32_t>(carry);
+  }
+  return x;
+}
+
+bool at_least(const Digits& x, const Digits& y) {  // x >= y
+  if (x.n != y.n) return x.n > y.n;
+  for (int k = x.n - 1; k >= 0; --k)
+    if (x.at[k] != y.at[k]) return x.at[k] > y.at[k];
+  return true;
+}
+
+// Bucket first + k begins at the least whole n >= first * (max / first)^(k /
+// rest).  Where that number is no whole one within double's error, rounding
+// up is safe; next to a whole number r the powers r^rest and first^(rest - k)
+// * max^k are compared exactly.
+train::BucketBounds bucket_bounds(int buckets, int max_distance) {
+  train::BucketBounds b{};
+  const int half = buckets / 2, first = half / 2, rest = half - first;
+  for (int k = 0; k < first; ++k) b.at[k] = k;
+  for (int k = 0; k < rest; ++k) {
+    const double x = first * std::pow(static_cast<double>(max_distance) / first, static_cast<double>(k) / rest);
+    const double r = std::round(x);
+    if (std::fabs(x - r) > 1e-9 * r)
+      b.at[first + k] = static_cast<int>(std::ceil(x));
+    else
+      b.at[first + k] = static_cast<int>(r) + (at_least(power_product(static_cast<uint32_t>(r), rest, 1, 0),
+                                                        power_product(static_cast<uint32_t>(first), rest - k,
+                                                                      static_cast<uint32_t>(max_distance), k))
+                                                   ? 0
+                                                   : 1);
+  }
+  return b;
+}
+
+// Where the workspace keeps what; offsets in bytes, each 16-byte aligned.
+struct TrainPlan {
+  int rel_half = 0;  // the bias table by distance covers rel in [-rel_half, rel_half)
+  int parts = 1;     // partials of the table's gradient per slice
+  size_t rel_bias = 0, rel_id = 0, delta = 0, part = 0;
+  size_t bytes = 0;
+};
+
+raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias, bool backward, TrainPlan* plan) {
+  raya_attn_status st = check_shape(d);
+  if (st != RAYA_ATTN_OK) return st;
+  if (bias && (st = check_buckets(bias->buckets, bias->max_distance)) != RAYA_ATTN_OK) return st;
+  // Below these every index of the kernels fits its type.
+  const long long kMaxRows = 1ll << 40, kMaxSlices = 0x7fffffffll;
+  if (d->batch > kMaxSlices / d->heads || d->batch * d->heads > kMaxRows / std::max<int64_t>(d->seq, 1))
+    return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: %lld sequences of %lld heads and %lld rows",
+                static_cast<long long>(d->batch), static_cast<long long>(d->heads), static_cast<long long>(d->seq));
+  *plan = TrainPlan{};
+  if (d->seq == 0) return RAYA_ATTN_OK;
+  const long long slices = d->batch * d->heads;
+  auto take = [plan](size_t bytes) {
+    const size_t at = plan->bytes;
+    plan->bytes += (bytes + 15) & ~static_cast<size_t>(15);
+    return at;
+  };
+  if (bias) {
+    plan->rel_half = static_cast<int>((d->seq + 127) / 128 * 128 + 128);
+    plan->rel_bias = take(static_cast<size_t>(d->heads) * 2 * plan->rel_half * sizeof(float));
+    plan->rel_id = take(2 * static_cast<size_t>(plan->rel_half));
+  }
+  // The row-wise kernels: blocks per slice for about eight blocks on each of
+  // the 148 SMs (more leaves warps with a row or two, and more partials).
+  const long long want = (d->seq + train::kRowWarps - 1) / train::kRowWarps;
+  plan->parts = static_cast<int>(std::min(want, std::max<long long>(1, 8 * 148 / slices)));
+  if (backward) {
+    plan->delta = take(static_cast<size_t>(slices) * d->seq * sizeof(float));
+    if (bias) plan->part = take(static_cast<size_t>(slices) * plan->parts * bias->buckets * sizeof(float));
+  }
+  return RAYA_ATTN_OK;
+}
+
+template <typename T>
+T* at(void* workspace, size_t offset) {
+  return reinterpret_cast<T*>(static_cast<char*>(workspace) + offset);
+}
+
+raya_attn_status check_launch(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? RAYA_ATTN_OK : cuda_fail(e, what);
+}
+
+// The tensors of a training call, in the order of the entry points.
+struct TrainIo {
+  const float *q, *k, *v, *out;
+  float* out_w;          // forward
+  const float* stats;    // backward
+  float* stats_w;        // forward, or nullptr
+  const float* dout;
+  float *dq, *dk, *dv, *dtable;
+  const int32_t* valid_len;
+};
+
+raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const raya_attn_bias* bias, void* workspace,
+                            size_t workspace_bytes, cudaStream_t stream, bool backward) {
+  TrainPlan plan;
+  raya_attn_status st = train_plan(d, bias, backward, &plan);
+  if (st != RAYA_ATTN_OK) return st;
+  if (!bias && io.dtable) return fail(RAYA_ATTN_ERR_SHAPE, "invalid shape: dtable without a bias");
+  if (bias && !bias->table) return fail(RAYA_ATTN_ERR_SHAPE, "invalid shape: null bias table");
+  if (d->seq == 0) {  // no rows; a gradient over none is zero
+    if (!io.dtable) return RAYA_ATTN_OK;
+    const cudaError_t e = cudaMemsetAsync(io.dtable, 0, static_cast<size_t>(d->heads) * bias->buckets * sizeof(float), stream);
+    return e == cudaSuccess ? RAYA_ATTN_OK : cuda_fail(e, "cudaMemsetAsync(dtable)");
+  }
+  const void* used[] = {io.q, io.k, io.v, backward ? io.out : io.out_w, backward ? io.stats : io.q,
+                        backward ? io.dout : io.q, backward ? io.dq : io.q, backward ? io.dk : io.q,
+                        backward ? io.dv : io.q};
+  for (const void* p : used)
+    if (!p) return fail(RAYA_ATTN_ERR_SHAPE, "invalid shape: null tensor pointer");
+  for (const void* p : used)
+    if (p != io.stats && !aligned16(p))
+      return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: tensors must be 16-byte aligned");
+  const float* stats = backward ? io.stats : io.stats_w;
+  if ((reinterpret_cast<uintptr_t>(stats) & 7u) != 0)
+    return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: stats must be 8-byte aligned");
+  if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes))
+    return fail_length("workspace", workspace ? workspace_bytes : 0, plan.bytes);
+  if (workspace && !aligned16(workspace))
+    return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: the workspace must be 16-byte aligned");
+  const long long slices = d->batch * d->heads;
+  const long long grid = slices * plan.parts;
+  if (grid > 0x7fffffffll)
+    return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: %lld CTAs exceed the grid limit", grid);
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  DeviceCtx* ctx = nullptr;
+  st = ensure_ready(dev, &ctx);
+  if (st != RAYA_ATTN_OK) return st;
+
+  train::TrainArgs t{};
+  t.a = make_args(d, io.q, io.k, io.v, backward ? const_cast<float*>(io.out) : io.out_w, io.valid_len, ctx->status);
+  t.scale = d->scale;
+  t.stats = reinterpret_cast<const float2*>(io.stats);
+  t.stats_out = reinterpret_cast<float2*>(io.stats_w);
+  t.dout = io.dout;
+  t.dq = io.dq;
+  t.dk = io.dk;
+  t.dv = io.dv;
+  t.parts = plan.parts;
+  if (bias) {
+    t.rel_half = plan.rel_half;
+    t.buckets = bias->buckets;
+    float* vec = at<float>(workspace, plan.rel_bias);
+    uint8_t* ids = at<uint8_t>(workspace, plan.rel_id);
+    t.rel_bias = vec;
+    t.rel_id = ids;
+    const dim3 blocks(static_cast<unsigned>(std::min<long long>((2ll * plan.rel_half + 255) / 256, 1024)),
+                      static_cast<unsigned>(std::min<int64_t>(d->heads, 64)));
+    train::rel_table_kernel<<<blocks, 256, 0, stream>>>(bias->table, static_cast<int>(d->heads), bias->buckets,
+                                                        plan.rel_half, bucket_bounds(bias->buckets, bias->max_distance),
+                                                        vec, ids);
+    if ((st = check_launch("bias table launch")) != RAYA_ATTN_OK) return st;
+  }
+  if (!backward) {
+    train::rowwise_train_fwd<<<static_cast<unsigned>(grid), train::kRowThreads, 0, stream>>>(t);
+    return check_launch("forward launch");
+  }
+  t.delta = at<float>(workspace, plan.delta);
+  size_t smem = 0;
+  if (io.dtable) {
+    t.part = at<float>(workspace, plan.part);
+    smem = static_cast<size_t>(bias->buckets) * train::kRowThreads * sizeof(float);
+  }
+  train::rowwise_train_dq<<<static_cast<unsigned>(grid), train::kRowThreads, smem, stream>>>(t);
+  if ((st = check_launch("query gradient launch")) != RAYA_ATTN_OK) return st;
+  train::rowwise_train_dkv<<<static_cast<unsigned>(grid), train::kRowThreads, 0, stream>>>(t);
+  if ((st = check_launch("key gradient launch")) != RAYA_ATTN_OK) return st;
+  if (io.dtable) {
+    train::bias_grad_kernel<<<dim3(static_cast<unsigned>(d->heads), static_cast<unsigned>(bias->buckets)), 256, 0, stream>>>(
+        t.part, static_cast<int>(d->batch), static_cast<int>(d->heads), plan.parts, bias->buckets, io.dtable);
+    st = check_launch("bias gradient launch");
+  }
+  return st;
+}
