@@ -26,6 +26,7 @@
 #include "tiled64.cuh"
 #include "train_common.cuh"
 #include "train_rowwise.cuh"
+#include "train_tc.cuh"
 
 namespace raya {
 namespace {
@@ -244,6 +245,13 @@ raya_attn_status ensure_ready(int dev, DeviceCtx** out) {
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              train::kMaxBuckets * train::kRowThreads * static_cast<int>(sizeof(float)));
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(rowwise_train_dq smem)");
+    for (auto fn : {train::tc_train_fwd<1, false>, train::tc_train_fwd<1, true>, train::tc_train_fwd<2, false>,
+                    train::tc_train_fwd<2, true>, train::tc_train_bwd<1, false>, train::tc_train_bwd<1, true>,
+                    train::tc_train_bwd<2, false>, train::tc_train_bwd<2, true>}) {
+      e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(train::kWholeCta));
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(tc_train smem)");
+    }
     c.ready = true;
   }
   *out = &c;

@@ -71,9 +71,17 @@ train::BucketBounds bucket_bounds(int buckets, int max_distance) {
 struct TrainPlan {
   int rel_half = 0;  // the bias table by distance covers rel in [-rel_half, rel_half)
   int parts = 1;     // partials of the table's gradient per slice
+  int panels = 0;    // 64-column panels of head_dim on the tensor cores; 0: the row-wise kernels
+  int tiles = 0;     // 64-row tiles per slice, an even number
+  long long chunk = 0;  // slices whose images the workspace holds at a time
   size_t rel_bias = 0, rel_id = 0, delta = 0, part = 0;
+  size_t img[4] = {}, exps[4] = {}, rows = 0;
   size_t bytes = 0;
 };
+
+// The images of one chunk of slices.  They are written and read within the
+// chunk's two launches, so the bound costs launches, not traffic.
+constexpr size_t kMaxImageBytes = size_t{2} << 30;
 
 raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias, bool backward, TrainPlan* plan) {
   raya_attn_status st = check_shape(d);
@@ -97,14 +105,30 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
     plan->rel_bias = take(static_cast<size_t>(d->heads) * 2 * plan->rel_half * sizeof(float));
     plan->rel_id = take(2 * static_cast<size_t>(plan->rel_half));
   }
-  // The row-wise kernels: blocks per slice for about eight blocks on each of
-  // the 148 SMs (more leaves warps with a row or two, and more partials).
-  const long long want = (d->seq + train::kRowWarps - 1) / train::kRowWarps;
-  plan->parts = static_cast<int>(std::min(want, std::max<long long>(1, 8 * 148 / slices)));
-  if (backward) {
-    plan->delta = take(static_cast<size_t>(slices) * d->seq * sizeof(float));
-    if (bias) plan->part = take(static_cast<size_t>(slices) * plan->parts * bias->buckets * sizeof(float));
+  if (d->head_dim <= 128) {
+    const int tensors = backward ? 4 : 3;
+    plan->panels = d->head_dim <= 64 ? 1 : 2;
+    plan->tiles = static_cast<int>((d->seq + 127) / 128 * 2);
+    plan->parts = plan->tiles / 2;
+    const size_t image = static_cast<size_t>(plan->tiles) * 2 * plan->panels * train::kPanelBytes;
+    // The grid of a chunk: three CTAs per 128-row tile and at most 2^31 in all.
+    plan->chunk = std::max<long long>(1, std::min<long long>({slices, static_cast<long long>(kMaxImageBytes / (tensors * image)),
+                                                              0x7fffffffll / (2ll * plan->tiles)}));
+    for (int i = 0; i < tensors; ++i) {
+      plan->img[i] = take(plan->chunk * image);
+      plan->exps[i] = take(plan->chunk * plan->tiles * sizeof(int));
+    }
+    if (backward) plan->rows = take(static_cast<size_t>(plan->chunk) * plan->tiles * 128 * sizeof(float));
+  } else {
+    // Blocks per slice for about eight blocks on each of the 148 SMs (more
+    // leaves warps with a row or two, and more partials).
+    const long long want = (d->seq + train::kRowWarps - 1) / train::kRowWarps;
+    plan->parts = static_cast<int>(std::min(want, std::max<long long>(1, 8 * 148 / slices)));
+    if (slices * plan->parts > 0x7fffffffll)
+      return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: %lld CTAs exceed the grid limit", slices * plan->parts);
+    if (backward) plan->delta = take(static_cast<size_t>(slices) * d->seq * sizeof(float));
   }
+  if (backward && bias) plan->part = take(static_cast<size_t>(slices) * plan->parts * bias->buckets * sizeof(float));
   return RAYA_ATTN_OK;
 }
 
@@ -128,6 +152,58 @@ struct TrainIo {
   float *dq, *dk, *dv, *dtable;
   const int32_t* valid_len;
 };
+
+raya_attn_status launch_rowwise(const TrainPlan& plan, train::TrainArgs t, void* workspace, cudaStream_t stream,
+                                bool backward) {
+  const unsigned grid = static_cast<unsigned>(static_cast<long long>(t.a.batch) * t.a.heads * plan.parts);
+  if (!backward) {
+    train::rowwise_train_fwd<<<grid, train::kRowThreads, 0, stream>>>(t);
+    return check_launch("forward launch");
+  }
+  t.delta = at<float>(workspace, plan.delta);
+  const size_t smem = t.part ? static_cast<size_t>(t.buckets) * train::kRowThreads * sizeof(float) : 0;
+  train::rowwise_train_dq<<<grid, train::kRowThreads, smem, stream>>>(t);
+  const raya_attn_status st = check_launch("query gradient launch");
+  if (st != RAYA_ATTN_OK) return st;
+  train::rowwise_train_dkv<<<grid, train::kRowThreads, 0, stream>>>(t);
+  return check_launch("key gradient launch");
+}
+
+// Chunk by chunk: the images of its slices, then every 128-row tile of them.
+template <int P>
+raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, void* workspace, cudaStream_t stream,
+                           bool backward) {
+  train::TcArgs c{};
+  c.t = t;
+  c.tiles = plan.tiles;
+  for (int i = 0; i < (backward ? 4 : 3); ++i) {
+    c.img[i] = at<uint8_t>(workspace, plan.img[i]);
+    c.exps[i] = at<int>(workspace, plan.exps[i]);
+  }
+  if (backward) c.rows = at<float>(workspace, plan.rows);
+  const int acc = t.part ? t.buckets : 0;
+  const size_t most = P == 1 ? train::kHalfSm : train::kWholeCta;
+  c.stages = train::tc_smem<P>(train::kMaxStages, acc) <= most ? train::kMaxStages : 2;
+  size_t smem = train::tc_smem<P>(c.stages, acc);
+  if (P == 1) smem = std::max(smem, train::kThirdSm);  // never three CTAs on an SM
+  const bool bias = t.rel_bias != nullptr;
+  const long long slices = static_cast<long long>(t.a.batch) * t.a.heads;
+  for (c.slice0 = 0; c.slice0 < slices; c.slice0 += plan.chunk) {
+    const long long n = std::min(plan.chunk, slices - c.slice0) * plan.tiles;
+    train::split_kernel<P><<<dim3(static_cast<unsigned>(n), backward ? 4 : 3), 256, 0, stream>>>(c);
+    raya_attn_status st = check_launch("operand split launch");
+    if (st != RAYA_ATTN_OK) return st;
+    if (backward)
+      (bias ? train::tc_train_bwd<P, true> : train::tc_train_bwd<P, false>)
+          <<<static_cast<unsigned>(3 * n / 2), train::kTcThreads, smem, stream>>>(c);
+    else
+      (bias ? train::tc_train_fwd<P, true> : train::tc_train_fwd<P, false>)
+          <<<static_cast<unsigned>(n / 2), train::kTcThreads, smem, stream>>>(c);
+    st = check_launch(backward ? "gradient launch" : "forward launch");
+    if (st != RAYA_ATTN_OK) return st;
+  }
+  return RAYA_ATTN_OK;
+}
 
 raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const raya_attn_bias* bias, void* workspace,
                             size_t workspace_bytes, cudaStream_t stream, bool backward) {
@@ -156,10 +232,6 @@ raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const ra
     return fail_length("workspace", workspace ? workspace_bytes : 0, plan.bytes);
   if (workspace && !aligned16(workspace))
     return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: the workspace must be 16-byte aligned");
-  const long long slices = d->batch * d->heads;
-  const long long grid = slices * plan.parts;
-  if (grid > 0x7fffffffll)
-    return fail(RAYA_ATTN_ERR_UNSUPPORTED, "unsupported: %lld CTAs exceed the grid limit", grid);
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -191,20 +263,13 @@ raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const ra
                                                         vec, ids);
     if ((st = check_launch("bias table launch")) != RAYA_ATTN_OK) return st;
   }
-  if (!backward) {
-    train::rowwise_train_fwd<<<static_cast<unsigned>(grid), train::kRowThreads, 0, stream>>>(t);
-    return check_launch("forward launch");
-  }
-  t.delta = at<float>(workspace, plan.delta);
-  size_t smem = 0;
-  if (io.dtable) {
-    t.part = at<float>(workspace, plan.part);
-    smem = static_cast<size_t>(bias->buckets) * train::kRowThreads * sizeof(float);
-  }
-  train::rowwise_train_dq<<<static_cast<unsigned>(grid), train::kRowThreads, smem, stream>>>(t);
-  if ((st = check_launch("query gradient launch")) != RAYA_ATTN_OK) return st;
-  train::rowwise_train_dkv<<<static_cast<unsigned>(grid), train::kRowThreads, 0, stream>>>(t);
-  if ((st = check_launch("key gradient launch")) != RAYA_ATTN_OK) return st;
+  if (io.dtable) t.part = at<float>(workspace, plan.part);
+  if (plan.panels > 0)
+    st = plan.panels == 1 ? launch_tc<1>(plan, t, workspace, stream, backward)
+                          : launch_tc<2>(plan, t, workspace, stream, backward);
+  else
+    st = launch_rowwise(plan, t, workspace, stream, backward);
+  if (st != RAYA_ATTN_OK) return st;
   if (io.dtable) {
     train::bias_grad_kernel<<<dim3(static_cast<unsigned>(d->heads), static_cast<unsigned>(bias->buckets)), 256, 0, stream>>>(
         t.part, static_cast<int>(d->batch), static_cast<int>(d->heads), plan.parts, bias->buckets, io.dtable);
