@@ -76,7 +76,7 @@ typedef struct {
 
 /* A learned relative position bias, added to the scaled score of query i and
  * key j: table[head][bucket(j - i)].  `table` is a DEVICE array
- * [heads][buckets] of floats; `buckets` is even, 4 to 128.  Half of the
+ * [heads][buckets] of floats; `buckets` is even, 4 to 64.  Half of the
  * buckets hold j - i <= 0, the other half (buckets / 2 + k) j - i > 0.  In
  * each half, with first = buckets / 4 and rest = buckets / 2 - first, bucket
  * k < first holds the distance k alone, bucket first + k the distances from

@@ -201,7 +201,7 @@ class RelativeBias:
     """A learned relative position bias (``raya_attn_bias``): ``table`` is a
     CUDA float32 tensor [heads][buckets], the bias of every distance bucket;
     query i and key j get ``table[head][bucket(j - i)]``.  buckets is even, 4
-    to 128; distances at or beyond ``max_distance`` share the last bucket of
+    to 64; distances at or beyond ``max_distance`` share the last bucket of
     their side.  An entry of -inf, or the type's lowest value, masks its
     bucket."""
 

@@ -245,9 +245,13 @@ raya_attn_status ensure_ready(int dev, DeviceCtx** out) {
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              train::kMaxBuckets * train::kRowThreads * static_cast<int>(sizeof(float)));
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(rowwise_train_dq smem)");
-    for (auto fn : {train::tc_train_fwd<1, false>, train::tc_train_fwd<1, true>, train::tc_train_fwd<2, false>,
-                    train::tc_train_fwd<2, true>, train::tc_train_bwd<1, false>, train::tc_train_bwd<1, true>,
-                    train::tc_train_bwd<2, false>, train::tc_train_bwd<2, true>}) {
+    using train::tc_train;
+    for (auto fn : {tc_train<train::kForward, 1, false>, tc_train<train::kForward, 1, true>,
+                    tc_train<train::kForward, 2, false>, tc_train<train::kForward, 2, true>,
+                    tc_train<train::kDq, 1, false>, tc_train<train::kDq, 1, true>, tc_train<train::kDq, 2, false>,
+                    tc_train<train::kDq, 2, true>, tc_train<train::kDk, 1, false>, tc_train<train::kDk, 1, true>,
+                    tc_train<train::kDk, 2, false>, tc_train<train::kDk, 2, true>, tc_train<train::kDv, 1, false>,
+                    tc_train<train::kDv, 1, true>, tc_train<train::kDv, 2, false>, tc_train<train::kDv, 2, true>}) {
       e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(train::kWholeCta));
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(tc_train smem)");

@@ -28,7 +28,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // value times log2(e) is no float, and no real score comes near it.
 constexpr float kMaskedBias = -1.2676506e30f;  // -2^100
 
-constexpr int kMaxBuckets = 128;
+constexpr int kMaxBuckets = 64;
 
 struct TrainArgs {
   AttnArgs a;              // q, k, v, out, valid_len, the mask, qscale = scale * log2(e)

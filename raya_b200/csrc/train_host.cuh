@@ -75,7 +75,7 @@ struct TrainPlan {
   int tiles = 0;     // 64-row tiles per slice, an even number
   long long chunk = 0;  // slices whose images the workspace holds at a time
   size_t rel_bias = 0, rel_id = 0, delta = 0, part = 0;
-  size_t img[4] = {}, exps[4] = {}, rows = 0;
+  size_t img[4] = {}, exps = 0, rows = 0;
   size_t bytes = 0;
 };
 
@@ -114,10 +114,8 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
     // The grid of a chunk: three CTAs per 128-row tile and at most 2^31 in all.
     plan->chunk = std::max<long long>(1, std::min<long long>({slices, static_cast<long long>(kMaxImageBytes / (tensors * image)),
                                                               0x7fffffffll / (2ll * plan->tiles)}));
-    for (int i = 0; i < tensors; ++i) {
-      plan->img[i] = take(plan->chunk * image);
-      plan->exps[i] = take(plan->chunk * plan->tiles * sizeof(int));
-    }
+    for (int i = 0; i < tensors; ++i) plan->img[i] = take(plan->chunk * image);
+    plan->exps = take(plan->chunk * plan->tiles * sizeof(int4));
     if (backward) plan->rows = take(static_cast<size_t>(plan->chunk) * plan->tiles * 128 * sizeof(float));
   } else {
     // Blocks per slice for about eight blocks on each of the 148 SMs (more
@@ -176,10 +174,8 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, voi
   train::TcArgs c{};
   c.t = t;
   c.tiles = plan.tiles;
-  for (int i = 0; i < (backward ? 4 : 3); ++i) {
-    c.img[i] = at<uint8_t>(workspace, plan.img[i]);
-    c.exps[i] = at<int>(workspace, plan.exps[i]);
-  }
+  for (int i = 0; i < (backward ? 4 : 3); ++i) c.img[i] = at<uint8_t>(workspace, plan.img[i]);
+  c.exps = at<int4>(workspace, plan.exps);
   if (backward) c.rows = at<float>(workspace, plan.rows);
   const int acc = t.part ? t.buckets : 0;
   const size_t most = P == 1 ? train::kHalfSm : train::kWholeCta;
@@ -193,13 +189,21 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, voi
     train::split_kernel<P><<<dim3(static_cast<unsigned>(n), backward ? 4 : 3), 256, 0, stream>>>(c);
     raya_attn_status st = check_launch("operand split launch");
     if (st != RAYA_ATTN_OK) return st;
-    if (backward)
-      (bias ? train::tc_train_bwd<P, true> : train::tc_train_bwd<P, false>)
-          <<<static_cast<unsigned>(3 * n / 2), train::kTcThreads, smem, stream>>>(c);
-    else
-      (bias ? train::tc_train_fwd<P, true> : train::tc_train_fwd<P, false>)
-          <<<static_cast<unsigned>(n / 2), train::kTcThreads, smem, stream>>>(c);
-    st = check_launch(backward ? "gradient launch" : "forward launch");
+    auto launch_kind = [&](void (*fn)(train::TcArgs), size_t shared, const char* what) {
+      fn<<<static_cast<unsigned>(n / 2), train::kTcThreads, shared, stream>>>(c);
+      return check_launch(what);
+    };
+    using train::tc_train;
+    if (!backward) {
+      st = launch_kind(bias ? tc_train<train::kForward, P, true> : tc_train<train::kForward, P, false>, smem, "forward launch");
+      if (st != RAYA_ATTN_OK) return st;
+      continue;
+    }
+    st = launch_kind(bias ? tc_train<train::kDq, P, true> : tc_train<train::kDq, P, false>, smem, "query gradient launch");
+    if (st == RAYA_ATTN_OK)
+      st = launch_kind(bias ? tc_train<train::kDk, P, true> : tc_train<train::kDk, P, false>, smem, "key gradient launch");
+    if (st == RAYA_ATTN_OK)
+      st = launch_kind(bias ? tc_train<train::kDv, P, true> : tc_train<train::kDv, P, false>, smem, "value gradient launch");
     if (st != RAYA_ATTN_OK) return st;
   }
   return RAYA_ATTN_OK;

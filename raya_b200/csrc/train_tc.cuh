@@ -41,9 +41,13 @@
 // the steps are serial, except that kForward and kDv compute the next scores
 // during the softmax (two score buffers).
 //
-// Roles (192 threads): warps 0-3 one row per thread (TMEM lane = row), warp 4
-// issues the MMAs, warp 5 the bulk copies; both run their loops on the whole
-// warp and issue from one lane.
+// Roles (320 threads): warps 0-7 the rows (TMEM lane = row), warps 0-3 the
+// first and 4-7 the second half of the columns of the scores and of the
+// output; what a row's two threads share (its maximum) passes through shared
+// memory at a barrier of their two warps.  Warp 8 issues the MMAs, warp 9 the
+// bulk copies; both run their loops on the whole warp and issue from one
+// lane.  With one thread per row (192 threads) the softmax's own latencies
+// set the pace: 3.4k cycles per tile and 31% of the issue slots used.
 //
 // Tensor memory, columns (P = panels): rows' operands (hi 32 P, lo 32 P,
 // twice for kDq and kDk), then scores: kForward and kDv two buffers of 64 and
@@ -64,8 +68,10 @@ namespace raya {
 namespace train {
 
 constexpr int kTileRows = 128, kTileCols = 64;
-constexpr int kTcThreads = 192;
-constexpr int kIssueWarp = 4, kCopyWarp = 5;
+constexpr int kTcThreads = 320;
+constexpr int kRowThreadsTc = 256;
+constexpr int kIssueWarp = 8, kCopyWarp = 9;
+constexpr int kPairBarrier = 1, kRowBarrier = 5;  // named barriers: 1-4 the warps of the same rows, 5 all row warps
 constexpr int kMaxStages = 3;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
@@ -81,7 +87,7 @@ enum { kImgQ = 0, kImgK = 1, kImgV = 2, kImgG = 3 };
 struct TcArgs {
   TrainArgs t;
   uint8_t* img[4];     // [chunk slices][tiles][2 P panels]: q, k, v, dout
-  int* exps[4];        // [chunk slices][tiles]
+  int4* exps;          // [chunk slices][tiles]: their exponents
   float* rows;         // [chunk slices][tiles][2][64]: m * log2(e) (inf: no key), and delta / l
   int tiles;           // 64-row tiles per slice (even)
   long long slice0;
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   for (int w = 1; w < 8; ++w) most = max(most, red[w]);
   const int e = tc16::scale_exp(most);
   const float sc = tc16::pow2(e);
-  if (tid == 0) c.exps[which][local * c.tiles + tile] = e;
+  if (tid == 0) reinterpret_cast<int*>(c.exps + local * c.tiles + tile)[which] = e;
   uint8_t* img = c.img[which] + (local * c.tiles + tile) * (2ll * P * kPanelBytes);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -181,7 +187,8 @@ struct TcTail {
   float vec[kMaxStages][kVec];       // bias * log2(e) by distance
   float rows[kMaxStages][2 * 64];    // kDk, kDv: the columns' exponent and delta
   uint8_t ids[kMaxStages][kVec];     // kDq: buckets by distance
-  int e1[kMaxStages], e2[kMaxStages];  // exponents of the stage's two operands
+  int exps[kMaxStages][4];           // exponents of the columns' 64 rows, by tensor
+  float red[2][2][kTileRows];        // [tile parity][half]: what a row's threads exchange
   uint64_t full[kMaxStages], freed[kMaxStages];
   uint64_t s_full[2], w_ready[2], part_full, part_free, a_ready;
   uint32_t tmem_base;
@@ -192,7 +199,7 @@ template <int P>
 constexpr size_t stage_bytes() { return 2ull * 2 * P * kPanelBytes; }
 template <int P>
 constexpr size_t tc_smem(int stages, int buckets) {
-  return 1024 + stages * stage_bytes<P>() + sizeof(TcTail) + static_cast<size_t>(buckets) * 128 * sizeof(float);
+  return 1024 + stages * stage_bytes<P>() + sizeof(TcTail) + static_cast<size_t>(buckets) * kRowThreadsTc * sizeof(float);
 }
 // head_dim <= 64: at most half of an SM's shared memory, and more than a
 // third, so that exactly two CTAs (2 x 256 tensor-memory columns) share it.
@@ -201,56 +208,43 @@ constexpr size_t kThirdSm = 233472 / 3;
 static_assert(tc_smem<1>(3, 0) <= kHalfSm, "two CTAs per SM");
 static_assert(tc_smem<1>(2, kMaxBuckets) <= kWholeCta && tc_smem<2>(2, kMaxBuckets) <= kWholeCta, "shared memory of a block");
 
-__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t* v) {
-  tc32::tmem_st32(taddr, reinterpret_cast<const float*>(v));
-}
-
 // A product of scales that would be infinite, as the largest float: 0 times it is 0.
 __device__ __forceinline__ float finite(float x) { return fmaxf(fminf(x, 3.4028235e38f), -3.4028235e38f); }
 
-// One row's operand, hi and lo, from its image into tensor memory columns
-// col..col + 64 P of this thread's lane.  Straight from global memory: each
-// row is read once, a whole 128-byte line per panel and half.
-template <int P>
-__device__ __forceinline__ void load_rows(const uint8_t* img, int row, uint32_t taddr) {
-  const uint8_t* base = img + static_cast<size_t>(row >> 6) * (2ll * P * kPanelBytes);
-  const int r = row & 63;
+// 128 bytes of an operand's row r (64 fp16 of one panel) as 32 words, from
+// its image.  Straight from global memory: each row is read once, a whole
+// line per panel and half.
+__device__ __forceinline__ void load_row(const uint8_t* panel, int r, uint32_t* w) {
 #pragma unroll
-  for (int part = 0; part < 2 * P; ++part) {  // hi panels, then lo panels
-    uint32_t w[32];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint4 x = *reinterpret_cast<const uint4*>(base + part * kPanelBytes + tc16::op_off(r, k));
-      w[4 * k] = x.x;
-      w[4 * k + 1] = x.y;
-      w[4 * k + 2] = x.z;
-      w[4 * k + 3] = x.w;
-    }
-    tmem_st32u(taddr + 32 * part, w);
+  for (int k = 0; k < 8; ++k) {
+    const uint4 x = *reinterpret_cast<const uint4*>(panel + tc16::op_off(r, k));
+    w[4 * k] = x.x;
+    w[4 * k + 1] = x.y;
+    w[4 * k + 2] = x.z;
+    w[4 * k + 3] = x.w;
   }
 }
 
-// Weights w[64] (fp32, already scaled) as fp16 hi and lo over their scores.
+// Weights w[32] (fp32, already scaled) as fp16 hi and lo over their scores.
 __device__ __forceinline__ void store_weights(uint32_t taddr, const float* w) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
+  for (int s = 0; s < 2; ++s) {
     uint32_t h[8], l[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) tc16::split2(w[16 * s + 2 * k], w[16 * s + 2 * k + 1], h[k], l[k]);
-    const uint32_t at = taddr + 32 * (s >> 1) + 8 * (s & 1);
-    tc16::tmem_st8u(at, h);
-    tc16::tmem_st8u(at + 16, l);
+    tc16::tmem_st8u(taddr + 8 * s, h);
+    tc16::tmem_st8u(taddr + 8 * s + 16, l);
   }
 }
 
-// The scores of 64 columns in place: s * mult (+ bias), -inf outside [lo, hi).
+// 32 scores in place: s * mult (+ bias), -inf outside [lo, hi).
 template <bool BIAS, int STEP>
 __device__ __forceinline__ void mask_scores(float* s, float mult, const float* vec, int lo, int hi, bool inside) {
 #pragma unroll
-  for (int i = 0; i < 64; ++i) s[i] = BIAS ? fmaf(s[i], mult, vec[STEP * i]) : s[i] * mult;
+  for (int i = 0; i < 32; ++i) s[i] = BIAS ? fmaf(s[i], mult, vec[STEP * i]) : s[i] * mult;
   if (!inside) {
 #pragma unroll
-    for (int i = 0; i < 64; ++i)
+    for (int i = 0; i < 32; ++i)
       if (i < lo || i >= hi) s[i] = -INFINITY;
   }
 }
@@ -260,12 +254,17 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
   using namespace tc32;
   constexpr bool kScores2 = KIND == kDq || KIND == kDk;      // S and dP, serial
   constexpr bool kByKey = KIND == kDk || KIND == kDv;        // rows are keys, columns queries
+  constexpr bool kShared = KIND != kDv;                      // a row's threads share a maximum
   constexpr uint32_t kCols = 256 * P;
   constexpr uint32_t kColA2 = 64 * P;
   constexpr uint32_t kColS = kScores2 ? 128 * P : 64 * P;
   constexpr uint32_t kColS2 = kColS + 64;                    // dP, or the second score buffer
   constexpr uint32_t kColPart = kScores2 ? (P == 1 ? kColS2 : kColS2 + 64) : kColS2 + 64;
   static_assert(kColPart + 64 * P <= kCols, "tensor memory");
+  constexpr int kB1 = kByKey ? kImgQ : kImgK, kB2 = kByKey ? kImgG : kImgV;  // the columns' operands
+  constexpr int kA1 = kByKey ? kImgK : kImgQ, kA2 = kByKey ? kImgV : kImgG;  // the rows'
+  constexpr uint32_t kOp = 2 * P * kPanelBytes;
+  constexpr int kOutCols = 32 * P;                           // output columns of a thread
 
   const AttnArgs& a = c.t.a;
   const int tid = threadIdx.x, warp = tid >> 5;
@@ -293,32 +292,65 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
   }
 
   TcTail& sm = *reinterpret_cast<TcTail*>(smem + c.stages * stage_bytes<P>());
-  float* acc = reinterpret_cast<float*>(&sm + 1);  // with_grad: [buckets][128]
+  float* acc = reinterpret_cast<float*>(&sm + 1);  // with_grad: [buckets][kRowThreadsTc]
   const int stages = c.stages;
-  constexpr int kB1 = kByKey ? kImgQ : kImgK, kB2 = kByKey ? kImgG : kImgV;  // the columns' operands
-  constexpr int kA1 = kByKey ? kImgK : kImgQ, kA2 = kByKey ? kImgV : kImgG;  // the rows'
+  const long long tile_base = local * c.tiles;
 
-  if (tid == 0) {
+  // Copies the operands and values of step g into its stage (one lane).
+  auto copy_stage = [&](int g) {
+    const int st = g % stages, c0 = (t0 + g) * kTileCols;
+    const long long tile = tile_base + t0 + g;
+    const int head = static_cast<int>(bh % a.heads);
+    // The tile's first distance j - i: rows' i from r0, or columns' i from c0.
+    const int rel = kByKey ? r0 - c0 - 64 : c0 - r0 - 128;
+    unsigned char* op = smem + st * stage_bytes<P>();
+    mbar_arrive_expect_tx(&sm.full[st], 2 * kOp + 16u + (BIAS ? kVec * 4u : 0u) + (kByKey ? 512u : 0u) +
+                                            (with_grad ? kVec : 0u));
+    tma_load_1d(op, c.img[kB1] + tile * static_cast<long long>(kOp), kOp, &sm.full[st]);
+    tma_load_1d(op + kOp, c.img[kB2] + tile * static_cast<long long>(kOp), kOp, &sm.full[st]);
+    tma_load_1d(sm.exps[st], c.exps + tile, 16u, &sm.full[st]);
+    if constexpr (BIAS)
+      tma_load_1d(sm.vec[st], c.t.rel_bias + (2ll * head + 1) * c.t.rel_half + rel, kVec * 4u, &sm.full[st]);
+    if (with_grad) tma_load_1d(sm.ids[st], c.t.rel_id + c.t.rel_half + rel, kVec, &sm.full[st]);
+    if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * 128, 512u, &sm.full[st]);
+  };
+
+  // Before the CTA's first barrier: the copy warp fills the stages, the
+  // issuing warp takes tensor memory, and the row threads load their rows
+  // (first halves of the row threads: the first operand, or its hi parts).
+  constexpr int kParts = kScores2 ? 2 * P : P;  // 32-word pieces of this thread
+  uint32_t arow[kParts][32];
+  const int half = warp >> 2, rt = tid & 127;
+  int4 ae = make_int4(0, 0, 0, 0);
+  if (warp < 8) {
+    const int which = kScores2 && half ? kA2 : kA1;
+    const uint8_t* img = c.img[which] + (tile_base + 2 * tile128 + (rt >> 6)) * static_cast<long long>(kOp) +
+                         (kScores2 ? 0 : half * P * kPanelBytes);
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) load_row(img + p * kPanelBytes, rt & 63, arow[p]);
+    ae = c.exps[tile_base + 2 * tile128 + (rt >> 6)];
+  } else if (warp == kIssueWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem_base)),
+                 "r"(kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (tc16::lane_is_first(tid)) {
     for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.freed[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sm.s_full[s], 1);
-      mbar_init(&sm.w_ready[s], 128);
+      mbar_init(&sm.w_ready[s], kRowThreadsTc);
     }
     mbar_init(&sm.part_full, 1);
-    mbar_init(&sm.part_free, 128);
-    mbar_init(&sm.a_ready, 128);
+    mbar_init(&sm.part_free, kRowThreadsTc);
+    mbar_init(&sm.a_ready, kRowThreadsTc);
     sm.abort_flag = 0;
     fence_mbar_init();
+    for (int g = 0; g < min(n, stages); ++g) copy_stage(g);
   }
-  if (warp == kIssueWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem_base)),
-                 "r"(kCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -327,91 +359,99 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait_bounded(bar, parity & 1u, abort_flag, a.status, a.timeout_cycles);
   };
+  // A bounded wait whose outcome is the same on every lane of the warp.
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
   // Read after the roles, by the warps that set them: the last copies and the last commit in flight.
-  int last_g = -1;
+  int last_g = min(n, stages) - 1;
   uint64_t* last_commit = nullptr;
   uint32_t last_parity = 0;
 
-  if (warp < 4) {
-    // ---------------- one row per thread ----------------
-    const uint32_t lane = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const int row = r0 + tid;
-    const long long tile_base = local * c.tiles;
-    const int at = static_cast<int>(2 * tile128 + (tid >> 6));  // this row's 64-row tile
-    load_rows<P>(c.img[kA1] + (tile_base + 2 * tile128) * (2ll * P * kPanelBytes), tid, lane);
-    if constexpr (kScores2)
-      load_rows<P>(c.img[kA2] + (tile_base + 2 * tile128) * (2ll * P * kPanelBytes), tid, lane + kColA2);
-    const int ea1 = c.exps[kA1][tile_base + at];
-    const int ea2 = kScores2 ? c.exps[kA2][tile_base + at] : 0;
-    const float qmul = a.qscale * tc16::pow2(-ea1), unit1 = tc16::pow2(-ea2);
-    float my_off = 0.f, my_delta = 0.f;
-    if constexpr (KIND == kDq) {
-      my_off = c.rows[(tile_base + at) * 128 + (tid & 63)];
-      my_delta = c.rows[(tile_base + at) * 128 + 64 + (tid & 63)];
-    }
-    if (with_grad)
-      for (int b = 0; b < c.t.buckets; ++b) acc[b * 128 + tid] = 0.f;
-    int rlo = 0, rhi = 0;
-    key_range(a, min(row, valid - 1), valid, rlo, rhi);
+  if (warp < 8) {
+    // ---------------- half a row per thread ----------------
+    const uint32_t lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+      tmem_st32(lane + (kScores2 ? half * kColA2 : half * 32 * P) + 32 * p, reinterpret_cast<const float*>(arow[p]));
     tmem_wait_st();
     tc_fence_before();
     mbar_arrive(&sm.a_ready);
 
-    // Where the row's first column finds its distance: j - i relative to the
-    // tile's first distance (kByKey: i runs with the column, so backwards).
-    const int vec_at = kByKey ? tid + 64 : 128 - tid;
+    const int row = r0 + rt;
+    const int ea1 = kByKey ? ae.y : ae.x, ea2 = kByKey ? ae.z : ae.w;
+    const float qmul = a.qscale * tc16::pow2(-ea1), unit1 = tc16::pow2(-ea2);
+    float my_off = 0.f, my_delta = 0.f;
+    if constexpr (KIND == kDq) {
+      const float* mine = c.rows + (tile_base + 2 * tile128 + (rt >> 6)) * 128 + (rt & 63);
+      my_off = mine[0];
+      my_delta = mine[64];
+    }
+    if (with_grad)
+      for (int b = 0; b < c.t.buckets; ++b) acc[b * kRowThreadsTc + tid] = 0.f;
+    int rlo = 0, rhi = 0;
+    key_range(a, min(row, valid - 1), valid, rlo, rhi);
+
+    // Where the thread's first column finds its distance: j - i relative to
+    // the tile's first one (kByKey: i runs with the column, so backwards).
     constexpr int kStep = kByKey ? -1 : 1;
-    float o[64 * P];
+    const int vec_at = (kByKey ? rt + 64 : 128 - rt) + kStep * 32 * half;
+    float o[kOutCols];
 #pragma unroll
-    for (int i = 0; i < 64 * P; ++i) o[i] = 0.f;
+    for (int i = 0; i < kOutCols; ++i) o[i] = 0.f;
     float m_used = -INFINITY, m_true = -INFINITY, lsum = 0.f;
-    bool ok = true;
+    bool ok = true;      // the same on every lane of the warp
     float factor = 0.f;  // of the partial that is in flight
 
     // o += partial of tile g * factor, and the partial's columns are free.
     auto add_partial = [&](int g) {
-      if (__any_sync(0xffffffffu, !wait(&sm.part_full, g))) return false;
+      if (!warp_wait(&sm.part_full, g)) return false;
       tc_fence_after();
       const float2 f2 = make_float2(factor, factor);
 #pragma unroll
       for (int q = 0; q < 2 * P; ++q) {
-        float x[32];
-        tmem_ld32(lane + kColPart + 32 * q, x);
+        float x[16];
+        tc16::tmem_ld16(lane + kColPart + kOutCols * half + 16 * q, x);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float2 r = __ffma2_rn(make_float2(x[i], x[i + 1]), f2, make_float2(o[32 * q + i], o[32 * q + i + 1]));
-          o[32 * q + i] = r.x;
-          o[32 * q + i + 1] = r.y;
+        for (int i = 0; i < 16; i += 2) {
+          const float2 r = __ffma2_rn(make_float2(x[i], x[i + 1]), f2, make_float2(o[16 * q + i], o[16 * q + i + 1]));
+          o[16 * q + i] = r.x;
+          o[16 * q + i + 1] = r.y;
         }
       }
       tc_fence_before();
       mbar_arrive(&sm.part_free);
       return true;
     };
+    // The larger of the row's two values x; false if either thread's warp gave up.
+    auto share_max = [&](int g, float& x) {
+      sm.red[g & 1][half][rt] = x;
+      if (bar_any(kPairBarrier + (warp & 3), 64, !ok)) return false;
+      x = fmaxf(x, sm.red[g & 1][half ^ 1][rt]);
+      return true;
+    };
 
     for (int g = 0; g < n; ++g) {
-      const int st = g % stages, c0 = (t0 + g) * kTileCols;
+      const int st = g % stages, c0 = (t0 + g) * kTileCols + 32 * half;
       const int sb = kScores2 ? 0 : g & 1;
-      const uint32_t sphase = kScores2 ? g : g >> 1;
-      bool w = wait(&sm.full[st], g / stages) && wait(&sm.s_full[sb], sphase);
-      if (__any_sync(0xffffffffu, !w)) { ok = false; break; }
+      if (ok) ok = warp_wait(&sm.full[st], g / stages) && warp_wait(&sm.s_full[sb], kScores2 ? g : g >> 1);
+      if (!kShared && !ok) break;
       tc_fence_after();
-      const uint32_t scol = lane + kColS + 64 * sb;
-      const int e1 = sm.e1[st], e2 = sm.e2[st];
-      const float mult = finite(qmul * tc16::pow2(-e1));
+      const uint32_t scol = lane + kColS + 64 * sb + 32 * half;
+      const int e1 = sm.exps[st][kB1], e2 = sm.exps[st][kB2];
       const int mlo = rlo - c0, mhi = rhi - c0;
-      const bool inside = __all_sync(0xffffffffu, mlo <= 0 && mhi >= 64);
-      const float* vec = &sm.vec[st][vec_at];
-      float s[64];
-      tmem_ld32(scol, s);
-      tmem_ld32(scol + 32, s + 32);
-      mask_scores<BIAS, kStep>(s, mult, vec, mlo, mhi, inside);
+      float s[32];
+      if (ok) {
+        const bool inside = __all_sync(0xffffffffu, mlo <= 0 && mhi >= 32);
+        tmem_ld32(scol, s);
+        mask_scores<BIAS, kStep>(s, finite(qmul * tc16::pow2(-e1)), &sm.vec[st][vec_at], mlo, mhi, inside);
+      }
 
       if constexpr (KIND == kForward) {
         float mx = -INFINITY;
+        if (ok) {
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) mx = fmax3(mx, s[i], s[i + 1]);
+          for (int i = 0; i < 32; i += 2) mx = fmax3(mx, s[i], s[i + 1]);
+        }
+        if (!share_max(g, mx)) { ok = false; break; }
         float alpha = 1.f;
         m_true = fmaxf(m_true, mx);
         if (mx > m_used + kRescale) {
@@ -421,7 +461,7 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
         const float base = (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2;
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
+        for (int i = 0; i < 32; i += 2) {
           s[i] = ex2(s[i] - base);
           s[i + 1] = ex2(s[i + 1] - base);
           sum = __fadd2_rn(sum, make_float2(s[i], s[i + 1]));
@@ -432,17 +472,17 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
         tc_fence_before();
         mbar_arrive(&sm.w_ready[sb]);
         if (g > 0) {
-          if (!add_partial(g - 1)) { ok = false; break; }
-          if (alpha != 1.f) {
+          ok = add_partial(g - 1);
+          if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-            for (int i = 0; i < 64 * P; ++i) o[i] *= alpha;
+            for (int i = 0; i < kOutCols; ++i) o[i] *= alpha;
           }
         }
         factor = tc16::pow2(-e2);
       } else if constexpr (KIND == kDv) {
-        const float* off = sm.rows[st];
+        const float* off = sm.rows[st] + 32 * half;
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
+        for (int i = 0; i < 32; i += 4) {
           const float4 f = *reinterpret_cast<const float4*>(off + i);
           s[i] = ex2(s[i] - f.x + kWeightLog2);
           s[i + 1] = ex2(s[i + 1] - f.y + kWeightLog2);
@@ -453,86 +493,111 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sm.w_ready[sb]);
-        if (g > 0 && !add_partial(g - 1)) { ok = false; break; }
+        if (g > 0) ok = add_partial(g - 1);
         factor = tc16::pow2(-e2) * 6.103515625e-05f;  // 2^-14
       } else {
         // ds = w (dP - delta), then an exponent for the row: its largest |ds| to [2^14, 2^15)
-        const float unit = finite(unit1 * tc16::pow2(-e2));
-        const float* off = sm.rows[st];
         float big = 0.f;
+        if (ok) {
+          const float unit = finite(unit1 * tc16::pow2(-e2));
+          const float* off = sm.rows[st] + 32 * half;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float dp[16];
-          tc16::tmem_ld16(lane + kColS2 + 16 * q, dp);
+          for (int q = 0; q < 2; ++q) {
+            float dp[16];
+            tc16::tmem_ld16(lane + kColS2 + 32 * half + 16 * q, dp);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int k = 16 * q + i;
-            const float p = ex2(s[k] - (KIND == kDk ? off[k] : my_off));
-            s[k] = p * fmaf(dp[i], unit, -(KIND == kDk ? off[64 + k] : my_delta));
+            for (int i = 0; i < 16; ++i) {
+              const int k = 16 * q + i;
+              const float w = ex2(s[k] - (KIND == kDk ? off[k] : my_off));
+              s[k] = w * fmaf(dp[i], unit, -(KIND == kDk ? off[64 + k] : my_delta));
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) big = fmax3(big, fabsf(s[16 * q + i]), fabsf(s[16 * q + i + 1]));
           }
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) big = fmax3(big, fabsf(s[16 * q + i]), fabsf(s[16 * q + i + 1]));
         }
+        if (!share_max(g, big)) { ok = false; break; }
+        const int e = tc16::scale_exp(__float_as_uint(big));
         if (with_grad) {
           // This thread's column of acc: runs of equal buckets along the row.
           const uint8_t* ids = &sm.ids[st][vec_at];
-          const int first = ids[0], last = ids[63];
+          const int first = ids[0], last = ids[31];
           if (__all_sync(0xffffffffu, first == last)) {  // ends equal: one bucket
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) sum += s[i];
-            acc[first * 128 + tid] += sum;
+            for (int i = 0; i < 32; ++i) sum += s[i];
+            acc[first * kRowThreadsTc + tid] += sum;
           } else {
             int cur = first;
             float run = 0.f;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
+            for (int i = 0; i < 32; ++i) {
               const int id = ids[i];
               if (id != cur) {
-                acc[cur * 128 + tid] += run;
+                acc[cur * kRowThreadsTc + tid] += run;
                 run = 0.f;
                 cur = id;
               }
               run += s[i];
             }
-            acc[cur * 128 + tid] += run;
+            acc[cur * kRowThreadsTc + tid] += run;
           }
           __syncwarp();  // the lanes' runs end at different columns
         }
-        const int e = tc16::scale_exp(__float_as_uint(big));
         const float up = tc16::pow2(e);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) s[i] *= up;
+        for (int i = 0; i < 32; ++i) s[i] *= up;
         store_weights(scol, s);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sm.w_ready[sb]);
         factor = finite(tc16::pow2(-e) * tc16::pow2(-e1));
-        if (!add_partial(g)) { ok = false; break; }
+        ok = add_partial(g);
       }
     }
     if constexpr (!kScores2)
       if (ok) ok = add_partial(n - 1);
-    if (ok && row < a.seq) {
-      float* orow = outp + (static_cast<size_t>(bh) * a.seq + row) * d;
-      float f = KIND == kForward ? (lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f) : KIND == kDv ? 1.f : c.t.scale;
+    float f = KIND == kDv ? 1.f : c.t.scale;
+    if constexpr (KIND == kForward) {  // the row's sum: first half + second half
+      sm.red[0][half][rt] = lsum;  // the last exchange is read: part_full follows both threads' w_ready
+      bar_named(kRowBarrier, kRowThreadsTc);
+      lsum = sm.red[0][0][rt] + sm.red[0][1][rt];
+      f = lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f;
+      if (ok && c.t.stats_out && half == 0 && row < a.seq)
+        c.t.stats_out[static_cast<size_t>(bh) * a.seq + row] =
+            row < valid ? make_stats(m_true, (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2, lsum)
+                        : make_float2(-INFINITY, 0.f);
+      __syncwarp();
+    }
+    // The warp's rows through shared memory (the stages are idle: every copy
+    // and product is complete), so that eight lanes store 128 bytes of a row.
+    if (ok) {
+      constexpr int kPitch = 64 * P + 4;  // 16-byte accesses of 8 rows or of one row meet no bank twice
+      static_assert(kTileRows * kPitch * 4 <= 2 * stage_bytes<P>(), "row staging");
+      float* stage = reinterpret_cast<float*>(smem) + (warp & 3) * 32 * kPitch + kOutCols * half;
       const bool live = row < valid;
 #pragma unroll
-      for (int i = 0; i < 64 * P; i += 4)
-        if (i < d) st_stream(orow + i, live ? make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f)
-                                            : make_float4(0.f, 0.f, 0.f, 0.f));
-      if (KIND == kForward && c.t.stats_out)
-        c.t.stats_out[static_cast<size_t>(bh) * a.seq + row] =
-            live ? make_stats(m_true, (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2, lsum)
-                 : make_float2(-INFINITY, 0.f);
+      for (int i = 0; i < kOutCols; i += 4)
+        *reinterpret_cast<float4*>(stage + (tid & 31) * kPitch + i) =
+            live ? make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+      __syncwarp();
+      const int wr0 = r0 + (warp & 3) * 32, wrows = min(32, a.seq - wr0);
+      float* dst = outp + (static_cast<size_t>(bh) * a.seq + wr0) * d + kOutCols * half;
+      constexpr int kLanes = kOutCols / 4;  // lanes of a row
+      const int col = (tid % kLanes) * 4;
+#pragma unroll
+      for (int i = 0; i < kLanes; ++i) {
+        const int r = i * (32 / kLanes) + (tid & 31) / kLanes;
+        if (r < wrows && kOutCols * half + col < d)
+          st_stream(dst + static_cast<size_t>(r) * d + col, *reinterpret_cast<const float4*>(stage + r * kPitch + col));
+      }
     }
     __syncwarp();
     if (with_grad) {
-      // The 128 threads' columns, bucket by bucket, in a fixed order.
-      bar_named(1, 128);
-      for (int b = warp; b < c.t.buckets; b += 4) {
+      // The threads' columns, bucket by bucket, in a fixed order.
+      bar_named(kRowBarrier, kRowThreadsTc);
+      for (int b = warp; b < c.t.buckets; b += 8) {
         float x = 0.f;
-        for (int u = tid & 31; u < 128; u += 32) x += acc[b * 128 + u];
+        for (int u = tid & 31; u < kRowThreadsTc; u += 32) x += acc[b * kRowThreadsTc + u];
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
         if ((tid & 31) == 0) partial[b] = x;
@@ -577,15 +642,15 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
     auto sums = [&](uint32_t wcol, uint32_t b) {
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const uint32_t dcol = tmem + kColPart + 64 * p, bh_ = b + p * kPanelBytes, bl = bh_ + P * kPanelBytes;
+        const uint32_t dcol = tmem + kColPart + 64 * p, bhi = b + p * kPanelBytes, blo = bhi + P * kPanelBytes;
         auto hi_at = [&](int k) { return tmem + wcol + 32 * (k >> 1) + 8 * (k & 1); };
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k), tc16::v_desc(bl, k), k > 0 ? 1u : 0u);
+          tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k), tc16::v_desc(blo, k), k > 0 ? 1u : 0u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k) + 16, tc16::v_desc(bh_, k), 1u);
+        for (int k = 0; k < 4; ++k) tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k) + 16, tc16::v_desc(bhi, k), 1u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k), tc16::v_desc(bh_, k), 1u);
+        for (int k = 0; k < 4; ++k) tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k), tc16::v_desc(bhi, k), 1u);
       }
     };
     if constexpr (kScores2) {
@@ -632,38 +697,12 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
       }
     }
   } else {
-    // ---------------- bulk copies ----------------
-    const int head = static_cast<int>(bh % a.heads);
-    const long long tile_base = local * c.tiles;
-    constexpr uint32_t kOp = 2 * P * kPanelBytes;
-    const bool ids_too = with_grad;
-    const uint32_t bytes = 2 * kOp + (BIAS ? kVec * 4u : 0u) + (kByKey ? 512u : 0u) + (ids_too ? kVec : 0u);
-    int e1s = 0, e2s = 0;
-    for (int g = 0; g < n; ++g) {
-      if ((g & 31) == 0) {  // the exponents of the next 32 tiles, one per lane
-        const int t = min(g + (tid & 31), n - 1) + t0;
-        e1s = c.exps[kB1][tile_base + t];
-        e2s = c.exps[kB2][tile_base + t];
-      }
-      const int e1 = __shfl_sync(0xffffffffu, e1s, g & 31), e2 = __shfl_sync(0xffffffffu, e2s, g & 31);
-      const int st = g % stages;
-      if (g >= stages && !warp_wait(&sm.freed[st], g / stages - 1)) break;
+    // ---------------- bulk copies (the first `stages` are on their way) ----------------
+    for (int g = stages; g < n; ++g) {
+      if (!warp_wait(&sm.freed[g % stages], g / stages - 1)) break;
       if (tc16::lane_is_first(tid)) {
         fence_proxy_async_smem();  // the row threads' reads of this stage, before the copies
-        sm.e1[st] = e1;
-        sm.e2[st] = e2;
-        unsigned char* op = smem + st * stage_bytes<P>();
-        const long long tile = tile_base + t0 + g;
-        mbar_arrive_expect_tx(&sm.full[st], bytes);
-        tma_load_1d(op, c.img[kB1] + tile * static_cast<long long>(kOp), kOp, &sm.full[st]);
-        tma_load_1d(op + kOp, c.img[kB2] + tile * static_cast<long long>(kOp), kOp, &sm.full[st]);
-        const int c0 = (t0 + g) * kTileCols;
-        // The tile's first distance j - i: rows' i from r0, or columns' i from c0.
-        const int rel = kByKey ? r0 - c0 - 64 : c0 - r0 - 128;
-        if constexpr (BIAS)
-          tma_load_1d(sm.vec[st], c.t.rel_bias + (2ll * head + 1) * c.t.rel_half + rel, kVec * 4u, &sm.full[st]);
-        if (ids_too) tma_load_1d(sm.ids[st], c.t.rel_id + c.t.rel_half + rel, kVec, &sm.full[st]);
-        if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * 128, 512u, &sm.full[st]);
+        copy_stage(g);
       }
       last_g = g;
       __syncwarp();
@@ -696,29 +735,16 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* raw) {
   return raw + (((at + 1023u) & ~1023u) - at);
 }
 
-// One CTA per 128-row tile of the chunk's slices.
-template <int P, bool BIAS>
-__global__ void __launch_bounds__(kTcThreads, P == 1 ? 2 : 1) tc_train_fwd(const __grid_constant__ TcArgs c) {
+// One CTA per 128-row tile of the chunk's slices.  A launch per kind: with
+// the three gradients in one grid, CTAs of different kinds on an SM evicted
+// one another's code from the instruction cache (4.0 of 17 stall cycles per
+// instruction were instruction fetch).
+template <int KIND, int P, bool BIAS>
+__global__ void __launch_bounds__(kTcThreads, P == 1 ? 2 : 1) tc_train(const __grid_constant__ TcArgs c) {
   extern __shared__ unsigned char raw[];
   const unsigned tiles = static_cast<unsigned>(c.tiles) / 2, local = blockIdx.x / tiles;
-  run_tile<kForward, P, BIAS>(c, local, static_cast<int>(blockIdx.x - local * tiles), aligned_smem(raw), 0);
-}
-
-// Three CTAs per tile, one for each gradient, next to one another in the
-// grid: they read the same images.
-template <int P, bool BIAS>
-__global__ void __launch_bounds__(kTcThreads, P == 1 ? 2 : 1) tc_train_bwd(const __grid_constant__ TcArgs c) {
-  extern __shared__ unsigned char raw[];
-  const unsigned tiles = static_cast<unsigned>(c.tiles) / 2, unit = blockIdx.x / 3, kind = blockIdx.x - 3 * unit;
-  const unsigned local = unit / tiles;
-  const int tile = static_cast<int>(unit - local * tiles);
-  unsigned char* smem = aligned_smem(raw);
-  if (kind == 0)
-    run_tile<kDq, P, BIAS>(c, local, tile, smem, tile);
-  else if (kind == 1)
-    run_tile<kDk, P, BIAS>(c, local, tile, smem, 0);
-  else
-    run_tile<kDv, P, BIAS>(c, local, tile, smem, 0);
+  const int tile = static_cast<int>(blockIdx.x - local * tiles);
+  run_tile<KIND, P, BIAS>(c, local, tile, aligned_smem(raw), tile);
 }
 
 }  // namespace train

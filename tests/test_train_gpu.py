@@ -113,7 +113,7 @@ CASES = [
     (2, 1, 257, 64, [257, 200], rb.Mask.sliding(0), 128, 0, 0),
     (1, 2, 400, 64, None, rb.Mask.sliding(17), 128, 64, 300),
     (2, 2, 577, 64, [577, 500], rb.Mask.FULL, 128, 32, 128),
-    (1, 1, 600, 64, None, rb.Mask.block(2), 32, 128, 600),
+    (1, 1, 600, 64, None, rb.Mask.block(2), 32, 64, 600),
     (2, 2, 333, 64, [333, 100], OWN, 48, 30, 100),
     (1, 2, 200, 64, None, rb.Mask.block(1), 7, 32, 128),
     (1, 1, 1300, 64, None, BLOCK3, 256, 0, 0),
@@ -124,7 +124,7 @@ CASES = [
     (1, 2, 390, 128, None, BLOCK3, 128, 64, 256),
     (2, 1, 129, 72, [100, 129], rb.Mask.sliding(30), 128, 32, 128),
     (1, 2, 140, 136, None, BLOCK3, 64, 32, 128),
-    (2, 1, 100, 256, [100, 41], rb.Mask.FULL, 128, 128, 4096),
+    (2, 1, 100, 256, [100, 41], rb.Mask.FULL, 128, 64, 4096),
 ]
 
 
