@@ -253,7 +253,7 @@ raya_attn_status ensure_ready(int dev, DeviceCtx** out) {
                     tc_train<train::kDk, 2, false>, tc_train<train::kDk, 2, true>, tc_train<train::kDv, 1, false>,
                     tc_train<train::kDv, 1, true>, tc_train<train::kDv, 2, false>, tc_train<train::kDv, 2, true>}) {
       e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(train::kWholeCta));
+                               static_cast<int>(train::kWholeSm));
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(tc_train smem)");
     }
     c.ready = true;

@@ -75,13 +75,16 @@ struct TrainPlan {
   int tiles = 0;     // 64-row tiles per slice, an even number
   long long chunk = 0;  // slices whose images the workspace holds at a time
   size_t rel_bias = 0, rel_id = 0, delta = 0, part = 0;
-  size_t img[4] = {}, exps = 0, rows = 0;
+  size_t img[4] = {}, exps = 0, rows = 0, next = 0;
+  int far = 0, slots = 0;           // the table's gradient by distance (train_tc.cuh)
+  size_t dist = 0, dist_bytes = 0;  // where it does not fit into shared memory
   size_t bytes = 0;
 };
 
 // The images of one chunk of slices.  They are written and read within the
 // chunk's two launches, so the bound costs launches, not traffic.
 constexpr size_t kMaxImageBytes = size_t{2} << 30;
+constexpr long long kMaxResident = 2 * 148;  // persistent CTAs: two on each SM
 
 raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias, bool backward, TrainPlan* plan) {
   raya_attn_status st = check_shape(d);
@@ -117,6 +120,18 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
     for (int i = 0; i < tensors; ++i) plan->img[i] = take(plan->chunk * image);
     plan->exps = take(plan->chunk * plan->tiles * sizeof(int4));
     if (backward) plan->rows = take(static_cast<size_t>(plan->chunk) * plan->tiles * 128 * sizeof(float));
+    plan->next = take(4 * sizeof(unsigned));
+    if (backward && bias) {
+      // Distances beyond seq do not occur.
+      plan->far = static_cast<int>(std::min<int64_t>(bucket_bounds(bias->buckets, bias->max_distance).at[bias->buckets / 2 - 1], d->seq));
+      plan->slots = 2 * plan->far + 128;
+      const size_t warps = train::kRowWarpsOf(plan->panels), bytes = warps * plan->slots * sizeof(float);
+      const size_t spare = plan->panels == 1 ? train::kHalfSm - train::tc_smem<1>() : train::kWholeSm - train::tc_smem<2>();
+      if (bytes > spare) {
+        plan->dist_bytes = kMaxResident * bytes;
+        plan->dist = take(plan->dist_bytes);
+      }
+    }
   } else {
     // Blocks per slice for about eight blocks on each of the 148 SMs (more
     // leaves warps with a row or two, and more partials).
@@ -169,28 +184,37 @@ raya_attn_status launch_rowwise(const TrainPlan& plan, train::TrainArgs t, void*
 
 // Chunk by chunk: the images of its slices, then every 128-row tile of them.
 template <int P>
-raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, void* workspace, cudaStream_t stream,
-                           bool backward) {
+raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, const train::BucketBounds& bounds,
+                           void* workspace, int sms, cudaStream_t stream, bool backward) {
   train::TcArgs c{};
   c.t = t;
   c.tiles = plan.tiles;
   for (int i = 0; i < (backward ? 4 : 3); ++i) c.img[i] = at<uint8_t>(workspace, plan.img[i]);
   c.exps = at<int4>(workspace, plan.exps);
   if (backward) c.rows = at<float>(workspace, plan.rows);
-  const int acc = t.part ? t.buckets : 0;
-  const size_t most = P == 1 ? train::kHalfSm : train::kWholeCta;
-  c.stages = train::tc_smem<P>(train::kMaxStages, acc) <= most ? train::kMaxStages : 2;
-  size_t smem = train::tc_smem<P>(c.stages, acc);
-  if (P == 1) smem = std::max(smem, train::kThirdSm);  // never three CTAs on an SM
+  c.next = at<unsigned>(workspace, plan.next);
+  const size_t smem = train::tc_smem<P>();
+  size_t dist = 0;
+  if (t.part) {
+    c.bounds = bounds;
+    c.far = plan.far;
+    c.slots = plan.slots;
+    if (plan.dist_bytes > 0)
+      c.dist = at<float>(workspace, plan.dist);
+    else
+      dist = static_cast<size_t>(train::kRowWarpsOf(P)) * plan.slots * sizeof(float);
+  }
+  const long long resident = std::min(kMaxResident, static_cast<long long>(sms) * (P == 1 ? 2 : 1));
   const bool bias = t.rel_bias != nullptr;
   const long long slices = static_cast<long long>(t.a.batch) * t.a.heads;
   for (c.slice0 = 0; c.slice0 < slices; c.slice0 += plan.chunk) {
     const long long n = std::min(plan.chunk, slices - c.slice0) * plan.tiles;
+    c.units = static_cast<unsigned>(n / 2);
     train::split_kernel<P><<<dim3(static_cast<unsigned>(n), backward ? 4 : 3), 256, 0, stream>>>(c);
     raya_attn_status st = check_launch("operand split launch");
     if (st != RAYA_ATTN_OK) return st;
     auto launch_kind = [&](void (*fn)(train::TcArgs), size_t shared, const char* what) {
-      fn<<<static_cast<unsigned>(n / 2), train::kTcThreads, shared, stream>>>(c);
+      fn<<<static_cast<unsigned>(std::min(n / 2, resident)), train::tc_threads(P), shared, stream>>>(c);
       return check_launch(what);
     };
     using train::tc_train;
@@ -199,7 +223,7 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, voi
       if (st != RAYA_ATTN_OK) return st;
       continue;
     }
-    st = launch_kind(bias ? tc_train<train::kDq, P, true> : tc_train<train::kDq, P, false>, smem, "query gradient launch");
+    st = launch_kind(bias ? tc_train<train::kDq, P, true> : tc_train<train::kDq, P, false>, smem + dist, "query gradient launch");
     if (st == RAYA_ATTN_OK)
       st = launch_kind(bias ? tc_train<train::kDk, P, true> : tc_train<train::kDk, P, false>, smem, "key gradient launch");
     if (st == RAYA_ATTN_OK)
@@ -253,7 +277,9 @@ raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const ra
   t.dk = io.dk;
   t.dv = io.dv;
   t.parts = plan.parts;
+  train::BucketBounds bounds{};
   if (bias) {
+    bounds = bucket_bounds(bias->buckets, bias->max_distance);
     t.rel_half = plan.rel_half;
     t.buckets = bias->buckets;
     float* vec = at<float>(workspace, plan.rel_bias);
@@ -263,14 +289,13 @@ raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const ra
     const dim3 blocks(static_cast<unsigned>(std::min<long long>((2ll * plan.rel_half + 255) / 256, 1024)),
                       static_cast<unsigned>(std::min<int64_t>(d->heads, 64)));
     train::rel_table_kernel<<<blocks, 256, 0, stream>>>(bias->table, static_cast<int>(d->heads), bias->buckets,
-                                                        plan.rel_half, bucket_bounds(bias->buckets, bias->max_distance),
-                                                        vec, ids);
+                                                        plan.rel_half, bounds, vec, ids);
     if ((st = check_launch("bias table launch")) != RAYA_ATTN_OK) return st;
   }
   if (io.dtable) t.part = at<float>(workspace, plan.part);
   if (plan.panels > 0)
-    st = plan.panels == 1 ? launch_tc<1>(plan, t, workspace, stream, backward)
-                          : launch_tc<2>(plan, t, workspace, stream, backward);
+    st = plan.panels == 1 ? launch_tc<1>(plan, t, bounds, workspace, ctx->sms, stream, backward)
+                          : launch_tc<2>(plan, t, bounds, workspace, ctx->sms, stream, backward);
   else
     st = launch_rowwise(plan, t, workspace, stream, backward);
   if (st != RAYA_ATTN_OK) return st;

@@ -68,11 +68,17 @@ namespace raya {
 namespace train {
 
 constexpr int kTileRows = 128, kTileCols = 64;
-constexpr int kTcThreads = 320;
-constexpr int kRowThreadsTc = 256;
-constexpr int kIssueWarp = 8, kCopyWarp = 9;
+// Threads per row: one where two CTAs share an SM, two where one has it alone.
+constexpr int kRowWarpsOf(int panels) { return 4 * panels; }
+constexpr int tc_threads(int panels) { return 128 * panels + 128; }
+// Registers (setmaxnreg): a row thread holds a row of scores next to a row of
+// the output.  The shares add up to what the launch gives its threads: 256
+// threads of 128 registers (two CTAs per SM), 384 of 168.
+constexpr int row_regs(int panels) { return panels == 1 ? 200 : 216; }
+constexpr int other_regs(int panels) { return panels == 1 ? 56 : 72; }
+static_assert(row_regs(1) + other_regs(1) <= 2 * 128 && 2 * row_regs(2) + other_regs(2) <= 3 * 168, "register shares");
 constexpr int kPairBarrier = 1, kRowBarrier = 5;  // named barriers: 1-4 the warps of the same rows, 5 all row warps
-constexpr int kMaxStages = 3;
+constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
 constexpr float kWeightLog2 = 14.f;                // kDv: w enters as w * 2^14, so that small ones keep their bits
@@ -91,7 +97,12 @@ struct TcArgs {
   float* rows;         // [chunk slices][tiles][2][64]: m * log2(e) (inf: no key), and delta / l
   int tiles;           // 64-row tiles per slice (even)
   long long slice0;
-  int stages;
+  unsigned units;      // 128-row tiles of the chunk
+  unsigned* next;      // [4] by kind: units handed out beyond the first one of each CTA; split_kernel clears them
+  BucketBounds bounds; // with t.part, and the rest of the table's gradient:
+  int far;             // the last bucket's first distance
+  int slots;           // distances kept apart: -far - 63 ... far + 64
+  float* dist;         // [CTAs][row warps][slots] where shared memory does not hold them, or nullptr
 };
 
 __device__ __forceinline__ int valid_of(const AttnArgs& a, long long bh) {
@@ -110,6 +121,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   const int tid = threadIdx.x, which = blockIdx.y, d = a.head_dim;
   const long long local = blockIdx.x / static_cast<unsigned>(c.tiles), bh = c.slice0 + local;
   const int tile = static_cast<int>(blockIdx.x - local * c.tiles);
+  if (blockIdx.x == 0 && which == 0 && tid < 4) c.next[tid] = 0;
   const int valid = valid_of(a, bh);
   const int r0 = tile * 64;
   if (r0 >= (valid + 127) / 128 * 128) return;  // no 128-row tile reads it
@@ -182,14 +194,23 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   }
 }
 
+// One unit of work: a 128-row tile of one slice.
+struct TcUnit {
+  int local;   // slice within the chunk
+  int valid, r0;
+  int t0, n;   // 64-column tiles [t0, t0 + n) that its rows see; n = 0: padding only, -1: no more units
+};
+
 // Shared memory behind the operand stages.
-struct TcTail {
-  float vec[kMaxStages][kVec];       // bias * log2(e) by distance
-  float rows[kMaxStages][2 * 64];    // kDk, kDv: the columns' exponent and delta
-  uint8_t ids[kMaxStages][kVec];     // kDq: buckets by distance
-  int exps[kMaxStages][4];           // exponents of the columns' 64 rows, by tensor
-  float red[2][2][kTileRows];        // [tile parity][half]: what a row's threads exchange
-  uint64_t full[kMaxStages], freed[kMaxStages];
+constexpr int kQueue = 2;
+struct alignas(16) TcTail {
+  float vec[kStages][kVec];       // bias * log2(e) by distance
+  float rows[kStages][2 * 64];    // kDk, kDv: the columns' exponent and delta
+  int exps[kStages][4];           // exponents of the columns' 64 rows, by tensor
+  float red[2][2][kTileRows];     // [tile parity][half]: what a row's threads exchange
+  TcUnit unit[kQueue];            // the units that the copy warp has begun
+  uint64_t u_full[kQueue], u_free[kQueue];
+  uint64_t full[kStages], freed[kStages];
   uint64_t s_full[2], w_ready[2], part_full, part_free, a_ready;
   uint32_t tmem_base;
   int abort_flag;
@@ -197,64 +218,121 @@ struct TcTail {
 
 template <int P>
 constexpr size_t stage_bytes() { return 2ull * 2 * P * kPanelBytes; }
+// Each row warp's 32 x 32 words: rows on their way between global memory and
+// the threads.  The pitch lets 8 lanes access 16 bytes of 8 rows, or of one,
+// without a bank conflict.
+constexpr int kPitch = 36;
 template <int P>
-constexpr size_t tc_smem(int stages, int buckets) {
-  return 1024 + stages * stage_bytes<P>() + sizeof(TcTail) + static_cast<size_t>(buckets) * kRowThreadsTc * sizeof(float);
+constexpr size_t tc_smem() {
+  return 1024 + kStages * stage_bytes<P>() + sizeof(TcTail) + kRowWarpsOf(P) * 32 * kPitch * sizeof(float);
 }
-// head_dim <= 64: at most half of an SM's shared memory, and more than a
-// third, so that exactly two CTAs (2 x 256 tensor-memory columns) share it.
-constexpr size_t kHalfSm = (233472 - 2 * 1024) / 2, kWholeCta = 232448;
-constexpr size_t kThirdSm = 233472 / 3;
-static_assert(tc_smem<1>(3, 0) <= kHalfSm, "two CTAs per SM");
-static_assert(tc_smem<1>(2, kMaxBuckets) <= kWholeCta && tc_smem<2>(2, kMaxBuckets) <= kWholeCta, "shared memory of a block");
+// head_dim <= 64: two CTAs (2 x 256 tensor-memory columns) share an SM and a
+// third does not fit beside them.
+constexpr size_t kHalfSm = (233472 - 2 * 1024) / 2, kWholeSm = 232448;
+static_assert(tc_smem<1>() <= kHalfSm && tc_smem<1>() > 233472 / 3 && tc_smem<2>() <= kWholeSm, "CTAs per SM");
 
 // A product of scales that would be infinite, as the largest float: 0 times it is 0.
 __device__ __forceinline__ float finite(float x) { return fmaxf(fminf(x, 3.4028235e38f), -3.4028235e38f); }
 
-// 128 bytes of an operand's row r (64 fp16 of one panel) as 32 words, from
-// its image.  Straight from global memory: each row is read once, a whole
-// line per panel and half.
-__device__ __forceinline__ void load_row(const uint8_t* panel, int r, uint32_t* w) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint4 x = *reinterpret_cast<const uint4*>(panel + tc16::op_off(r, k));
-    w[4 * k] = x.x;
-    w[4 * k + 1] = x.y;
-    w[4 * k + 2] = x.z;
-    w[4 * k + 3] = x.w;
-  }
-}
-
-// Weights w[32] (fp32, already scaled) as fp16 hi and lo over their scores.
+// Weights w[N] (fp32, already scaled) as fp16 hi and lo over their scores.
+template <int N>
 __device__ __forceinline__ void store_weights(uint32_t taddr, const float* w) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
+  for (int s = 0; s < N / 16; ++s) {
     uint32_t h[8], l[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) tc16::split2(w[16 * s + 2 * k], w[16 * s + 2 * k + 1], h[k], l[k]);
-    tc16::tmem_st8u(taddr + 8 * s, h);
-    tc16::tmem_st8u(taddr + 8 * s + 16, l);
+    tc16::tmem_st8u(taddr + 32 * (s >> 1) + 8 * (s & 1), h);
+    tc16::tmem_st8u(taddr + 32 * (s >> 1) + 8 * (s & 1) + 16, l);
   }
 }
 
-// 32 scores in place: s * mult (+ bias), -inf outside [lo, hi).
-template <bool BIAS, int STEP>
+// N scores in place: s * mult (+ bias), -inf outside [lo, hi).
+template <int N, bool BIAS, int STEP>
 __device__ __forceinline__ void mask_scores(float* s, float mult, const float* vec, int lo, int hi, bool inside) {
+  const float2 m2 = make_float2(mult, mult);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i] = BIAS ? fmaf(s[i], mult, vec[STEP * i]) : s[i] * mult;
+  for (int q = 0; q < N; q += 16) {  // 16 loads in flight
+    float2 b[8];
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = make_float2(vec[STEP * (q + 2 * i)], vec[STEP * (q + 2 * i + 1)]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 x = make_float2(s[q + 2 * i], s[q + 2 * i + 1]);
+      const float2 y = BIAS ? __ffma2_rn(x, m2, b[i]) : __fmul2_rn(x, m2);
+      s[q + 2 * i] = y.x;
+      s[q + 2 * i + 1] = y.y;
+    }
+  }
   if (!inside) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < N; ++i)
       if (i < lo || i >= hi) s[i] = -INFINITY;
   }
 }
 
+// 32 x 32 words between rows and lanes: the warp's 32 rows of 128 bytes at
+// `src` (swizzled within each 8 rows) into this lane's row w[32], through the
+// warp's buffer.  Eight lanes load a row's line.
+__device__ __forceinline__ void gather_rows(const uint8_t* src, uint4* x, int lane) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(src + (4 * i + (lane >> 3)) * 128 + (lane & 7) * 16);
+}
+__device__ __forceinline__ void turn_rows(float* buf, const uint4* x, int lane, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    *reinterpret_cast<uint4*>(buf + r * kPitch + (((lane & 7) ^ (r & 7)) << 2)) = x[i];
+  }
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint4 y = *reinterpret_cast<const uint4*>(buf + lane * kPitch + 4 * k);
+    w[4 * k] = y.x;
+    w[4 * k + 1] = y.y;
+    w[4 * k + 2] = y.z;
+    w[4 * k + 3] = y.w;
+  }
+  __syncwarp();
+}
+
+// The sums along the diagonals of a 32 x 32 block whose row `lane` is s[32]:
+// before is the sum of column - row = lane - 31, after that of lane + 1.
+// Lane k reads column (k + 1 + row) mod 32 of every row: no bank conflict.
+__device__ __forceinline__ void diagonal_sums(float* buf, const float* s, int lane, float& before, float& after) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4)
+    *reinterpret_cast<float4*>(buf + lane * kPitch + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+  __syncwarp();
+  before = after = 0.f;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) {
+    const bool wrapped = lane >= 31 - r;
+    const float x = buf[r * (kPitch + 1) + lane + 1 - (wrapped ? 32 : 0)];
+    if (wrapped)
+      before += x;
+    else
+      after += x;
+  }
+  __syncwarp();
+}
+
+// Persistent: the copy warp takes one unit after the other (the first by
+// blockIdx, the others from a counter, since padding makes them uneven) and
+// hands them to the other warps.  Every barrier and ring runs on across them:
+// G counts the CTA's 64-column tiles, U its units with any.
 template <int KIND, int P, bool BIAS>
-__device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned char* smem, int part_index) {
+__global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const __grid_constant__ TcArgs c) {
   using namespace tc32;
   constexpr bool kScores2 = KIND == kDq || KIND == kDk;      // S and dP, serial
   constexpr bool kByKey = KIND == kDk || KIND == kDv;        // rows are keys, columns queries
-  constexpr bool kShared = KIND != kDv;                      // a row's threads share a maximum
+  constexpr int kHalves = P;                                 // threads per row
+  constexpr int kW = 64 / kHalves;                           // score columns of a thread
+  constexpr bool kShared = KIND != kDv && kHalves == 2;      // a row's threads share a maximum
+  constexpr int kRowThreadsTc = 128 * kHalves;
+  constexpr int kIssueWarp = kRowWarpsOf(P);                 // and the copy warp behind it; two more idle
   constexpr uint32_t kCols = 256 * P;
   constexpr uint32_t kColA2 = 64 * P;
   constexpr uint32_t kColS = kScores2 ? 128 * P : 64 * P;
@@ -264,78 +342,19 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
   constexpr int kB1 = kByKey ? kImgQ : kImgK, kB2 = kByKey ? kImgG : kImgV;  // the columns' operands
   constexpr int kA1 = kByKey ? kImgK : kImgQ, kA2 = kByKey ? kImgV : kImgG;  // the rows'
   constexpr uint32_t kOp = 2 * P * kPanelBytes;
-  constexpr int kOutCols = 32 * P;                           // output columns of a thread
+  constexpr int kOutCols = kW * P;                           // output columns of a thread
+
+  extern __shared__ unsigned char raw[];
+  unsigned char* const smem = raw + (((smem_addr(raw) + 1023u) & ~1023u) - smem_addr(raw));
+  TcTail& sm = *reinterpret_cast<TcTail*>(smem + kStages * stage_bytes<P>());
+  float* const row_bufs = reinterpret_cast<float*>(&sm + 1);
 
   const AttnArgs& a = c.t.a;
-  const int tid = threadIdx.x, warp = tid >> 5;
-  const long long bh = c.slice0 + local;
-  const int valid = valid_of(a, bh);
-  const int r0 = tile128 * kTileRows, d = a.head_dim;
-  float* outp = KIND == kForward ? a.out : KIND == kDq ? c.t.dq : KIND == kDk ? c.t.dk : c.t.dv;
+  const int tid = threadIdx.x, warp = tid >> 5, d = a.head_dim;
   const bool with_grad = KIND == kDq && c.t.part != nullptr;
-  float* partial = with_grad ? c.t.part + (static_cast<size_t>(bh) * c.t.parts + part_index) * c.t.buckets : nullptr;
 
-  int lo = 0, hi = 0, unused;
-  if (r0 < valid) {
-    key_range(a, r0, valid, lo, unused);
-    key_range(a, min(r0 + kTileRows, valid) - 1, valid, unused, hi);
-  }
-  const int t0 = lo / kTileCols, n = hi > lo ? (hi + kTileCols - 1) / kTileCols - t0 : 0;
-  if (n == 0) {  // padding only
-    const int rows = min(kTileRows, a.seq - r0);
-    float* o = outp + (static_cast<size_t>(bh) * a.seq + r0) * d;
-    for (int i = tid; i < rows * d / 4; i += kTcThreads) st_stream(o + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f));
-    if (KIND == kForward && c.t.stats_out && tid < rows)
-      c.t.stats_out[static_cast<size_t>(bh) * a.seq + r0 + tid] = make_float2(-INFINITY, 0.f);
-    if (with_grad && tid < c.t.buckets) partial[tid] = 0.f;
-    return;
-  }
-
-  TcTail& sm = *reinterpret_cast<TcTail*>(smem + c.stages * stage_bytes<P>());
-  float* acc = reinterpret_cast<float*>(&sm + 1);  // with_grad: [buckets][kRowThreadsTc]
-  const int stages = c.stages;
-  const long long tile_base = local * c.tiles;
-
-  // Copies the operands and values of step g into its stage (one lane).
-  auto copy_stage = [&](int g) {
-    const int st = g % stages, c0 = (t0 + g) * kTileCols;
-    const long long tile = tile_base + t0 + g;
-    const int head = static_cast<int>(bh % a.heads);
-    // The tile's first distance j - i: rows' i from r0, or columns' i from c0.
-    const int rel = kByKey ? r0 - c0 - 64 : c0 - r0 - 128;
-    unsigned char* op = smem + st * stage_bytes<P>();
-    mbar_arrive_expect_tx(&sm.full[st], 2 * kOp + 16u + (BIAS ? kVec * 4u : 0u) + (kByKey ? 512u : 0u) +
-                                            (with_grad ? kVec : 0u));
-    tma_load_1d(op, c.img[kB1] + tile * static_cast<long long>(kOp), kOp, &sm.full[st]);
-    tma_load_1d(op + kOp, c.img[kB2] + tile * static_cast<long long>(kOp), kOp, &sm.full[st]);
-    tma_load_1d(sm.exps[st], c.exps + tile, 16u, &sm.full[st]);
-    if constexpr (BIAS)
-      tma_load_1d(sm.vec[st], c.t.rel_bias + (2ll * head + 1) * c.t.rel_half + rel, kVec * 4u, &sm.full[st]);
-    if (with_grad) tma_load_1d(sm.ids[st], c.t.rel_id + c.t.rel_half + rel, kVec, &sm.full[st]);
-    if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * 128, 512u, &sm.full[st]);
-  };
-
-  // Before the CTA's first barrier: the copy warp fills the stages, the
-  // issuing warp takes tensor memory, and the row threads load their rows
-  // (first halves of the row threads: the first operand, or its hi parts).
-  constexpr int kParts = kScores2 ? 2 * P : P;  // 32-word pieces of this thread
-  uint32_t arow[kParts][32];
-  const int half = warp >> 2, rt = tid & 127;
-  int4 ae = make_int4(0, 0, 0, 0);
-  if (warp < 8) {
-    const int which = kScores2 && half ? kA2 : kA1;
-    const uint8_t* img = c.img[which] + (tile_base + 2 * tile128 + (rt >> 6)) * static_cast<long long>(kOp) +
-                         (kScores2 ? 0 : half * P * kPanelBytes);
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) load_row(img + p * kPanelBytes, rt & 63, arow[p]);
-    ae = c.exps[tile_base + 2 * tile128 + (rt >> 6)];
-  } else if (warp == kIssueWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem_base)),
-                 "r"(kCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else if (tc16::lane_is_first(tid)) {
-    for (int s = 0; s < kMaxStages; ++s) {
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.freed[s], 1);
     }
@@ -346,9 +365,18 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
     mbar_init(&sm.part_full, 1);
     mbar_init(&sm.part_free, kRowThreadsTc);
     mbar_init(&sm.a_ready, kRowThreadsTc);
+    for (int s = 0; s < kQueue; ++s) {
+      mbar_init(&sm.u_full[s], 1);
+      mbar_init(&sm.u_free[s], kIssueWarp + 1);
+    }
     sm.abort_flag = 0;
     fence_mbar_init();
-    for (int g = 0; g < min(n, stages); ++g) copy_stage(g);
+  }
+  if (warp == kIssueWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem_base)),
+                 "r"(kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   __syncwarp();
   tc_fence_before();
@@ -361,252 +389,365 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
   };
   // A bounded wait whose outcome is the same on every lane of the warp.
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
-  // Read after the roles, by the warps that set them: the last copies and the last commit in flight.
-  int last_g = min(n, stages) - 1;
+  // Read after the roles, by the warps that set them: the tiles copied and the products committed.
+  int copied = 0, committed = 0;
   uint64_t* last_commit = nullptr;
   uint32_t last_parity = 0;
 
-  if (warp < 8) {
-    // ---------------- half a row per thread ----------------
+  // The consumers' next unit (n = -1 after the last one, or a timeout).
+  int queued = 0;
+  auto take_unit = [&](TcUnit& u) {
+    const int s = queued % kQueue;
+    const bool got = warp_wait(&sm.u_full[s], queued / kQueue);
+    u = sm.unit[s];
+    if (!got) u.n = -1;
+    __syncwarp();
+    if ((tid & 31) == 0) mbar_arrive(&sm.u_free[s]);
+    ++queued;
+    return got;
+  };
+
+  if (warp < kIssueWarp)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(row_regs(P)));
+  else
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs(P)));
+  if (warp < kIssueWarp) {
+    // ---------------- rows ----------------
+    const int half = warp >> 2, rt = tid & 127, ln = tid & 31;
+    float* const buf = row_bufs + warp * 32 * kPitch;
     const uint32_t lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-#pragma unroll
-    for (int p = 0; p < kParts; ++p)
-      tmem_st32(lane + (kScores2 ? half * kColA2 : half * 32 * P) + 32 * p, reinterpret_cast<const float*>(arow[p]));
-    tmem_wait_st();
-    tc_fence_before();
-    mbar_arrive(&sm.a_ready);
-
-    const int row = r0 + rt;
-    const int ea1 = kByKey ? ae.y : ae.x, ea2 = kByKey ? ae.z : ae.w;
-    const float qmul = a.qscale * tc16::pow2(-ea1), unit1 = tc16::pow2(-ea2);
-    float my_off = 0.f, my_delta = 0.f;
-    if constexpr (KIND == kDq) {
-      const float* mine = c.rows + (tile_base + 2 * tile128 + (rt >> 6)) * 128 + (rt & 63);
-      my_off = mine[0];
-      my_delta = mine[64];
-    }
-    if (with_grad)
-      for (int b = 0; b < c.t.buckets; ++b) acc[b * kRowThreadsTc + tid] = 0.f;
-    int rlo = 0, rhi = 0;
-    key_range(a, min(row, valid - 1), valid, rlo, rhi);
-
+    float* const outp = KIND == kForward ? a.out : KIND == kDq ? c.t.dq : KIND == kDk ? c.t.dk : c.t.dv;
+    constexpr int kStep = kByKey ? -1 : 1;
     // Where the thread's first column finds its distance: j - i relative to
     // the tile's first one (kByKey: i runs with the column, so backwards).
-    constexpr int kStep = kByKey ? -1 : 1;
-    const int vec_at = (kByKey ? rt + 64 : 128 - rt) + kStep * 32 * half;
-    float o[kOutCols];
-#pragma unroll
-    for (int i = 0; i < kOutCols; ++i) o[i] = 0.f;
-    float m_used = -INFINITY, m_true = -INFINITY, lsum = 0.f;
-    bool ok = true;      // the same on every lane of the warp
-    float factor = 0.f;  // of the partial that is in flight
+    const int vec_at = (kByKey ? rt + 64 : 128 - rt) + kStep * kW * half;
 
-    // o += partial of tile g * factor, and the partial's columns are free.
-    auto add_partial = [&](int g) {
-      if (!warp_wait(&sm.part_full, g)) return false;
-      tc_fence_after();
-      const float2 f2 = make_float2(factor, factor);
+    // The next unit with columns; the rows of those without are padding and
+    // get their zeros on the way.
+    auto next_unit = [&](TcUnit& u) {
+      for (;;) {
+        if (!take_unit(u)) return false;
+        if (u.n != 0) return true;
+        const int rows = min(kTileRows, a.seq - u.r0);
+        const size_t first = static_cast<size_t>(c.slice0 + u.local) * a.seq + u.r0;
+        float* o = outp + first * d;
+        for (int i = tid; i < rows * d / 4; i += kRowThreadsTc) st_stream(o + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f));
+        if (KIND == kForward && c.t.stats_out && tid < rows) c.t.stats_out[first + tid] = make_float2(-INFINITY, 0.f);
+        if (with_grad && tid < c.t.buckets)
+          c.t.part[(static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets + tid] = 0.f;
+        __syncwarp();
+      }
+    };
+    // What a row needs besides its operands: 2^-e of these, the columns that
+    // it sees, and for kDq its exponent and delta.
+    struct Row {
+      float qmul, unit, off, delta;
+      int lo, hi;
+    };
+    // Unit u's rows into tensor memory.  Called while the last tile of the
+    // unit before is in its second product: its scores are complete.
+    auto load_rows = [&](const TcUnit& u, Row& r) {
+      const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64 + ((warp & 3) >> 1);
+      const int4 e = c.exps[tile];
+      constexpr int kParts = (kScores2 ? 4 : 2) * P / kHalves;  // 32-word pieces of this thread
 #pragma unroll
-      for (int q = 0; q < 2 * P; ++q) {
-        float x[16];
-        tc16::tmem_ld16(lane + kColPart + kOutCols * half + 16 * q, x);
+      for (int p0 = 0; p0 < kParts; p0 += 2) {  // two in flight
+        uint4 x[2][8];
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float2 r = __ffma2_rn(make_float2(x[i], x[i + 1]), f2, make_float2(o[16 * q + i], o[16 * q + i + 1]));
-          o[16 * q + i] = r.x;
-          o[16 * q + i + 1] = r.y;
+        for (int p = 0; p < 2; ++p) {
+          const int piece = half * kParts + p0 + p;  // hi and lo panels of the first operand, then of the second
+          gather_rows(c.img[piece < 2 * P ? kA1 : kA2] + tile * static_cast<long long>(kOp) +
+                          piece % (2 * P) * kPanelBytes + (warp & 1) * 32 * 128, x[p], ln);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          uint32_t w[32];
+          turn_rows(buf, x[p], ln, w);
+          tmem_st32(lane + 32 * (half * kParts + p0 + p), reinterpret_cast<const float*>(w));
         }
       }
+      r.qmul = a.qscale * tc16::pow2(-(kByKey ? e.y : e.x));
+      r.unit = kScores2 ? tc16::pow2(-(kByKey ? e.z : e.w)) : 0.f;
+      r.off = r.delta = 0.f;
+      if constexpr (KIND == kDq) {
+        r.off = c.rows[tile * 128 + (rt & 63)];
+        r.delta = c.rows[tile * 128 + 64 + (rt & 63)];
+      }
+      key_range(a, min(u.r0 + rt, u.valid - 1), u.valid, r.lo, r.hi);
+      tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&sm.part_free);
-      return true;
-    };
-    // The larger of the row's two values x; false if either thread's warp gave up.
-    auto share_max = [&](int g, float& x) {
-      sm.red[g & 1][half][rt] = x;
-      if (bar_any(kPairBarrier + (warp & 3), 64, !ok)) return false;
-      x = fmaxf(x, sm.red[g & 1][half ^ 1][rt]);
-      return true;
+      mbar_arrive(&sm.a_ready);
     };
 
-    for (int g = 0; g < n; ++g) {
-      const int st = g % stages, c0 = (t0 + g) * kTileCols + 32 * half;
-      const int sb = kScores2 ? 0 : g & 1;
-      if (ok) ok = warp_wait(&sm.full[st], g / stages) && warp_wait(&sm.s_full[sb], kScores2 ? g : g >> 1);
-      if (!kShared && !ok) break;
-      tc_fence_after();
-      const uint32_t scol = lane + kColS + 64 * sb + 32 * half;
-      const int e1 = sm.exps[st][kB1], e2 = sm.exps[st][kB2];
-      const int mlo = rlo - c0, mhi = rhi - c0;
-      float s[32];
-      if (ok) {
-        const bool inside = __all_sync(0xffffffffu, mlo <= 0 && mhi >= 32);
-        tmem_ld32(scol, s);
-        mask_scores<BIAS, kStep>(s, finite(qmul * tc16::pow2(-e1)), &sm.vec[st][vec_at], mlo, mhi, inside);
+    TcUnit u, nu;
+    Row r, nr;
+    int G = 0;
+    bool ok = true;  // the same on every lane of the warp
+    // The table's gradient: this warp's sums by distance, and of what lies
+    // beyond the last bucket's bound on either side.
+    float* const dist = !with_grad ? nullptr
+                        : c.dist   ? c.dist + (static_cast<size_t>(blockIdx.x) * kIssueWarp + warp) * c.slots
+                                   : row_bufs + kIssueWarp * 32 * kPitch + warp * c.slots;
+    ok = next_unit(u);
+    if (u.n > 0) load_rows(u, r);
+    while (ok && u.n > 0) {
+      const int row = u.r0 + rt;
+      const size_t first_row = static_cast<size_t>(c.slice0 + u.local) * a.seq + u.r0;
+      float far_before = 0.f, far_after = 0.f;
+      float o[kOutCols];
+#pragma unroll
+      for (int i = 0; i < kOutCols; ++i) o[i] = 0.f;
+      float m_used = -INFINITY, m_true = -INFINITY, lsum = 0.f;
+      float factor = 0.f;  // of the partial that is in flight
+      if (with_grad) {
+        for (int i = ln; i < c.slots; i += 32) dist[i] = 0.f;
+        __syncwarp();
       }
 
-      if constexpr (KIND == kForward) {
-        float mx = -INFINITY;
-        if (ok) {
+      // o += partial of tile g * factor, and the partial's columns are free.
+      auto add_partial = [&](int g) {
+        if (!warp_wait(&sm.part_full, g)) return false;
+        tc_fence_after();
+        const float2 f2 = make_float2(factor, factor);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) mx = fmax3(mx, s[i], s[i + 1]);
-        }
-        if (!share_max(g, mx)) { ok = false; break; }
-        float alpha = 1.f;
-        m_true = fmaxf(m_true, mx);
-        if (mx > m_used + kRescale) {
-          alpha = ex2(m_used - mx);
-          m_used = mx;
-        }
-        const float base = (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2;
-        float2 sum = make_float2(0.f, 0.f);
+        for (int q = 0; q < kOutCols / 16; ++q) {
+          float x[16];
+          tc16::tmem_ld16(lane + kColPart + kOutCols * half + 16 * q, x);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          s[i] = ex2(s[i] - base);
-          s[i + 1] = ex2(s[i + 1] - base);
-          sum = __fadd2_rn(sum, make_float2(s[i], s[i + 1]));
-        }
-        lsum = fmaf(lsum, alpha, sum.x + sum.y);
-        store_weights(scol, s);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&sm.w_ready[sb]);
-        if (g > 0) {
-          ok = add_partial(g - 1);
-          if (__any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < kOutCols; ++i) o[i] *= alpha;
+          for (int i = 0; i < 16; i += 2) {
+            const float2 y = __ffma2_rn(make_float2(x[i], x[i + 1]), f2, make_float2(o[16 * q + i], o[16 * q + i + 1]));
+            o[16 * q + i] = y.x;
+            o[16 * q + i + 1] = y.y;
           }
         }
-        factor = tc16::pow2(-e2);
-      } else if constexpr (KIND == kDv) {
-        const float* off = sm.rows[st] + 32 * half;
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(off + i);
-          s[i] = ex2(s[i] - f.x + kWeightLog2);
-          s[i + 1] = ex2(s[i + 1] - f.y + kWeightLog2);
-          s[i + 2] = ex2(s[i + 2] - f.z + kWeightLog2);
-          s[i + 3] = ex2(s[i + 3] - f.w + kWeightLog2);
-        }
-        store_weights(scol, s);
-        tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&sm.w_ready[sb]);
-        if (g > 0) ok = add_partial(g - 1);
-        factor = tc16::pow2(-e2) * 6.103515625e-05f;  // 2^-14
-      } else {
-        // ds = w (dP - delta), then an exponent for the row: its largest |ds| to [2^14, 2^15)
-        float big = 0.f;
+        mbar_arrive(&sm.part_free);
+        return true;
+      };
+      // The larger of the row's two values x; false if either thread's warp gave up.
+      auto share_max = [&](int g, float& x) {
+        if constexpr (kHalves == 1) return ok;
+        sm.red[g & 1][half][rt] = x;
+        if (bar_any(kPairBarrier + (warp & 3), 64, !ok)) return false;
+        x = fmaxf(x, sm.red[g & 1][half ^ 1][rt]);
+        return true;
+      };
+      nu.n = -1;
+      // After the last tile's scores: the next unit's rows.
+      auto prepare_next = [&](int t) {
+        if (t + 1 < u.n) return;
+        if (next_unit(nu) && nu.n > 0) load_rows(nu, nr);
+      };
+
+      for (int t = 0; t < u.n; ++t, ++G) {
+        const int st = G % kStages, c0 = (u.t0 + t) * kTileCols + kW * half;
+        const int sb = kScores2 ? 0 : G & 1;
+        if (ok) ok = warp_wait(&sm.full[st], G / kStages) && warp_wait(&sm.s_full[sb], kScores2 ? G : G >> 1);
+        if (!kShared && !ok) break;
+        tc_fence_after();
+        const uint32_t scol = lane + kColS + 64 * sb + kW * half;
+        const int e1 = sm.exps[st][kB1], e2 = sm.exps[st][kB2];
+        const int mlo = r.lo - c0, mhi = r.hi - c0;
+        float s[kW];
         if (ok) {
-          const float unit = finite(unit1 * tc16::pow2(-e2));
-          const float* off = sm.rows[st] + 32 * half;
+          const bool inside = __all_sync(0xffffffffu, mlo <= 0 && mhi >= kW);
+          tmem_ld32(scol, s);
+          if constexpr (kW == 64) tmem_ld32(scol + 32, s + 32);
+          mask_scores<kW, BIAS, kStep>(s, finite(r.qmul * tc16::pow2(-e1)), &sm.vec[st][vec_at], mlo, mhi, inside);
+        }
+
+        if constexpr (KIND == kForward) {
+          float mx = -INFINITY;
+          if (ok) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float dp[16];
-            tc16::tmem_ld16(lane + kColS2 + 32 * half + 16 * q, dp);
+            for (int i = 0; i < kW; i += 2) mx = fmax3(mx, s[i], s[i + 1]);
+          }
+          if (!share_max(G, mx)) { ok = false; break; }
+          float alpha = 1.f;
+          m_true = fmaxf(m_true, mx);
+          if (mx > m_used + kRescale) {
+            alpha = ex2(m_used - mx);
+            m_used = mx;
+          }
+          const float base = (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2;
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int k = 16 * q + i;
-              const float w = ex2(s[k] - (KIND == kDk ? off[k] : my_off));
-              s[k] = w * fmaf(dp[i], unit, -(KIND == kDk ? off[64 + k] : my_delta));
+          for (int i = 0; i < kW; i += 2) {
+            s[i] = ex2(s[i] - base);
+            s[i + 1] = ex2(s[i + 1] - base);
+            sum = __fadd2_rn(sum, make_float2(s[i], s[i + 1]));
+          }
+          lsum = fmaf(lsum, alpha, sum.x + sum.y);
+          store_weights<kW>(scol, s);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&sm.w_ready[sb]);
+          if (t > 0) {
+            ok = add_partial(G - 1);
+            if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+              for (int i = 0; i < kOutCols; ++i) o[i] *= alpha;
             }
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) big = fmax3(big, fabsf(s[16 * q + i]), fabsf(s[16 * q + i + 1]));
           }
-        }
-        if (!share_max(g, big)) { ok = false; break; }
-        const int e = tc16::scale_exp(__float_as_uint(big));
-        if (with_grad) {
-          // This thread's column of acc: runs of equal buckets along the row.
-          const uint8_t* ids = &sm.ids[st][vec_at];
-          const int first = ids[0], last = ids[31];
-          if (__all_sync(0xffffffffu, first == last)) {  // ends equal: one bucket
-            float sum = 0.f;
+          factor = tc16::pow2(-e2);
+          prepare_next(t);
+        } else if constexpr (KIND == kDv) {
+          const float* off = sm.rows[st] + kW * half;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum += s[i];
-            acc[first * kRowThreadsTc + tid] += sum;
-          } else {
-            int cur = first;
-            float run = 0.f;
+          for (int i = 0; i < kW; i += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(off + i);
+            s[i] = ex2(s[i] - f.x + kWeightLog2);
+            s[i + 1] = ex2(s[i + 1] - f.y + kWeightLog2);
+            s[i + 2] = ex2(s[i + 2] - f.z + kWeightLog2);
+            s[i + 3] = ex2(s[i + 3] - f.w + kWeightLog2);
+          }
+          store_weights<kW>(scol, s);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&sm.w_ready[sb]);
+          if (t > 0) ok = add_partial(G - 1);
+          factor = tc16::pow2(-e2) * 6.103515625e-05f;  // 2^-14
+          prepare_next(t);
+        } else {
+          // ds = w (dP - delta), then an exponent for the row: its largest |ds| to [2^14, 2^15)
+          float big = 0.f;
+          if (ok) {
+            const float unit = finite(r.unit * tc16::pow2(-e2));
+            const float* off = sm.rows[st] + kW * half;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int id = ids[i];
-              if (id != cur) {
-                acc[cur * kRowThreadsTc + tid] += run;
-                run = 0.f;
-                cur = id;
+            for (int q = 0; q < kW / 16; ++q) {
+              float dp[16];
+              tc16::tmem_ld16(lane + kColS2 + kW * half + 16 * q, dp);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int k = 16 * q + i;
+                const float w = ex2(s[k] - (KIND == kDk ? off[k] : r.off));
+                s[k] = w * fmaf(dp[i], unit, -(KIND == kDk ? off[64 + k] : r.delta));
               }
-              run += s[i];
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) big = fmax3(big, fabsf(s[16 * q + i]), fabsf(s[16 * q + i + 1]));
             }
-            acc[cur * kRowThreadsTc + tid] += run;
           }
-          __syncwarp();  // the lanes' runs end at different columns
+          if (!share_max(G, big)) { ok = false; break; }
+          const int e = tc16::scale_exp(__float_as_uint(big));
+          if (with_grad) {
+#pragma unroll
+            for (int q = 0; q < kW; q += 32) {
+              const int base = c0 + q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
+              if (base - 31 >= c.far || base + 31 <= -c.far) {     // all beyond the last bound
+                float x = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x += s[q + i];
+                if (base > 0)
+                  far_after += x;
+                else
+                  far_before += x;
+              } else {
+                float before, after;
+                diagonal_sums(buf, s + q, ln, before, after);
+                float* at = dist + base + c.far + 63;
+                at[ln - 31] += before;
+                at[ln + 1] += after;  // lane 31: 0, one slot past the block's distances
+                __syncwarp();
+              }
+            }
+          }
+          const float up = tc16::pow2(e);
+#pragma unroll
+          for (int i = 0; i < kW; ++i) s[i] *= up;
+          store_weights<kW>(scol, s);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&sm.w_ready[sb]);
+          factor = finite(tc16::pow2(-e) * tc16::pow2(-e1));
+          prepare_next(t);
+          ok = add_partial(G);
         }
-        const float up = tc16::pow2(e);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) s[i] *= up;
-        store_weights(scol, s);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&sm.w_ready[sb]);
-        factor = finite(tc16::pow2(-e) * tc16::pow2(-e1));
-        ok = add_partial(g);
       }
-    }
-    if constexpr (!kScores2)
-      if (ok) ok = add_partial(n - 1);
-    float f = KIND == kDv ? 1.f : c.t.scale;
-    if constexpr (KIND == kForward) {  // the row's sum: first half + second half
-      sm.red[0][half][rt] = lsum;  // the last exchange is read: part_full follows both threads' w_ready
-      bar_named(kRowBarrier, kRowThreadsTc);
-      lsum = sm.red[0][0][rt] + sm.red[0][1][rt];
-      f = lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f;
-      if (ok && c.t.stats_out && half == 0 && row < a.seq)
-        c.t.stats_out[static_cast<size_t>(bh) * a.seq + row] =
-            row < valid ? make_stats(m_true, (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2, lsum)
-                        : make_float2(-INFINITY, 0.f);
-      __syncwarp();
-    }
-    // The warp's rows through shared memory (the stages are idle: every copy
-    // and product is complete), so that eight lanes store 128 bytes of a row.
-    if (ok) {
-      constexpr int kPitch = 64 * P + 4;  // 16-byte accesses of 8 rows or of one row meet no bank twice
-      static_assert(kTileRows * kPitch * 4 <= 2 * stage_bytes<P>(), "row staging");
-      float* stage = reinterpret_cast<float*>(smem) + (warp & 3) * 32 * kPitch + kOutCols * half;
-      const bool live = row < valid;
-#pragma unroll
-      for (int i = 0; i < kOutCols; i += 4)
-        *reinterpret_cast<float4*>(stage + (tid & 31) * kPitch + i) =
-            live ? make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
-      __syncwarp();
-      const int wr0 = r0 + (warp & 3) * 32, wrows = min(32, a.seq - wr0);
-      float* dst = outp + (static_cast<size_t>(bh) * a.seq + wr0) * d + kOutCols * half;
-      constexpr int kLanes = kOutCols / 4;  // lanes of a row
-      const int col = (tid % kLanes) * 4;
-#pragma unroll
-      for (int i = 0; i < kLanes; ++i) {
-        const int r = i * (32 / kLanes) + (tid & 31) / kLanes;
-        if (r < wrows && kOutCols * half + col < d)
-          st_stream(dst + static_cast<size_t>(r) * d + col, *reinterpret_cast<const float4*>(stage + r * kPitch + col));
+      if constexpr (!kScores2)
+        if (ok) ok = add_partial(G - 1);
+
+      float f = KIND == kDv ? 1.f : c.t.scale;
+      if constexpr (KIND == kForward) {
+        if constexpr (kHalves == 2) {  // the row's sum: first half + second half
+          sm.red[0][half][rt] = lsum;  // the last exchange is read: part_full follows both threads' w_ready
+          if (bar_any(kRowBarrier, kRowThreadsTc, !ok)) { ok = false; break; }
+          lsum = sm.red[0][0][rt] + sm.red[0][1][rt];
+          bar_named(kRowBarrier, kRowThreadsTc);  // read before the next unit's exchange
+        }
+        f = lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f;
+        if (ok && c.t.stats_out && half == 0 && row < a.seq)
+          c.t.stats_out[first_row + rt] =
+              row < u.valid ? make_stats(m_true, (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2, lsum)
+                            : make_float2(-INFINITY, 0.f);
+        __syncwarp();
       }
-    }
-    __syncwarp();
-    if (with_grad) {
-      // The threads' columns, bucket by bucket, in a fixed order.
-      bar_named(kRowBarrier, kRowThreadsTc);
-      for (int b = warp; b < c.t.buckets; b += 8) {
-        float x = 0.f;
-        for (int u = tid & 31; u < kRowThreadsTc; u += 32) x += acc[b * kRowThreadsTc + u];
+      if (with_grad) {
+        // The warps' distances, bucket by bucket, in a fixed order.
+        dist[0] = dist[c.slots - 1] = 0.f;  // of no pair: the far sums go there
+        __syncwarp();
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-        if ((tid & 31) == 0) partial[b] = x;
+        for (int off = 16; off > 0; off >>= 1) {
+          far_before += __shfl_xor_sync(0xffffffffu, far_before, off);
+          far_after += __shfl_xor_sync(0xffffffffu, far_after, off);
+        }
+        if (ln == 0) {
+          dist[0] = far_before;
+          dist[c.slots - 1] = far_after;
+        }
+        __syncwarp();
+        if (bar_any(kRowBarrier, kRowThreadsTc, !ok)) { ok = false; break; }
+        float* partial = c.t.part + (static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets;
+        const float* all = dist - warp * c.slots;
+        const int sides = c.t.buckets / 2;
+        for (int b = warp; b < c.t.buckets; b += kIssueWarp) {
+          const bool behind = b >= sides;  // keys after the query
+          const int k = behind ? b - sides : b;
+          const int from = max(c.bounds.at[k], behind ? 1 : 0);
+          const int end = behind ? c.far + 65 : c.far + 64;  // past the far sums' slot
+          const int to = k + 1 < sides ? min(c.bounds.at[k + 1], end) : end;
+          const int mid = c.far + 63;
+          float x = 0.f;
+          for (int i = from + ln; i < to; i += 32)
+            for (int w = 0; w < kIssueWarp; ++w) x += all[w * c.slots + mid + (behind ? i : -i)];
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+          if (ln == 0) partial[b] = x;
+        }
+        __syncwarp();
+        bar_named(kRowBarrier, kRowThreadsTc);
       }
+      if (!ok) break;
+      {
+        // The warp's rows, 32 columns at a time, through its buffer: eight lanes store 128 bytes of a row.
+        const bool live = row < u.valid;
+        const int wr0 = (warp & 3) * 32, wrows = min(32, a.seq - u.r0 - wr0);
+        float* dst = outp + (first_row + wr0) * d + kOutCols * half + (ln & 7) * 4;
+#pragma unroll
+        for (int q = 0; q < kOutCols; q += 32) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(buf + ln * kPitch + i) =
+                live ? make_float4(o[q + i] * f, o[q + i + 1] * f, o[q + i + 2] * f, o[q + i + 3] * f)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+          __syncwarp();
+          float4 x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            x[i] = *reinterpret_cast<const float4*>(buf + (4 * i + (ln >> 3)) * kPitch + (ln & 7) * 4);
+          if (kOutCols * half + q + (ln & 7) * 4 < d) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (4 * i + (ln >> 3) < wrows) st_stream(dst + static_cast<size_t>(4 * i + (ln >> 3)) * d + q, x[i]);
+          }
+          __syncwarp();
+        }
+      }
+      u = nu;
+      r = nr;
     }
   } else if (warp == kIssueWarp) {
     // ---------------- MMA issue ----------------
-    bool ok = warp_wait(&sm.a_ready, 0);
-    if (ok) tc_fence_after();
     auto commit = [&](uint64_t* bar, uint32_t parity) {
       mma_commit_e(bar);
       last_commit = bar;
@@ -614,7 +755,7 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
     };
     const uint32_t ops = smem_addr(smem);
     auto operand = [&](int g, int which) {
-      return ops + static_cast<uint32_t>((g % stages) * stage_bytes<P>() + which * (2 * P * kPanelBytes));
+      return ops + static_cast<uint32_t>((g % kStages) * stage_bytes<P>() + which * kOp);
     };
     // rows x columns^T into dcol: the small products first
     auto scores = [&](uint32_t dcol, uint32_t acol, uint32_t b) {
@@ -653,59 +794,104 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
         for (int k = 0; k < 4; ++k) tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k), tc16::v_desc(bhi, k), 1u);
       }
     };
-    if constexpr (kScores2) {
-      for (int g = 0; ok && g < n; ++g) {
-        ok = warp_wait(&sm.full[g % stages], g / stages);
-        // The row threads have added the last partial, so its columns (dP's, for P = 1) and the weights' are free.
-        if (ok && g > 0) ok = warp_wait(&sm.part_free, g - 1);
-        if (!ok) break;
-        tc_fence_after();
-        scores(kColS, 0, operand(g, 0));
-        scores(kColS2, kColA2, operand(g, 1));
-        commit(&sm.s_full[0], g);
-        ok = warp_wait(&sm.w_ready[0], g);
-        if (!ok) break;
-        tc_fence_after();
-        sums(kColS, operand(g, 0));
-        commit(&sm.part_full, g);
-        if (g + stages < n) commit(&sm.freed[g % stages], g / stages);
-      }
-    } else {
-      if (ok) ok = warp_wait(&sm.full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        scores(kColS, 0, operand(0, 0));
-        commit(&sm.s_full[0], 0);
-      }
-      for (int g = 0; ok && g < n; ++g) {
-        if (g + 1 < n) {
-          // The other score buffer held the weights of tile g - 1: its product is complete.
-          if (g > 0) ok = warp_wait(&sm.part_full, g - 1);
-          if (ok) ok = warp_wait(&sm.full[(g + 1) % stages], (g + 1) / stages);
+    int G = 0, U = 0;
+    bool ok = true;
+    TcUnit u;
+    while (ok && take_unit(u) && u.n >= 0) {
+      const int n = u.n;
+      if (n == 0) continue;
+      ok = warp_wait(&sm.a_ready, U++);
+      for (int t = 0; ok && t < n; ++t, ++G) {
+        if constexpr (kScores2) {
+          ok = warp_wait(&sm.full[G % kStages], G / kStages);
+          // The row threads have added the last partial, so its columns (dP's, for P = 1) and the weights' are free.
+          if (ok && G > 0) ok = warp_wait(&sm.part_free, G - 1);
           if (!ok) break;
           tc_fence_after();
-          scores(kColS + 64 * ((g + 1) & 1), 0, operand(g + 1, 0));
-          commit(&sm.s_full[(g + 1) & 1], (g + 1) >> 1);
+          scores(kColS, 0, operand(G, 0));
+          scores(kColS2, kColA2, operand(G, 1));
+          commit(&sm.s_full[0], G);
+        } else {
+          // The scores of tile g go to the buffer that held the weights of tile g - 2, whose product is complete.
+          auto scores_of = [&](int g) {
+            ok = warp_wait(&sm.full[g % kStages], g / kStages);
+            if (!ok) return;
+            tc_fence_after();
+            scores(kColS + 64 * (g & 1), 0, operand(g, 0));
+            commit(&sm.s_full[g & 1], g >> 1);
+          };
+          if (t == 0) scores_of(G);
+          if (ok && t + 1 < n) {
+            if (G > 0) ok = warp_wait(&sm.part_full, G - 1);
+            if (ok) scores_of(G + 1);
+          }
         }
-        ok = warp_wait(&sm.w_ready[g & 1], g >> 1);
-        if (ok && g > 0) ok = warp_wait(&sm.part_free, g - 1);
+        if (ok) ok = warp_wait(&sm.w_ready[kScores2 ? 0 : G & 1], kScores2 ? G : G >> 1);
+        if (!kScores2 && ok && G > 0) ok = warp_wait(&sm.part_free, G - 1);
         if (!ok) break;
         tc_fence_after();
-        sums(kColS + 64 * (g & 1), operand(g, 1));
-        commit(&sm.part_full, g);
-        if (g + stages < n) commit(&sm.freed[g % stages], g / stages);
+        sums(kScores2 ? kColS : kColS + 64 * (G & 1), operand(G, kScores2 ? 0 : 1));
+        commit(&sm.freed[G % kStages], G / kStages);
+        commit(&sm.part_full, G);
+        committed = G + 1;
       }
     }
-  } else {
-    // ---------------- bulk copies (the first `stages` are on their way) ----------------
-    for (int g = stages; g < n; ++g) {
-      if (!warp_wait(&sm.freed[g % stages], g / stages - 1)) break;
-      if (tc16::lane_is_first(tid)) {
-        fence_proxy_async_smem();  // the row threads' reads of this stage, before the copies
-        copy_stage(g);
+    // Nothing arrives on a barrier after the CTA has ended.
+    for (int g = max(0, committed - kStages); ok && g < committed; ++g) ok = warp_wait(&sm.freed[g % kStages], g / kStages);
+  } else if (warp == kIssueWarp + 1) {
+    // ---------------- units and bulk copies ----------------
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      unsigned unit = blockIdx.x;
+      if (k > 0) {
+        if ((tid & 31) == 0) unit = gridDim.x + atomicAdd(c.next + KIND, 1u);
+        unit = __shfl_sync(0xffffffffu, unit, 0);
       }
-      last_g = g;
+      TcUnit u{0, 0, 0, 0, -1};
+      if (unit < c.units) {
+        const unsigned tiles = static_cast<unsigned>(c.tiles) / 2;
+        u.local = static_cast<int>(unit / tiles);
+        u.valid = valid_of(a, c.slice0 + u.local);
+        u.r0 = static_cast<int>(unit - u.local * tiles) * kTileRows;
+        int lo = 0, hi = 0, unused;
+        if (u.r0 < u.valid) {
+          key_range(a, u.r0, u.valid, lo, unused);
+          key_range(a, min(u.r0 + kTileRows, u.valid) - 1, u.valid, unused, hi);
+        }
+        u.t0 = lo / kTileCols;
+        u.n = hi > lo ? (hi + kTileCols - 1) / kTileCols - u.t0 : 0;
+      }
+      if (k >= kQueue) ok = warp_wait(&sm.u_free[k % kQueue], k / kQueue - 1);
+      if (!ok) break;
+      if ((tid & 31) == 0) {
+        sm.unit[k % kQueue] = u;
+        mbar_arrive(&sm.u_full[k % kQueue]);
+      }
       __syncwarp();
+      if (u.n < 0) break;
+      const int head = static_cast<int>((c.slice0 + u.local) % a.heads);
+      for (int t = 0; t < u.n; ++t) {
+        const int st = copied % kStages, c0 = (u.t0 + t) * kTileCols;
+        if (copied >= kStages) ok = warp_wait(&sm.freed[st], copied / kStages - 1);
+        if (!ok) break;
+        if (tc16::lane_is_first(tid)) {
+          fence_proxy_async_smem();  // the row threads' reads of this stage, before the copies
+          const long long tile = static_cast<long long>(u.local) * c.tiles + u.t0 + t;
+          // The tile's first distance j - i: rows' i from r0, or columns' i from c0.
+          const int rel = kByKey ? u.r0 - c0 - 64 : c0 - u.r0 - 128;
+          unsigned char* op = smem + st * stage_bytes<P>();
+          uint64_t* bar = &sm.full[st];
+          mbar_arrive_expect_tx(bar, 2 * kOp + 16u + (BIAS ? kVec * 4u : 0u) + (kByKey ? 512u : 0u));
+          tma_load_1d(op, c.img[kB1] + tile * static_cast<long long>(kOp), kOp, bar);
+          tma_load_1d(op + kOp, c.img[kB2] + tile * static_cast<long long>(kOp), kOp, bar);
+          tma_load_1d(sm.exps[st], c.exps + tile, 16u, bar);
+          if constexpr (BIAS)
+            tma_load_1d(sm.vec[st], c.t.rel_bias + (2ll * head + 1) * c.t.rel_half + rel, kVec * 4u, bar);
+          if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * 128, 512u, bar);
+        }
+        __syncwarp();
+        ++copied;
+      }
     }
   }
   __syncwarp();
@@ -719,8 +905,8 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
       while (!mbar_try_wait(bar, parity & 1u) && clock64() < t_end) {
       }
     };
-    if (tid == kCopyWarp * 32)
-      for (int g = max(0, last_g - stages + 1); g <= last_g; ++g) drain(&sm.full[g % stages], g / stages);
+    if (tid == (kIssueWarp + 1) * 32)
+      for (int g = max(0, copied - kStages); g < copied; ++g) drain(&sm.full[g % kStages], g / kStages);
     if (tid == kIssueWarp * 32 && last_commit) drain(last_commit, last_parity);
   }
   __syncthreads();
@@ -728,23 +914,6 @@ __device__ void run_tile(const TcArgs& c, long long local, int tile128, unsigned
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
   }
-}
-
-__device__ __forceinline__ unsigned char* aligned_smem(unsigned char* raw) {
-  const uint32_t at = smem_addr(raw);
-  return raw + (((at + 1023u) & ~1023u) - at);
-}
-
-// One CTA per 128-row tile of the chunk's slices.  A launch per kind: with
-// the three gradients in one grid, CTAs of different kinds on an SM evicted
-// one another's code from the instruction cache (4.0 of 17 stall cycles per
-// instruction were instruction fetch).
-template <int KIND, int P, bool BIAS>
-__global__ void __launch_bounds__(kTcThreads, P == 1 ? 2 : 1) tc_train(const __grid_constant__ TcArgs c) {
-  extern __shared__ unsigned char raw[];
-  const unsigned tiles = static_cast<unsigned>(c.tiles) / 2, local = blockIdx.x / tiles;
-  const int tile = static_cast<int>(blockIdx.x - local * tiles);
-  run_tile<KIND, P, BIAS>(c, local, tile, aligned_smem(raw), tile);
 }
 
 }  // namespace train
