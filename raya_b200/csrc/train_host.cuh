@@ -119,11 +119,11 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
                                                               0x7fffffffll / (2ll * plan->tiles)}));
     for (int i = 0; i < tensors; ++i) plan->img[i] = take(plan->chunk * image);
     plan->exps = take(plan->chunk * plan->tiles * sizeof(int4));
-    if (backward) plan->rows = take(static_cast<size_t>(plan->chunk) * plan->tiles * 128 * sizeof(float));
+    if (backward) plan->rows = take(static_cast<size_t>(plan->chunk) * plan->tiles * train::kRowValues * sizeof(float));
     plan->next = take(4 * sizeof(unsigned));
-    if (backward && bias) {
-      // Distances beyond seq do not occur.
+    if (bias)  // distances beyond seq do not occur
       plan->far = static_cast<int>(std::min<int64_t>(bucket_bounds(bias->buckets, bias->max_distance).at[bias->buckets / 2 - 1], d->seq));
+    if (backward && bias) {
       plan->slots = 2 * plan->far + 128;
       const size_t warps = train::kRowWarpsOf(plan->panels), bytes = warps * plan->slots * sizeof(float);
       const size_t spare = plan->panels == 1 ? train::kHalfSm - train::tc_smem<1>() : train::kWholeSm - train::tc_smem<2>();
@@ -193,11 +193,11 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   c.exps = at<int4>(workspace, plan.exps);
   if (backward) c.rows = at<float>(workspace, plan.rows);
   c.next = at<unsigned>(workspace, plan.next);
+  c.far = plan.far;
   const size_t smem = train::tc_smem<P>();
   size_t dist = 0;
   if (t.part) {
     c.bounds = bounds;
-    c.far = plan.far;
     c.slots = plan.slots;
     if (plan.dist_bytes > 0)
       c.dist = at<float>(workspace, plan.dist);

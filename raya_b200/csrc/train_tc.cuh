@@ -82,6 +82,7 @@ constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
 constexpr float kWeightLog2 = 14.f;                // kDv: w enters as w * 2^14, so that small ones keep their bits
+constexpr int kRowValues = 3 * 64;                 // values per 64 rows of dout
 constexpr float kRescale = 8.f, kForwardLog2 = 7.f;  // kForward: p <= 2^8 of the kept maximum, times 2^7
 
 enum TcKind { kForward = 0, kDq = 1, kDk = 2, kDv = 3 };
@@ -94,7 +95,7 @@ struct TcArgs {
   TrainArgs t;
   uint8_t* img[4];     // [chunk slices][tiles][2 P panels]: q, k, v, dout
   int4* exps;          // [chunk slices][tiles]: their exponents
-  float* rows;         // [chunk slices][tiles][2][64]: m * log2(e) (inf: no key), and delta / l
+  float* rows;         // [chunk slices][tiles][3][64]: m * log2(e) (inf: no key), that - kWeightLog2, and delta / l
   int tiles;           // 64-row tiles per slice (even)
   long long slice0;
   unsigned units;      // 128-row tiles of the chunk
@@ -157,9 +158,11 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
 #pragma unroll
       for (int off = 8; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
       if ((tid & 15) == 0) {
-        float* rows = c.rows + (local * c.tiles + tile) * 128;
-        rows[r + 16 * i] = linv != 0.f ? m2 : INFINITY;  // 2^(x - inf) = 0: no key, or past valid_len
-        rows[64 + r + 16 * i] = dot;
+        float* rows = c.rows + (local * c.tiles + tile) * kRowValues;
+        const float off = linv != 0.f ? m2 : INFINITY;  // 2^(x - inf) = 0: no key, or past valid_len
+        rows[r + 16 * i] = off;
+        rows[64 + r + 16 * i] = off - kWeightLog2;
+        rows[128 + r + 16 * i] = dot;
       }
     }
   }
@@ -205,8 +208,9 @@ struct TcUnit {
 constexpr int kQueue = 2;
 struct alignas(16) TcTail {
   float vec[kStages][kVec];       // bias * log2(e) by distance
-  float rows[kStages][2 * 64];    // kDk, kDv: the columns' exponent and delta
+  float rows[kStages][kRowValues];  // kDk, kDv: the columns' exponents and delta
   int exps[kStages][4];           // exponents of the columns' 64 rows, by tensor
+  int flat[kStages];              // the tile's pairs all lie in one distance bucket
   float red[2][2][kTileRows];     // [tile parity][half]: what a row's threads exchange
   TcUnit unit[kQueue];            // the units that the copy warp has begun
   uint64_t u_full[kQueue], u_free[kQueue];
@@ -234,36 +238,44 @@ static_assert(tc_smem<1>() <= kHalfSm && tc_smem<1>() > 233472 / 3 && tc_smem<2>
 // A product of scales that would be infinite, as the largest float: 0 times it is 0.
 __device__ __forceinline__ float finite(float x) { return fmaxf(fminf(x, 3.4028235e38f), -3.4028235e38f); }
 
-// Weights w[N] (fp32, already scaled) as fp16 hi and lo over their scores.
-template <int N>
+// Weights w[32] (fp32, already scaled) as fp16 hi and lo over their scores.
 __device__ __forceinline__ void store_weights(uint32_t taddr, const float* w) {
 #pragma unroll
-  for (int s = 0; s < N / 16; ++s) {
+  for (int s = 0; s < 2; ++s) {
     uint32_t h[8], l[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) tc16::split2(w[16 * s + 2 * k], w[16 * s + 2 * k + 1], h[k], l[k]);
-    tc16::tmem_st8u(taddr + 32 * (s >> 1) + 8 * (s & 1), h);
-    tc16::tmem_st8u(taddr + 32 * (s >> 1) + 8 * (s & 1) + 16, l);
+    tc16::tmem_st8u(taddr + 8 * s, h);
+    tc16::tmem_st8u(taddr + 8 * s + 16, l);
   }
 }
 
+// Two neighbouring values for the packed operations.
+__device__ __forceinline__ float2 get2(const float* x) { return make_float2(x[0], x[1]); }
+__device__ __forceinline__ void put2(float* x, float2 y) {
+  x[0] = y.x;
+  x[1] = y.y;
+}
+
+__device__ __forceinline__ float2 sub2(float2 x, float2 y) { return __ffma2_rn(y, make_float2(-1.f, -1.f), x); }
+
 // N scores in place: s * mult (+ bias), -inf outside [lo, hi).
+// flat: one bias for all of them.
 template <int N, bool BIAS, int STEP>
-__device__ __forceinline__ void mask_scores(float* s, float mult, const float* vec, int lo, int hi, bool inside) {
+__device__ __forceinline__ void mask_scores(float* s, float mult, const float* vec, bool flat, int lo, int hi, bool inside) {
   const float2 m2 = make_float2(mult, mult);
+  if (!BIAS || flat) {
+    const float2 b = BIAS ? make_float2(vec[0], vec[0]) : make_float2(-0.f, -0.f);
 #pragma unroll
-  for (int q = 0; q < N; q += 16) {  // 16 loads in flight
-    float2 b[8];
-    if constexpr (BIAS) {
+    for (int i = 0; i < N; i += 2) put2(s + i, BIAS ? __ffma2_rn(get2(s + i), m2, b) : __fmul2_rn(get2(s + i), m2));
+  } else {
+#pragma unroll
+    for (int q = 0; q < N; q += 16) {  // 16 loads in flight
+      float2 b[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) b[i] = make_float2(vec[STEP * (q + 2 * i)], vec[STEP * (q + 2 * i + 1)]);
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 x = make_float2(s[q + 2 * i], s[q + 2 * i + 1]);
-      const float2 y = BIAS ? __ffma2_rn(x, m2, b[i]) : __fmul2_rn(x, m2);
-      s[q + 2 * i] = y.x;
-      s[q + 2 * i + 1] = y.y;
+      for (int i = 0; i < 8; ++i) put2(s + q + 2 * i, __ffma2_rn(get2(s + q + 2 * i), m2, b[i]));
     }
   }
   if (!inside) {
@@ -306,15 +318,16 @@ __device__ __forceinline__ void diagonal_sums(float* buf, const float* s, int la
   for (int i = 0; i < 32; i += 4)
     *reinterpret_cast<float4*>(buf + lane * kPitch + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
   __syncwarp();
+  float x[32];
+#pragma unroll
+  for (int r = 0; r < 32; ++r) x[r] = buf[r * (kPitch + 1) + lane + 1 - (lane >= 31 - r ? 32 : 0)];
   before = after = 0.f;
 #pragma unroll
   for (int r = 0; r < 32; ++r) {
-    const bool wrapped = lane >= 31 - r;
-    const float x = buf[r * (kPitch + 1) + lane + 1 - (wrapped ? 32 : 0)];
-    if (wrapped)
-      before += x;
+    if (lane >= 31 - r)
+      before += x[r];
     else
-      after += x;
+      after += x[r];
   }
   __syncwarp();
 }
@@ -330,6 +343,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
   constexpr bool kByKey = KIND == kDk || KIND == kDv;        // rows are keys, columns queries
   constexpr int kHalves = P;                                 // threads per row
   constexpr int kW = 64 / kHalves;                           // score columns of a thread
+  constexpr int kBlocks = kW / 32;
   constexpr bool kShared = KIND != kDv && kHalves == 2;      // a row's threads share a maximum
   constexpr int kRowThreadsTc = 128 * kHalves;
   constexpr int kIssueWarp = kRowWarpsOf(P);                 // and the copy warp behind it; two more idle
@@ -470,8 +484,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       r.unit = kScores2 ? tc16::pow2(-(kByKey ? e.z : e.w)) : 0.f;
       r.off = r.delta = 0.f;
       if constexpr (KIND == kDq) {
-        r.off = c.rows[tile * 128 + (rt & 63)];
-        r.delta = c.rows[tile * 128 + 64 + (rt & 63)];
+        r.off = c.rows[tile * kRowValues + (rt & 63)];
+        r.delta = c.rows[tile * kRowValues + 128 + (rt & 63)];
       }
       key_range(a, min(u.r0 + rt, u.valid - 1), u.valid, r.lo, r.hi);
       tmem_wait_st();
@@ -510,15 +524,11 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         tc_fence_after();
         const float2 f2 = make_float2(factor, factor);
 #pragma unroll
-        for (int q = 0; q < kOutCols / 16; ++q) {
-          float x[16];
-          tc16::tmem_ld16(lane + kColPart + kOutCols * half + 16 * q, x);
+        for (int q = 0; q < kOutCols; q += 32) {
+          float x[32];
+          tmem_ld32(lane + kColPart + kOutCols * half + q, x);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float2 y = __ffma2_rn(make_float2(x[i], x[i + 1]), f2, make_float2(o[16 * q + i], o[16 * q + i + 1]));
-            o[16 * q + i] = y.x;
-            o[16 * q + i + 1] = y.y;
-          }
+          for (int i = 0; i < 32; i += 2) put2(o + q + i, __ffma2_rn(get2(x + i), f2, get2(o + q + i)));
         }
         tc_fence_before();
         mbar_arrive(&sm.part_free);
@@ -548,19 +558,30 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         const uint32_t scol = lane + kColS + 64 * sb + kW * half;
         const int e1 = sm.exps[st][kB1], e2 = sm.exps[st][kB2];
         const int mlo = r.lo - c0, mhi = r.hi - c0;
-        float s[kW];
-        if (ok) {
-          const bool inside = __all_sync(0xffffffffu, mlo <= 0 && mhi >= kW);
-          tmem_ld32(scol, s);
-          if constexpr (kW == 64) tmem_ld32(scol + 32, s + 32);
-          mask_scores<kW, BIAS, kStep>(s, finite(r.qmul * tc16::pow2(-e1)), &sm.vec[st][vec_at], mlo, mhi, inside);
-        }
+        const bool inside = __all_sync(0xffffffffu, mlo <= 0 && mhi >= kW);
+        const float mult = finite(r.qmul * tc16::pow2(-e1));
+        const bool flat = BIAS && sm.flat[st] != 0;
+        const float* const vec = &sm.vec[st][vec_at];
+        // 32 columns at a time, in rolled loops (the loop over the tiles is to
+        // fit the instruction cache nearest to the scheduler): block q's masked
+        // scores, and back into tensor memory until the row's maximum is known.
+        auto block_scores = [&](int q, float* s) {
+          tmem_ld32(scol + 32 * q, s);
+          mask_scores<32, BIAS, kStep>(s, mult, vec + kStep * 32 * q, flat, mlo - 32 * q, mhi - 32 * q, inside);
+        };
 
         if constexpr (KIND == kForward) {
           float mx = -INFINITY;
           if (ok) {
+#pragma unroll 1
+            for (int q = 0; q < kBlocks; ++q) {
+              float s[32];
+              block_scores(q, s);
 #pragma unroll
-            for (int i = 0; i < kW; i += 2) mx = fmax3(mx, s[i], s[i + 1]);
+              for (int i = 0; i < 32; i += 2) mx = fmax3(mx, s[i], s[i + 1]);
+              tmem_st32(scol + 32 * q, s);
+            }
+            tmem_wait_st();
           }
           if (!share_max(G, mx)) { ok = false; break; }
           float alpha = 1.f;
@@ -570,15 +591,24 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
             m_used = mx;
           }
           const float base = (m_used == -INFINITY ? 0.f : m_used) - kForwardLog2;
-          float2 sum = make_float2(0.f, 0.f);
+          const float2 nb = make_float2(-base, -base);
+          float2 sum = make_float2(0.f, 0.f), sum1 = sum;
+#pragma unroll 1
+          for (int q = 0; q < kBlocks; ++q) {
+            float s[32];
+            tmem_ld32(scol + 32 * q, s);
 #pragma unroll
-          for (int i = 0; i < kW; i += 2) {
-            s[i] = ex2(s[i] - base);
-            s[i + 1] = ex2(s[i + 1] - base);
-            sum = __fadd2_rn(sum, make_float2(s[i], s[i + 1]));
+            for (int i = 0; i < 32; i += 4) {
+              const float2 x = __fadd2_rn(get2(s + i), nb), y = __fadd2_rn(get2(s + i + 2), nb);
+              put2(s + i, make_float2(ex2(x.x), ex2(x.y)));
+              put2(s + i + 2, make_float2(ex2(y.x), ex2(y.y)));
+              sum = __fadd2_rn(sum, get2(s + i));
+              sum1 = __fadd2_rn(sum1, get2(s + i + 2));
+            }
+            store_weights(scol + 32 * q, s);
           }
+          sum = __fadd2_rn(sum, sum1);
           lsum = fmaf(lsum, alpha, sum.x + sum.y);
-          store_weights<kW>(scol, s);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&sm.w_ready[sb]);
@@ -586,22 +616,26 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
             ok = add_partial(G - 1);
             if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-              for (int i = 0; i < kOutCols; ++i) o[i] *= alpha;
+              for (int i = 0; i < kOutCols; i += 2) put2(o + i, __fmul2_rn(get2(o + i), make_float2(alpha, alpha)));
             }
           }
           factor = tc16::pow2(-e2);
           prepare_next(t);
         } else if constexpr (KIND == kDv) {
-          const float* off = sm.rows[st] + kW * half;
+#pragma unroll 1
+          for (int q = 0; q < kBlocks; ++q) {
+            const float* off = sm.rows[st] + 64 + kW * half + 32 * q;
+            float s[32];
+            block_scores(q, s);
 #pragma unroll
-          for (int i = 0; i < kW; i += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(off + i);
-            s[i] = ex2(s[i] - f.x + kWeightLog2);
-            s[i + 1] = ex2(s[i + 1] - f.y + kWeightLog2);
-            s[i + 2] = ex2(s[i + 2] - f.z + kWeightLog2);
-            s[i + 3] = ex2(s[i + 3] - f.w + kWeightLog2);
+            for (int i = 0; i < 32; i += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(off + i);
+              const float2 x = sub2(get2(s + i), make_float2(f.x, f.y)), y = sub2(get2(s + i + 2), make_float2(f.z, f.w));
+              put2(s + i, make_float2(ex2(x.x), ex2(x.y)));
+              put2(s + i + 2, make_float2(ex2(y.x), ex2(y.y)));
+            }
+            store_weights(scol + 32 * q, s);
           }
-          store_weights<kW>(scol, s);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&sm.w_ready[sb]);
@@ -613,49 +647,66 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
           float big = 0.f;
           if (ok) {
             const float unit = finite(r.unit * tc16::pow2(-e2));
-            const float* off = sm.rows[st] + kW * half;
+            const float2 unit2 = make_float2(unit, unit);
+#pragma unroll 1
+            for (int q = 0; q < kBlocks; ++q) {
+              const float* off = sm.rows[st] + kW * half + 32 * q;
+              float s[32], dp[32];
+              block_scores(q, s);
+              tmem_ld32(lane + kColS2 + kW * half + 32 * q, dp);
 #pragma unroll
-            for (int q = 0; q < kW / 16; ++q) {
-              float dp[16];
-              tc16::tmem_ld16(lane + kColS2 + kW * half + 16 * q, dp);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int k = 16 * q + i;
-                const float w = ex2(s[k] - (KIND == kDk ? off[k] : r.off));
-                s[k] = w * fmaf(dp[i], unit, -(KIND == kDk ? off[64 + k] : r.delta));
+              for (int i = 0; i < 32; i += 4) {
+                float4 f, g;
+                if constexpr (KIND == kDk) {
+                  f = *reinterpret_cast<const float4*>(off + i);
+                  g = *reinterpret_cast<const float4*>(off + 128 + i);
+                } else {
+                  f = make_float4(r.off, r.off, r.off, r.off);
+                  g = make_float4(r.delta, r.delta, r.delta, r.delta);
+                }
+                const float2 x = sub2(get2(s + i), make_float2(f.x, f.y));
+                const float2 y = sub2(get2(s + i + 2), make_float2(f.z, f.w));
+                put2(s + i, __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)),
+                                       __ffma2_rn(get2(dp + i), unit2, make_float2(-g.x, -g.y))));
+                put2(s + i + 2, __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)),
+                                           __ffma2_rn(get2(dp + i + 2), unit2, make_float2(-g.z, -g.w))));
+                big = fmax3(big, fabsf(s[i]), fabsf(s[i + 1]));
+                big = fmax3(big, fabsf(s[i + 2]), fabsf(s[i + 3]));
               }
+              tmem_st32(scol + 32 * q, s);
+              if (with_grad) {
+                const int base = c0 + 32 * q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
+                if (base - 31 >= c.far || base + 31 <= -c.far) {          // all beyond the last bound
+                  float x = 0.f;
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) big = fmax3(big, fabsf(s[16 * q + i]), fabsf(s[16 * q + i + 1]));
+                  for (int i = 0; i < 32; ++i) x += s[i];
+                  if (base > 0)
+                    far_after += x;
+                  else
+                    far_before += x;
+                } else {
+                  float before, after;
+                  diagonal_sums(buf, s, ln, before, after);
+                  float* at = dist + base + c.far + 63;
+                  at[ln - 31] += before;
+                  at[ln + 1] += after;  // lane 31: 0, one slot past the block's distances
+                  __syncwarp();
+                }
+              }
             }
+            tmem_wait_st();
           }
           if (!share_max(G, big)) { ok = false; break; }
           const int e = tc16::scale_exp(__float_as_uint(big));
-          if (with_grad) {
+          const float2 up = make_float2(tc16::pow2(e), tc16::pow2(e));
+#pragma unroll 1
+          for (int q = 0; q < kBlocks; ++q) {
+            float s[32];
+            tmem_ld32(scol + 32 * q, s);
 #pragma unroll
-            for (int q = 0; q < kW; q += 32) {
-              const int base = c0 + q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
-              if (base - 31 >= c.far || base + 31 <= -c.far) {     // all beyond the last bound
-                float x = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x += s[q + i];
-                if (base > 0)
-                  far_after += x;
-                else
-                  far_before += x;
-              } else {
-                float before, after;
-                diagonal_sums(buf, s + q, ln, before, after);
-                float* at = dist + base + c.far + 63;
-                at[ln - 31] += before;
-                at[ln + 1] += after;  // lane 31: 0, one slot past the block's distances
-                __syncwarp();
-              }
-            }
+            for (int i = 0; i < 32; i += 2) put2(s + i, __fmul2_rn(get2(s + i), up));
+            store_weights(scol + 32 * q, s);
           }
-          const float up = tc16::pow2(e);
-#pragma unroll
-          for (int i = 0; i < kW; ++i) s[i] *= up;
-          store_weights<kW>(scol, s);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&sm.w_ready[sb]);
@@ -881,13 +932,14 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
           const int rel = kByKey ? u.r0 - c0 - 64 : c0 - u.r0 - 128;
           unsigned char* op = smem + st * stage_bytes<P>();
           uint64_t* bar = &sm.full[st];
-          mbar_arrive_expect_tx(bar, 2 * kOp + 16u + (BIAS ? kVec * 4u : 0u) + (kByKey ? 512u : 0u));
+          if constexpr (BIAS) sm.flat[st] = rel + 1 >= c.far || rel + kVec - 1 <= -c.far;
+          mbar_arrive_expect_tx(bar, 2 * kOp + 16u + (BIAS ? kVec * 4u : 0u) + (kByKey ? kRowValues * 4u : 0u));
           tma_load_1d(op, c.img[kB1] + tile * static_cast<long long>(kOp), kOp, bar);
           tma_load_1d(op + kOp, c.img[kB2] + tile * static_cast<long long>(kOp), kOp, bar);
           tma_load_1d(sm.exps[st], c.exps + tile, 16u, bar);
           if constexpr (BIAS)
             tma_load_1d(sm.vec[st], c.t.rel_bias + (2ll * head + 1) * c.t.rel_half + rel, kVec * 4u, bar);
-          if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * 128, 512u, bar);
+          if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * kRowValues, kRowValues * 4u, bar);
         }
         __syncwarp();
         ++copied;
