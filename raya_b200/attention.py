@@ -21,7 +21,6 @@ CUDA library; there is no CPU path.
 from __future__ import annotations
 
 import abc
-import contextlib
 import ctypes
 from dataclasses import dataclass, field
 from typing import Sequence, Union
@@ -432,10 +431,8 @@ class Cuda(AttentionKernel):
         (a CUDA tensor of at least train_workspace bytes) must not be used by
         another call meanwhile; without one the call takes it from torch's
         caching allocator."""
-        c = _TrainCall(shape, params, bias, valid_len, workspace, stream, {"q": q, "k": k, "v": v, "out": out}, stats)
-        with c.run(False) as ws:
-            _check(lib.raya_attn_forward_bias(c.desc, c.ptr["q"], c.ptr["k"], c.ptr["v"], c.ptr["out"],
-                                              c.ptr["stats"], c.valid, c.bias, *ws, c.stream))
+        _train_call(lib.raya_attn_forward_bias, False, shape, params, (("q", q), ("k", k), ("v", v), ("out", out)), stats,
+                    (), bias, None, valid_len, workspace, stream)
 
     def attend_backward(self, shape: AttnShape, params: AttnParams, q, k, v, out, stats, dout, dq, dk, dv,
                         bias: RelativeBias | None = None, dtable=None, valid_len=None, workspace=None,
@@ -449,89 +446,96 @@ class Cuda(AttentionKernel):
         and workspace as for attend_bias."""
         if stats is None:
             raise TypeError("attend_backward needs the stats of attend_bias")
-        c = _TrainCall(shape, params, bias, valid_len, workspace, stream,
-                       {"q": q, "k": k, "v": v, "out": out, "dout": dout, "dq": dq, "dk": dk, "dv": dv}, stats, dtable)
-        with c.run(True) as ws:
-            _check(lib.raya_attn_backward(c.desc, *(c.ptr[n] for n in ("q", "k", "v", "out", "stats", "dout", "dq", "dk", "dv")),
-                                          c.valid, c.bias, c.ptr["dtable"], *ws, c.stream))
+        _train_call(lib.raya_attn_backward, True, shape, params, (("q", q), ("k", k), ("v", v), ("out", out)), stats,
+                    (("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)), bias, dtable, valid_len, workspace, stream)
 
 
 def train_workspace(shape: AttnShape, params: AttnParams, bias: RelativeBias | None = None,
                     backward: bool = False) -> int:
     """Workspace bytes of attend_bias, or of attend_backward (host-only)."""
-    d, need = make_desc(shape, params), ctypes.c_size_t()
     b = None if bias is None else _lib.Bias(None, bias.buckets, bias.max_distance)
-    _check(lib.raya_attn_train_workspace(ctypes.byref(d), b, int(backward), ctypes.byref(need)))
+    return _train_bytes(make_desc(shape, params), b, backward)
+
+
+def _train_bytes(d: Desc, b, backward: bool) -> int:
+    need = ctypes.c_size_t()
+    _check(lib.raya_attn_train_workspace(d, b, int(backward), need))
     return need.value
 
 
-class _TrainCall:
-    """The checked arguments of one training call: every tensor a contiguous
-    CUDA float32 tensor of its size, all on one device."""
+def _train_call(call, backward, shape, params, tensors, stats, more, bias, dtable, valid_len, workspace, stream) -> None:
+    """One training call: every tensor checked to be a contiguous CUDA float32
+    tensor of its size, all on one device, then ``call`` with that device and
+    the stream current.  Written for a short way to the launches: a call on
+    one sequence takes the GPU about 20 us."""
+    import torch
 
-    def __init__(self, shape, params, bias, valid_len, workspace, stream, tensors, stats, dtable=None):
-        import torch
+    q = tensors[0][1]
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise TypeError("`q` must be a contiguous CUDA torch.float32 tensor")
+    device = q.device
 
-        self.torch, self.device = torch, None
-        d = make_desc(shape, params)
-        self.desc, numel = ctypes.byref(d), shape.numel()
-        self.ptr = {n: self._take(n, x, numel) for n, x in tensors.items()}
-        self.ptr["stats"] = None if stats is None else self._take("stats", stats, 2 * shape.batch * shape.heads * shape.seq)
-        self.bias, self.ptr["dtable"] = None, None
-        if bias is not None:
-            entries = shape.heads * bias.buckets
-            self.bias = _lib.Bias(self._take("table", bias.table, entries), bias.buckets, bias.max_distance)
-            if dtable is not None:
-                self.ptr["dtable"] = self._take("dtable", dtable, entries)
-        elif dtable is not None:
-            raise TypeError("dtable without a bias")
-        self.keep = None
-        if valid_len is None:
-            host = params.valid_array(shape.batch)
-            if (host < 0).any() or (host > shape.seq).any():
-                raise ShapeError(f"invalid shape: valid_len outside [0, {shape.seq}]")
-            if (host != shape.seq).any():
-                self.keep = valid_len = torch.from_numpy(host).to(self.device)
-        self.valid = None if valid_len is None else self._take("valid_len", valid_len, shape.batch, torch.int32)
-        if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        elif not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream), device=self.device)
-        if stream.device != self.device:
-            raise TypeError(f"the stream is on {stream.device}, the tensors are on {self.device}")
-        self.on, self.stream = stream, stream.cuda_stream
-        if workspace is not None and (not isinstance(workspace, torch.Tensor) or not workspace.is_contiguous()
-                                      or workspace.device != self.device):
-            raise TypeError("the workspace must be a contiguous CUDA tensor on the tensors' device")
-        self.workspace = workspace
-
-    def _take(self, name, x, numel, dtype=None):
-        dtype = dtype or self.torch.float32
-        if not isinstance(x, self.torch.Tensor) or not x.is_cuda or x.dtype != dtype or not x.is_contiguous():
+    def ptr(name, x, numel, dtype=torch.float32):
+        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype is not dtype or not x.is_contiguous():
             raise TypeError(f"`{name}` must be a contiguous CUDA {dtype} tensor")
-        if self.device is None:
-            self.device = x.device
-        if x.device != self.device:
-            raise TypeError(f"`{name}` is on {x.device}, the other tensors are on {self.device}")
+        if x.device != device:
+            raise TypeError(f"`{name}` is on {x.device}, the other tensors are on {device}")
         if x.numel() != numel:
             raise LengthError(f"buffer `{name}` has length {x.numel()}, expected {numel}", name=name, got=x.numel(),
                               expected=numel)
         return x.data_ptr()
 
-    @contextlib.contextmanager
-    def run(self, backward: bool):
-        """Makes the tensors' device and the call's stream current and gives
-        the workspace's pointer and size.  Memory that is taken here is taken
-        on the call's stream, so the allocator orders its next use."""
-        with self.torch.cuda.stream(self.on):
-            ws = self.workspace
-            if ws is None:
-                need = ctypes.c_size_t()
-                _check(lib.raya_attn_train_workspace(self.desc, self.bias, int(backward), ctypes.byref(need)))
-                ws = self.torch.empty(need.value, dtype=self.torch.uint8, device=self.device)
-            yield (ws.data_ptr() or None, ws.numel() * ws.element_size())
-            if self.keep is not None:  # keep the uploaded lengths alive until the kernels have run
-                _sync(self.stream)
+    d = make_desc(shape, params)
+    rows = shape.batch * shape.heads * shape.seq
+    numel = rows * shape.head_dim
+    args = [ptr(name, x, numel) for name, x in tensors]
+    args.append(None if stats is None else ptr("stats", stats, 2 * rows))
+    args += [ptr(name, x, numel) for name, x in more]
+    b = dtable_ptr = None
+    if bias is not None:
+        entries = shape.heads * bias.buckets
+        b = _lib.Bias(ptr("table", bias.table, entries), bias.buckets, bias.max_distance)
+        if dtable is not None:
+            dtable_ptr = ptr("dtable", dtable, entries)
+    elif dtable is not None:
+        raise TypeError("dtable without a bias")
+    keep = None
+    if valid_len is None:
+        host = params.valid_array(shape.batch)
+        if (host < 0).any() or (host > shape.seq).any():
+            raise ShapeError(f"invalid shape: valid_len outside [0, {shape.seq}]")
+        if (host != shape.seq).any():
+            keep = valid_len = torch.from_numpy(host).to(device)
+    args.append(None if valid_len is None else ptr("valid_len", valid_len, shape.batch, torch.int32))
+    args.append(b)
+    if backward:
+        args.append(dtable_ptr)
+    if workspace is not None and (not isinstance(workspace, torch.Tensor) or not workspace.is_contiguous()
+                                  or workspace.device != device):
+        raise TypeError("the workspace must be a contiguous CUDA tensor on the tensors' device")
+
+    def launch(handle):
+        # Memory that is taken here is taken on the call's stream, so the allocator orders its next use.
+        ws = workspace
+        if ws is None:
+            ws = torch.empty(_train_bytes(d, b, backward), dtype=torch.uint8, device=device)
+        status = call(d, *args, ws.data_ptr() or None, ws.numel() * ws.element_size(), handle)
+        if status != _lib.OK:
+            _check(status)
+        if keep is not None:  # keep the uploaded lengths alive until the kernels have run
+            _sync(handle)
+
+    if stream is None and device.index == torch.cuda.current_device():
+        launch(torch.cuda.current_stream(device.index).cuda_stream)
+        return
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    elif not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    if stream.device != device:
+        raise TypeError(f"the stream is on {stream.device}, the tensors are on {device}")
+    with torch.cuda.stream(stream):
+        launch(stream.cuda_stream)
 
 
 STAGE_NAMES = ("qk", "softmax", "pv", "k_wait", "v_wait", "refill", "tiles", "total")

@@ -39,7 +39,7 @@ struct TrainArgs {
   float* dk;
   float* dv;
   const float* rel_bias;   // [heads][2 * rel_half]: bias * log2(e) of rel = index - rel_half, or nullptr
-  const uint8_t* rel_id;   // [2 * rel_half]: its bucket
+  const uint8_t* rel_id;   // [2 * rel_half]: its bucket (the row-wise kernels)
   int rel_half;
   int buckets;
   float scale;
@@ -73,15 +73,15 @@ struct BucketBounds {
 };
 
 // The bias by distance: vec[head][rel + half] = table[head][bucket(rel)] *
-// log2(e), ids[rel + half] = bucket(rel).  One thread per (head, rel); heads
-// * 2 * half floats, once per call, so that the attention kernels copy the
-// slice that a tile needs instead of searching buckets (~1 us at seq 8192
-// with 16 heads).
-__global__ void __launch_bounds__(256) rel_table_kernel(const float* __restrict__ table, int heads, int buckets,
-                                                        int half, const __grid_constant__ BucketBounds b,
-                                                        float* __restrict__ vec, uint8_t* __restrict__ ids) {
+// log2(e), and where ids is given ids[rel + half] = bucket(rel).  Thread
+// `first` of `step` takes every step-th distance; once per call, so that the
+// attention kernels copy the slice that a tile needs instead of searching
+// buckets.
+__device__ __forceinline__ void rel_table(const float* __restrict__ table, int heads, int buckets, int half,
+                                          const BucketBounds& b, float* __restrict__ vec, uint8_t* __restrict__ ids,
+                                          long long first, long long step) {
   const long long n = 2ll * half;
-  for (long long t = blockIdx.x * 256ll + threadIdx.x; t < n; t += gridDim.x * 256ll) {
+  for (long long t = first; t < n; t += step) {
     const int rel = static_cast<int>(t - half), dist = rel < 0 ? -rel : rel;
     int lo = 0, hi = buckets / 2 - 1;  // the last bound at or below dist
     while (lo < hi) {
@@ -92,12 +92,16 @@ __global__ void __launch_bounds__(256) rel_table_kernel(const float* __restrict_
         hi = mid - 1;
     }
     const int id = lo + (rel > 0 ? buckets / 2 : 0);
-    for (int h = blockIdx.y; h < heads; h += gridDim.y) {
+    for (int h = 0; h < heads; ++h) {
       const float x = table[static_cast<size_t>(h) * buckets + id];
       vec[static_cast<size_t>(h) * n + t] = x <= kMaskedBias ? -INFINITY : x * kLog2e;
     }
-    if (blockIdx.y == 0) ids[t] = static_cast<uint8_t>(id);
+    if (ids) ids[t] = static_cast<uint8_t>(id);
   }
+}
+__global__ void __launch_bounds__(256) rel_table_kernel(const float* table, int heads, int buckets, int half,
+                                                        const __grid_constant__ BucketBounds b, float* vec, uint8_t* ids) {
+  rel_table(table, heads, buckets, half, b, vec, ids, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
 }
 
 // dtable[head][b] = the sum of its partials over the batch and the parts of

@@ -166,9 +166,16 @@ struct TrainIo {
   const int32_t* valid_len;
 };
 
-raya_attn_status launch_rowwise(const TrainPlan& plan, train::TrainArgs t, void* workspace, cudaStream_t stream,
-                                bool backward) {
+raya_attn_status launch_rowwise(const TrainPlan& plan, train::TrainArgs t, const float* table,
+                                const train::BucketBounds& bounds, void* workspace, cudaStream_t stream, bool backward) {
   const unsigned grid = static_cast<unsigned>(static_cast<long long>(t.a.batch) * t.a.heads * plan.parts);
+  if (table) {
+    const unsigned blocks = static_cast<unsigned>(std::min<long long>((2ll * plan.rel_half + 255) / 256, 1024));
+    train::rel_table_kernel<<<blocks, 256, 0, stream>>>(table, t.a.heads, t.buckets, plan.rel_half, bounds,
+                                                        at<float>(workspace, plan.rel_bias), at<uint8_t>(workspace, plan.rel_id));
+    const raya_attn_status st = check_launch("bias table launch");
+    if (st != RAYA_ATTN_OK) return st;
+  }
   if (!backward) {
     train::rowwise_train_fwd<<<grid, train::kRowThreads, 0, stream>>>(t);
     return check_launch("forward launch");
@@ -182,22 +189,43 @@ raya_attn_status launch_rowwise(const TrainPlan& plan, train::TrainArgs t, void*
   return check_launch("key gradient launch");
 }
 
+// A 3-D tensor map over a [slices][seq][head_dim] fp32 output with boxes of
+// [1][32 rows][32 floats], 128-byte swizzle: a store clips rows past seq and
+// columns past head_dim.
+raya_attn_status encode_out(CUtensorMap* map, float* base, uint64_t head_dim, uint64_t seq, uint64_t slices) {
+  raya_attn_status st = load_encoder();
+  if (st != RAYA_ATTN_OK) return st;
+  const cuuint64_t gdim[3] = {head_dim, seq, slices};
+  const cuuint64_t gstride[2] = {head_dim * sizeof(float), seq * head_dim * sizeof(float)};
+  const cuuint32_t box[3] = {32, 32, 1};
+  const cuuint32_t estride[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, gdim, gstride, box, estride,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(RAYA_ATTN_ERR_CUDA, "cuda: cuTensorMapEncodeTiled (output) failed (%d)", static_cast<int>(r));
+  return RAYA_ATTN_OK;
+}
+
 // Chunk by chunk: the images of its slices, then every 128-row tile of them.
 template <int P>
-raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, const train::BucketBounds& bounds,
+raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, const float* table, const train::BucketBounds& bounds,
                            void* workspace, int sms, cudaStream_t stream, bool backward) {
   train::TcArgs c{};
   c.t = t;
   c.tiles = plan.tiles;
+  c.backward = backward;
   for (int i = 0; i < (backward ? 4 : 3); ++i) c.img[i] = at<uint8_t>(workspace, plan.img[i]);
   c.exps = at<int4>(workspace, plan.exps);
   if (backward) c.rows = at<float>(workspace, plan.rows);
   c.next = at<unsigned>(workspace, plan.next);
+  c.table = table;
+  c.vec = at<float>(workspace, plan.rel_bias);
+  c.bounds = bounds;
   c.far = plan.far;
   const size_t smem = train::tc_smem<P>();
   size_t dist = 0;
   if (t.part) {
-    c.bounds = bounds;
     c.slots = plan.slots;
     if (plan.dist_bytes > 0)
       c.dist = at<float>(workspace, plan.dist);
@@ -210,24 +238,37 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   for (c.slice0 = 0; c.slice0 < slices; c.slice0 += plan.chunk) {
     const long long n = std::min(plan.chunk, slices - c.slice0) * plan.tiles;
     c.units = static_cast<unsigned>(n / 2);
-    train::split_kernel<P><<<dim3(static_cast<unsigned>(n), backward ? 4 : 3), 256, 0, stream>>>(c);
+    train::split_kernel<P><<<dim3(static_cast<unsigned>(n), (backward ? 4 : 3) + (bias ? 1 : 0)), 256, 0, stream>>>(c);
     raya_attn_status st = check_launch("operand split launch");
     if (st != RAYA_ATTN_OK) return st;
-    auto launch_kind = [&](void (*fn)(train::TcArgs), size_t shared, const char* what) {
-      fn<<<static_cast<unsigned>(std::min(n / 2, resident)), train::tc_threads(P), shared, stream>>>(c);
-      return check_launch(what);
+    auto launch_kind = [&](void (*fn)(train::TcArgs, CUtensorMap), size_t shared, float* out, const char* what) {
+      CUtensorMap map;
+      const raya_attn_status encoded = encode_out(&map, out, t.a.head_dim, t.a.seq, slices);
+      if (encoded != RAYA_ATTN_OK) return encoded;
+      cudaLaunchAttribute overlap{};  // with the end of the launch before (train_tc.cuh)
+      overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      overlap.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(static_cast<unsigned>(std::min(n / 2, resident)));
+      config.blockDim = dim3(train::tc_threads(P));
+      config.dynamicSmemBytes = shared;
+      config.stream = stream;
+      config.attrs = &overlap;
+      config.numAttrs = 1;
+      const cudaError_t e = cudaLaunchKernelEx(&config, fn, c, map);
+      return e == cudaSuccess ? check_launch(what) : cuda_fail(e, what);
     };
     using train::tc_train;
     if (!backward) {
-      st = launch_kind(bias ? tc_train<train::kForward, P, true> : tc_train<train::kForward, P, false>, smem, "forward launch");
+      st = launch_kind(bias ? tc_train<train::kForward, P, true> : tc_train<train::kForward, P, false>, smem, t.a.out, "forward launch");
       if (st != RAYA_ATTN_OK) return st;
       continue;
     }
-    st = launch_kind(bias ? tc_train<train::kDq, P, true> : tc_train<train::kDq, P, false>, smem + dist, "query gradient launch");
+    st = launch_kind(bias ? tc_train<train::kDq, P, true> : tc_train<train::kDq, P, false>, smem + dist, t.dq, "query gradient launch");
     if (st == RAYA_ATTN_OK)
-      st = launch_kind(bias ? tc_train<train::kDk, P, true> : tc_train<train::kDk, P, false>, smem, "key gradient launch");
+      st = launch_kind(bias ? tc_train<train::kDk, P, true> : tc_train<train::kDk, P, false>, smem, t.dk, "key gradient launch");
     if (st == RAYA_ATTN_OK)
-      st = launch_kind(bias ? tc_train<train::kDv, P, true> : tc_train<train::kDv, P, false>, smem, "value gradient launch");
+      st = launch_kind(bias ? tc_train<train::kDv, P, true> : tc_train<train::kDv, P, false>, smem, t.dv, "value gradient launch");
     if (st != RAYA_ATTN_OK) return st;
   }
   return RAYA_ATTN_OK;
@@ -282,22 +323,15 @@ raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const ra
     bounds = bucket_bounds(bias->buckets, bias->max_distance);
     t.rel_half = plan.rel_half;
     t.buckets = bias->buckets;
-    float* vec = at<float>(workspace, plan.rel_bias);
-    uint8_t* ids = at<uint8_t>(workspace, plan.rel_id);
-    t.rel_bias = vec;
-    t.rel_id = ids;
-    const dim3 blocks(static_cast<unsigned>(std::min<long long>((2ll * plan.rel_half + 255) / 256, 1024)),
-                      static_cast<unsigned>(std::min<int64_t>(d->heads, 64)));
-    train::rel_table_kernel<<<blocks, 256, 0, stream>>>(bias->table, static_cast<int>(d->heads), bias->buckets,
-                                                        plan.rel_half, bounds, vec, ids);
-    if ((st = check_launch("bias table launch")) != RAYA_ATTN_OK) return st;
+    t.rel_bias = at<float>(workspace, plan.rel_bias);
+    t.rel_id = at<uint8_t>(workspace, plan.rel_id);
   }
   if (io.dtable) t.part = at<float>(workspace, plan.part);
   if (plan.panels > 0)
-    st = plan.panels == 1 ? launch_tc<1>(plan, t, bounds, workspace, ctx->sms, stream, backward)
-                          : launch_tc<2>(plan, t, bounds, workspace, ctx->sms, stream, backward);
+    st = plan.panels == 1 ? launch_tc<1>(plan, t, bias ? bias->table : nullptr, bounds, workspace, ctx->sms, stream, backward)
+                          : launch_tc<2>(plan, t, bias ? bias->table : nullptr, bounds, workspace, ctx->sms, stream, backward);
   else
-    st = launch_rowwise(plan, t, workspace, stream, backward);
+    st = launch_rowwise(plan, t, bias ? bias->table : nullptr, bounds, workspace, stream, backward);
   if (st != RAYA_ATTN_OK) return st;
   if (io.dtable) {
     train::bias_grad_kernel<<<dim3(static_cast<unsigned>(d->heads), static_cast<unsigned>(bias->buckets)), 256, 0, stream>>>(

@@ -96,12 +96,16 @@ struct TcArgs {
   uint8_t* img[4];     // [chunk slices][tiles][2 P panels]: q, k, v, dout
   int4* exps;          // [chunk slices][tiles]: their exponents
   float* rows;         // [chunk slices][tiles][3][64]: m * log2(e) (inf: no key), that - kWeightLog2, and delta / l
+  const float* table;  // the bias, or nullptr
+  float* vec;          // where it goes by distance (t.rel_bias)
   int tiles;           // 64-row tiles per slice (even)
+  bool backward;
   long long slice0;
   unsigned units;      // 128-row tiles of the chunk
   unsigned* next;      // [4] by kind: units handed out beyond the first one of each CTA; split_kernel clears them
-  BucketBounds bounds; // with t.part, and the rest of the table's gradient:
+  BucketBounds bounds;
   int far;             // the last bucket's first distance
+  // With t.part, the table's gradient:
   int slots;           // distances kept apart: -far - 63 ... far + 64
   float* dist;         // [CTAs][row warps][slots] where shared memory does not hold them, or nullptr
 };
@@ -111,21 +115,45 @@ __device__ __forceinline__ int valid_of(const AttnArgs& a, long long bh) {
   return v < 0 ? 0 : (v > a.seq ? a.seq : v);
 }
 
+// Programmatic dependent launch.  A kernel that says launch_dependents lets the
+// next one's CTAs start where it leaves room; wait_for_primary returns when
+// the kernel before is complete and its writes are visible.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // 64 rows of one tensor into their image.  256 threads: 16 lanes take a row's
 // 64 columns of a panel (16-byte loads, 8-byte stores), 16 rows at a time.
-// blockIdx.y: the tensor.  Bound by HBM: 4 bytes read and 4 written per
+// blockIdx.y: the tensor, and behind them the bias by distance.  Tiles of padding write the zeros of the results
+// there instead.  Bound by HBM: 4 bytes read and 4 written per
 // element (dout: 8 read).
 template <int P>
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcArgs c) {
   __shared__ uint32_t red[8];
   const AttnArgs& a = c.t.a;
   const int tid = threadIdx.x, which = blockIdx.y, d = a.head_dim;
+  launch_dependents();
+  if (which == 4 || (which == 3 && !c.backward)) {
+    rel_table(c.table, a.heads, c.t.buckets, c.t.rel_half, c.bounds, c.vec, nullptr, blockIdx.x * 256ll + tid,
+              gridDim.x * 256ll);
+    return;
+  }
   const long long local = blockIdx.x / static_cast<unsigned>(c.tiles), bh = c.slice0 + local;
   const int tile = static_cast<int>(blockIdx.x - local * c.tiles);
   if (blockIdx.x == 0 && which == 0 && tid < 4) c.next[tid] = 0;
   const int valid = valid_of(a, bh);
   const int r0 = tile * 64;
-  if (r0 >= (valid + 127) / 128 * 128) return;  // no 128-row tile reads it
+  if (r0 >= (valid + 127) / 128 * 128) {  // no 128-row tile reads it: padding, whose results are zero
+    float* o = which == kImgQ ? (c.backward ? c.t.dq : a.out) : which == kImgK ? c.t.dk : which == kImgV ? c.t.dv : nullptr;
+    if (!c.backward && which != kImgQ) o = nullptr;
+    const size_t first = static_cast<size_t>(bh) * a.seq + r0;
+    const int rows = min(64, a.seq - r0);
+    if (o)
+      for (int i = tid; i < rows * d / 4; i += 256) st_stream(o + first * d + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f));
+    if (!c.backward && which == kImgQ && c.t.stats_out && tid < rows) c.t.stats_out[first + tid] = make_float2(-INFINITY, 0.f);
+    if (c.t.part && which == kImgQ && tile % 2 == 0 && tid < c.t.buckets)
+      c.t.part[(static_cast<size_t>(bh) * c.t.parts + tile / 2) * c.t.buckets + tid] = 0.f;
+    return;
+  }
   const float* src = which == kImgQ ? a.q : which == kImgK ? a.k : which == kImgV ? a.v : c.t.dout;
   src += static_cast<size_t>(bh) * a.seq * d;
   const float* out = a.out + static_cast<size_t>(bh) * a.seq * d;
@@ -201,7 +229,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
 struct TcUnit {
   int local;   // slice within the chunk
   int valid, r0;
-  int t0, n;   // 64-column tiles [t0, t0 + n) that its rows see; n = 0: padding only, -1: no more units
+  int t0, n;   // 64-column tiles [t0, t0 + n) that its rows see; n = 0: padding only (not queued), -1: no more units
 };
 
 // Shared memory behind the operand stages.
@@ -216,19 +244,24 @@ struct alignas(16) TcTail {
   uint64_t u_full[kQueue], u_free[kQueue];
   uint64_t full[kStages], freed[kStages];
   uint64_t s_full[2], w_ready[2], part_full, part_free, a_ready;
+  uint64_t rows_full[8];          // by row warp
   uint32_t tmem_base;
   int abort_flag;
 };
 
 template <int P>
 constexpr size_t stage_bytes() { return 2ull * 2 * P * kPanelBytes; }
-// Each row warp's 32 x 32 words: rows on their way between global memory and
-// the threads.  The pitch lets 8 lanes access 16 bytes of 8 rows, or of one,
-// without a bank conflict.
-constexpr int kPitch = 36;
+// Each row warp's buffer: two blocks of 32 rows x 128 bytes under the 128-byte
+// swizzle.  The next unit's rows come in through it by bulk copies, the
+// output leaves through it by tensor stores (which clip rows past seq and
+// columns past head_dim), and neither holds the row threads up: with loads
+// and stores of their own these took 5 to 7k of a unit's 30k cycles.
+constexpr int kBlockBytes = 32 * 128, kRowBuf = 2 * kBlockBytes;
+constexpr int kPitch = 36;  // diagonal_sums: words per row
+static_assert(32 * kPitch * 4 <= kRowBuf, "the diagonal sums' block");
 template <int P>
 constexpr size_t tc_smem() {
-  return 1024 + kStages * stage_bytes<P>() + sizeof(TcTail) + kRowWarpsOf(P) * 32 * kPitch * sizeof(float);
+  return 1024 + kStages * stage_bytes<P>() + kRowWarpsOf(P) * kRowBuf + sizeof(TcTail);
 }
 // head_dim <= 64: two CTAs (2 x 256 tensor-memory columns) share an SM and a
 // third does not fit beside them.
@@ -237,6 +270,10 @@ static_assert(tc_smem<1>() <= kHalfSm && tc_smem<1>() > 233472 / 3 && tc_smem<2>
 
 // A product of scales that would be infinite, as the largest float: 0 times it is 0.
 __device__ __forceinline__ float finite(float x) { return fmaxf(fminf(x, 3.4028235e38f), -3.4028235e38f); }
+
+__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 
 // Weights w[32] (fp32, already scaled) as fp16 hi and lo over their scores.
 __device__ __forceinline__ void store_weights(uint32_t taddr, const float* w) {
@@ -285,31 +322,6 @@ __device__ __forceinline__ void mask_scores(float* s, float mult, const float* v
   }
 }
 
-// 32 x 32 words between rows and lanes: the warp's 32 rows of 128 bytes at
-// `src` (swizzled within each 8 rows) into this lane's row w[32], through the
-// warp's buffer.  Eight lanes load a row's line.
-__device__ __forceinline__ void gather_rows(const uint8_t* src, uint4* x, int lane) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(src + (4 * i + (lane >> 3)) * 128 + (lane & 7) * 16);
-}
-__device__ __forceinline__ void turn_rows(float* buf, const uint4* x, int lane, uint32_t* w) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (lane >> 3);
-    *reinterpret_cast<uint4*>(buf + r * kPitch + (((lane & 7) ^ (r & 7)) << 2)) = x[i];
-  }
-  __syncwarp();
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint4 y = *reinterpret_cast<const uint4*>(buf + lane * kPitch + 4 * k);
-    w[4 * k] = y.x;
-    w[4 * k + 1] = y.y;
-    w[4 * k + 2] = y.z;
-    w[4 * k + 3] = y.w;
-  }
-  __syncwarp();
-}
-
 // The sums along the diagonals of a 32 x 32 block whose row `lane` is s[32]:
 // before is the sum of column - row = lane - 31, after that of lane + 1.
 // Lane k reads column (k + 1 + row) mod 32 of every row: no bank conflict.
@@ -332,15 +344,22 @@ __device__ __forceinline__ void diagonal_sums(float* buf, const float* s, int la
   __syncwarp();
 }
 
+// The launches of a call overlap.  kForward and kDq start while split_kernel
+// ends and wait for it before they read what it wrote; kDk and kDv start
+// where the gradient before leaves room, which is after it waited for
+// split_kernel itself, so they wait for it only before they end (a kernel
+// behind them is to find all three complete).
+//
 // Persistent: the copy warp takes one unit after the other (the first by
 // blockIdx, the others from a counter, since padding makes them uneven) and
 // hands them to the other warps.  Every barrier and ring runs on across them:
 // G counts the CTA's 64-column tiles, U its units with any.
 template <int KIND, int P, bool BIAS>
-__global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const __grid_constant__ TcArgs c) {
+__global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const __grid_constant__ TcArgs c, const __grid_constant__ CUtensorMap out_map) {
   using namespace tc32;
   constexpr bool kScores2 = KIND == kDq || KIND == kDk;      // S and dP, serial
   constexpr bool kByKey = KIND == kDk || KIND == kDv;        // rows are keys, columns queries
+  constexpr bool kBehindSplit = !kByKey;                     // the launch before is split_kernel
   constexpr int kHalves = P;                                 // threads per row
   constexpr int kW = 64 / kHalves;                           // score columns of a thread
   constexpr int kBlocks = kW / 32;
@@ -360,8 +379,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
 
   extern __shared__ unsigned char raw[];
   unsigned char* const smem = raw + (((smem_addr(raw) + 1023u) & ~1023u) - smem_addr(raw));
-  TcTail& sm = *reinterpret_cast<TcTail*>(smem + kStages * stage_bytes<P>());
-  float* const row_bufs = reinterpret_cast<float*>(&sm + 1);
+  unsigned char* const row_bufs = smem + kStages * stage_bytes<P>();
+  TcTail& sm = *reinterpret_cast<TcTail*>(row_bufs + kRowWarpsOf(P) * kRowBuf);
 
   const AttnArgs& a = c.t.a;
   const int tid = threadIdx.x, warp = tid >> 5, d = a.head_dim;
@@ -379,6 +398,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     mbar_init(&sm.part_full, 1);
     mbar_init(&sm.part_free, kRowThreadsTc);
     mbar_init(&sm.a_ready, kRowThreadsTc);
+    for (int s = 0; s < kIssueWarp; ++s) mbar_init(&sm.rows_full[s], 1);
     for (int s = 0; s < kQueue; ++s) {
       mbar_init(&sm.u_full[s], 1);
       mbar_init(&sm.u_free[s], kIssueWarp + 1);
@@ -427,59 +447,70 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs(P)));
   if (warp < kIssueWarp) {
     // ---------------- rows ----------------
+    if constexpr (kBehindSplit) wait_for_primary();
     const int half = warp >> 2, rt = tid & 127, ln = tid & 31;
-    float* const buf = row_bufs + warp * 32 * kPitch;
+    unsigned char* const buf = row_bufs + warp * kRowBuf;
     const uint32_t lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    float* const outp = KIND == kForward ? a.out : KIND == kDq ? c.t.dq : KIND == kDk ? c.t.dk : c.t.dv;
     constexpr int kStep = kByKey ? -1 : 1;
     // Where the thread's first column finds its distance: j - i relative to
     // the tile's first one (kByKey: i runs with the column, so backwards).
     const int vec_at = (kByKey ? rt + 64 : 128 - rt) + kStep * kW * half;
 
-    // The next unit with columns; the rows of those without are padding and
-    // get their zeros on the way.
-    auto next_unit = [&](TcUnit& u) {
-      for (;;) {
-        if (!take_unit(u)) return false;
-        if (u.n != 0) return true;
-        const int rows = min(kTileRows, a.seq - u.r0);
-        const size_t first = static_cast<size_t>(c.slice0 + u.local) * a.seq + u.r0;
-        float* o = outp + first * d;
-        for (int i = tid; i < rows * d / 4; i += kRowThreadsTc) st_stream(o + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f));
-        if (KIND == kForward && c.t.stats_out && tid < rows) c.t.stats_out[first + tid] = make_float2(-INFINITY, 0.f);
-        if (with_grad && tid < c.t.buckets)
-          c.t.part[(static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets + tid] = 0.f;
-        __syncwarp();
-      }
-    };
     // What a row needs besides its operands: 2^-e of these, the columns that
     // it sees, and for kDq its exponent and delta.
     struct Row {
       float qmul, unit, off, delta;
       int lo, hi;
     };
-    // Unit u's rows into tensor memory.  Called while the last tile of the
-    // unit before is in its second product: its scores are complete.
+    // Unit u's rows, in rounds of two 32-word pieces of a thread (hi and lo
+    // panels of the first operand, then of the second): from the images into
+    // the warp's buffer, and on into tensor memory.
+    constexpr int kRounds = (kScores2 ? 2 : 1) * P / kHalves;
+    int fetched = 0;
+    bool in_flight = false;
+    auto fetch_rows = [&](const TcUnit& u, int round) {
+      fence_proxy_async_smem();  // the warp's own accesses of the buffer, before the copies
+      __syncwarp();
+      if (ln == 0) {
+        tma_store_wait_read();  // and the last unit's way out
+        const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64 + ((warp & 3) >> 1);
+        mbar_arrive_expect_tx(&sm.rows_full[warp], kRowBuf);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int piece = (half * kRounds + round) * 2 + p;
+          tma_load_1d(buf + p * kBlockBytes,
+                      c.img[piece < 2 * P ? kA1 : kA2] + tile * static_cast<long long>(kOp) +
+                          piece % (2 * P) * kPanelBytes + (warp & 1) * kBlockBytes,
+                      kBlockBytes, &sm.rows_full[warp]);
+        }
+      }
+      __syncwarp();
+      in_flight = true;
+    };
+    auto place_rows = [&](int round) {
+      if (!warp_wait(&sm.rows_full[warp], fetched)) return false;
+      in_flight = false;
+      ++fetched;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        float w[32];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(buf + p * kBlockBytes + ln * 128 + ((k ^ (ln & 7)) << 4));
+          w[4 * k] = x.x;
+          w[4 * k + 1] = x.y;
+          w[4 * k + 2] = x.z;
+          w[4 * k + 3] = x.w;
+        }
+        tmem_st32(lane + 32 * ((half * kRounds + round) * 2 + p), w);
+      }
+      return true;
+    };
+    // The rest of a unit's rows (its first round is on the way) and what goes
+    // with them.  Called when the scores of the unit before are complete.
     auto load_rows = [&](const TcUnit& u, Row& r) {
       const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64 + ((warp & 3) >> 1);
       const int4 e = c.exps[tile];
-      constexpr int kParts = (kScores2 ? 4 : 2) * P / kHalves;  // 32-word pieces of this thread
-#pragma unroll
-      for (int p0 = 0; p0 < kParts; p0 += 2) {  // two in flight
-        uint4 x[2][8];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int piece = half * kParts + p0 + p;  // hi and lo panels of the first operand, then of the second
-          gather_rows(c.img[piece < 2 * P ? kA1 : kA2] + tile * static_cast<long long>(kOp) +
-                          piece % (2 * P) * kPanelBytes + (warp & 1) * 32 * 128, x[p], ln);
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          uint32_t w[32];
-          turn_rows(buf, x[p], ln, w);
-          tmem_st32(lane + 32 * (half * kParts + p0 + p), reinterpret_cast<const float*>(w));
-        }
-      }
       r.qmul = a.qscale * tc16::pow2(-(kByKey ? e.y : e.x));
       r.unit = kScores2 ? tc16::pow2(-(kByKey ? e.z : e.w)) : 0.f;
       r.off = r.delta = 0.f;
@@ -488,9 +519,15 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         r.delta = c.rows[tile * kRowValues + 128 + (rt & 63)];
       }
       key_range(a, min(u.r0 + rt, u.valid - 1), u.valid, r.lo, r.hi);
+#pragma unroll 1
+      for (int round = 0; round < kRounds; ++round) {
+        if (round > 0) fetch_rows(u, round);
+        if (!place_rows(round)) return false;
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&sm.a_ready);
+      return true;
     };
 
     TcUnit u, nu;
@@ -501,9 +538,12 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     // beyond the last bucket's bound on either side.
     float* const dist = !with_grad ? nullptr
                         : c.dist   ? c.dist + (static_cast<size_t>(blockIdx.x) * kIssueWarp + warp) * c.slots
-                                   : row_bufs + kIssueWarp * 32 * kPitch + warp * c.slots;
-    ok = next_unit(u);
-    if (u.n > 0) load_rows(u, r);
+                                   : reinterpret_cast<float*>(&sm + 1) + warp * c.slots;
+    ok = take_unit(u);
+    if (u.n > 0) {
+      fetch_rows(u, 0);
+      ok = load_rows(u, r);
+    }
     while (ok && u.n > 0) {
       const int row = u.r0 + rt;
       const size_t first_row = static_cast<size_t>(c.slice0 + u.local) * a.seq + u.r0;
@@ -515,6 +555,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       float factor = 0.f;  // of the partial that is in flight
       if (with_grad) {
         for (int i = ln; i < c.slots; i += 32) dist[i] = 0.f;
+        if (ln == 0) tma_store_wait_read();  // the diagonal sums use the buffer
         __syncwarp();
       }
 
@@ -543,15 +584,21 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         return true;
       };
       nu.n = -1;
-      // After the last tile's scores: the next unit's rows.
+      // The next unit's rows: begun before the last tile (with the table's
+      // gradient behind it, since that uses the buffer), placed behind it.
+      auto begin_next = [&] {
+        if (ok && take_unit(nu) && nu.n > 0) fetch_rows(nu, 0);
+      };
       auto prepare_next = [&](int t) {
         if (t + 1 < u.n) return;
-        if (next_unit(nu) && nu.n > 0) load_rows(nu, nr);
+        if (with_grad) begin_next();
+        if (ok && nu.n > 0) ok = load_rows(nu, nr);
       };
 
       for (int t = 0; t < u.n; ++t, ++G) {
         const int st = G % kStages, c0 = (u.t0 + t) * kTileCols + kW * half;
         const int sb = kScores2 ? 0 : G & 1;
+        if (!with_grad && t + 1 == u.n) begin_next();
         if (ok) ok = warp_wait(&sm.full[st], G / kStages) && warp_wait(&sm.s_full[sb], kScores2 ? G : G >> 1);
         if (!kShared && !ok) break;
         tc_fence_after();
@@ -686,7 +733,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
                     far_before += x;
                 } else {
                   float before, after;
-                  diagonal_sums(buf, s, ln, before, after);
+                  diagonal_sums(reinterpret_cast<float*>(buf), s, ln, before, after);
                   float* at = dist + base + c.far + 63;
                   at[ln - 31] += before;
                   at[ln + 1] += after;  // lane 31: 0, one slot past the block's distances
@@ -712,7 +759,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
           mbar_arrive(&sm.w_ready[sb]);
           factor = finite(tc16::pow2(-e) * tc16::pow2(-e1));
           prepare_next(t);
-          ok = add_partial(G);
+          if (ok) ok = add_partial(G);
         }
       }
       if constexpr (!kScores2)
@@ -770,33 +817,37 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       }
       if (!ok) break;
       {
-        // The warp's rows, 32 columns at a time, through its buffer: eight lanes store 128 bytes of a row.
         const bool live = row < u.valid;
-        const int wr0 = (warp & 3) * 32, wrows = min(32, a.seq - u.r0 - wr0);
-        float* dst = outp + (first_row + wr0) * d + kOutCols * half + (ln & 7) * 4;
+        const int wr0 = u.r0 + (warp & 3) * 32;
 #pragma unroll
         for (int q = 0; q < kOutCols; q += 32) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(buf + ln * kPitch + i) =
+            *reinterpret_cast<float4*>(buf + q * 128 + ln * 128 + (((i >> 2) ^ (ln & 7)) << 4)) =
                 live ? make_float4(o[q + i] * f, o[q + i + 1] * f, o[q + i + 2] * f, o[q + i + 3] * f)
                      : make_float4(0.f, 0.f, 0.f, 0.f);
-          __syncwarp();
-          float4 x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            x[i] = *reinterpret_cast<const float4*>(buf + (4 * i + (ln >> 3)) * kPitch + (ln & 7) * 4);
-          if (kOutCols * half + q + (ln & 7) * 4 < d) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (4 * i + (ln >> 3) < wrows) st_stream(dst + static_cast<size_t>(4 * i + (ln >> 3)) * d + q, x[i]);
-          }
-          __syncwarp();
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (ln == 0 && wr0 < a.seq) {
+#pragma unroll
+          for (int q = 0; q < kOutCols; q += 32)
+            if (kOutCols * half + q < d)
+              tma_store_3d(&out_map, buf + q * 128, kOutCols * half + q, wr0, static_cast<int>(c.slice0 + u.local));
+          tma_store_commit();
+        }
+        __syncwarp();
       }
       u = nu;
       r = nr;
     }
+    if (ln == 0) tma_store_wait_read();
+    if (in_flight) {  // only after a timeout: bounded, as the drains below
+      const long long t_end = clock64() + a.timeout_cycles;
+      while (!mbar_try_wait(&sm.rows_full[warp], fetched & 1u) && clock64() < t_end) {
+      }
+    }
+    __syncwarp();
   } else if (warp == kIssueWarp) {
     // ---------------- MMA issue ----------------
     auto commit = [&](uint64_t* bar, uint32_t parity) {
@@ -848,9 +899,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     int G = 0, U = 0;
     bool ok = true;
     TcUnit u;
-    while (ok && take_unit(u) && u.n >= 0) {
+    while (ok && take_unit(u) && u.n > 0) {
       const int n = u.n;
-      if (n == 0) continue;
       ok = warp_wait(&sm.a_ready, U++);
       for (int t = 0; ok && t < n; ++t, ++G) {
         if constexpr (kScores2) {
@@ -891,13 +941,9 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     for (int g = max(0, committed - kStages); ok && g < committed; ++g) ok = warp_wait(&sm.freed[g % kStages], g / kStages);
   } else if (warp == kIssueWarp + 1) {
     // ---------------- units and bulk copies ----------------
-    bool ok = true;
-    for (int k = 0; ok; ++k) {
-      unsigned unit = blockIdx.x;
-      if (k > 0) {
-        if ((tid & 31) == 0) unit = gridDim.x + atomicAdd(c.next + KIND, 1u);
-        unit = __shfl_sync(0xffffffffu, unit, 0);
-      }
+    bool ok = true, first = true;
+    unsigned unit = blockIdx.x;
+    for (int k = 0; ok;) {
       TcUnit u{0, 0, 0, 0, -1};
       if (unit < c.units) {
         const unsigned tiles = static_cast<unsigned>(c.tiles) / 2;
@@ -912,13 +958,29 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         u.t0 = lo / kTileCols;
         u.n = hi > lo ? (hi + kTileCols - 1) / kTileCols - u.t0 : 0;
       }
+      if (first) {
+        if constexpr (kBehindSplit) wait_for_primary();
+        if constexpr (KIND == kDq || KIND == kDk) launch_dependents();
+        first = false;
+      }
+      if ((tid & 31) == 0) unit = gridDim.x + atomicAdd(c.next + KIND, 1u);  // the next one, used a unit later
+      if (u.n == 0) {  // padding only: split_kernel has written its zeros
+        unit = __shfl_sync(0xffffffffu, unit, 0);
+        continue;
+      }
       if (k >= kQueue) ok = warp_wait(&sm.u_free[k % kQueue], k / kQueue - 1);
       if (!ok) break;
       if ((tid & 31) == 0) {
         sm.unit[k % kQueue] = u;
         mbar_arrive(&sm.u_full[k % kQueue]);
+        if (u.n > 0) {  // its rows, a unit ahead of their use
+          const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64;
+          prefetch_l2(c.img[kA1] + tile * static_cast<long long>(kOp), 2 * kOp);
+          if constexpr (kScores2) prefetch_l2(c.img[kA2] + tile * static_cast<long long>(kOp), 2 * kOp);
+        }
       }
       __syncwarp();
+      ++k;
       if (u.n < 0) break;
       const int head = static_cast<int>((c.slice0 + u.local) % a.heads);
       for (int t = 0; t < u.n; ++t) {
@@ -944,6 +1006,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         __syncwarp();
         ++copied;
       }
+      unit = __shfl_sync(0xffffffffu, unit, 0);
     }
   }
   __syncwarp();
@@ -965,6 +1028,9 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
   if (warp == kIssueWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+  }
+  if constexpr (!kBehindSplit) {
+    if (tid == 0) wait_for_primary();
   }
 }
 
