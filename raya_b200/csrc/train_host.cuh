@@ -125,7 +125,7 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
       plan->far = static_cast<int>(std::min<int64_t>(bucket_bounds(bias->buckets, bias->max_distance).at[bias->buckets / 2 - 1], d->seq));
     if (backward && bias) {
       plan->slots = 2 * plan->far + 128;
-      const size_t warps = train::kRowWarpsOf(plan->panels), bytes = warps * plan->slots * sizeof(float);
+      const size_t bytes = size_t{2} * plan->slots * sizeof(float);
       const size_t spare = plan->panels == 1 ? train::kHalfSm - train::tc_smem<1>() : train::kWholeSm - train::tc_smem<2>();
       if (bytes > spare) {
         plan->dist_bytes = kMaxResident * bytes;
@@ -230,7 +230,7 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
     if (plan.dist_bytes > 0)
       c.dist = at<float>(workspace, plan.dist);
     else
-      dist = static_cast<size_t>(train::kRowWarpsOf(P)) * plan.slots * sizeof(float);
+      dist = size_t{2} * plan.slots * sizeof(float);
   }
   const long long resident = std::min(kMaxResident, static_cast<long long>(sms) * (P == 1 ? 2 : 1));
   const bool bias = t.rel_bias != nullptr;

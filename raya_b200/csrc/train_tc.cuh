@@ -74,10 +74,10 @@ constexpr int tc_threads(int panels) { return 128 * panels + 128; }
 // Registers (setmaxnreg): a row thread holds a row of scores next to a row of
 // the output.  The shares add up to what the launch gives its threads: 256
 // threads of 128 registers (two CTAs per SM), 384 of 168.
-constexpr int row_regs(int panels) { return panels == 1 ? 200 : 216; }
-constexpr int other_regs(int panels) { return panels == 1 ? 56 : 72; }
+constexpr int row_regs(int panels) { return panels == 1 ? 192 : 208; }
+constexpr int other_regs(int panels) { return panels == 1 ? 64 : 88; }
 static_assert(row_regs(1) + other_regs(1) <= 2 * 128 && 2 * row_regs(2) + other_regs(2) <= 3 * 168, "register shares");
-constexpr int kPairBarrier = 1, kRowBarrier = 5;  // named barriers: 1-4 the warps of the same rows, 5 all row warps
+constexpr int kPairBarrier = 1, kRowBarrier = 5, kTableBarrier = 6;  // named barriers: 1-4 the warps of the same rows, 5 all row warps, 6 the table's
 constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
@@ -106,8 +106,8 @@ struct TcArgs {
   BucketBounds bounds;
   int far;             // the last bucket's first distance
   // With t.part, the table's gradient:
-  int slots;           // distances kept apart: -far - 63 ... far + 64
-  float* dist;         // [CTAs][row warps][slots] where shared memory does not hold them, or nullptr
+  int slots;           // distances kept apart: -far - 63 ... far + 64 (a near block reaches 62 beyond the last bound)
+  float* dist;         // [CTAs][2][slots] where shared memory does not hold them, or nullptr
 };
 
 __device__ __forceinline__ int valid_of(const AttnArgs& a, long long bh) {
@@ -245,6 +245,10 @@ struct alignas(16) TcTail {
   uint64_t full[kStages], freed[kStages];
   uint64_t s_full[2], w_ready[2], part_full, part_free, a_ready;
   uint64_t rows_full[8];          // by row warp
+  // The table's gradient: each row warp's blocks of ds in its buffer, and at a
+  // unit's end its sums beyond the last bound on either side.
+  uint64_t ds_ready[8], ds_free[8], far_ready, far_free;
+  float far[8][2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -257,8 +261,6 @@ constexpr size_t stage_bytes() { return 2ull * 2 * P * kPanelBytes; }
 // columns past head_dim), and neither holds the row threads up: with loads
 // and stores of their own these took 5 to 7k of a unit's 30k cycles.
 constexpr int kBlockBytes = 32 * 128, kRowBuf = 2 * kBlockBytes;
-constexpr int kPitch = 36;  // diagonal_sums: words per row
-static_assert(32 * kPitch * 4 <= kRowBuf, "the diagonal sums' block");
 template <int P>
 constexpr size_t tc_smem() {
   return 1024 + kStages * stage_bytes<P>() + kRowWarpsOf(P) * kRowBuf + sizeof(TcTail);
@@ -322,26 +324,25 @@ __device__ __forceinline__ void mask_scores(float* s, float mult, const float* v
   }
 }
 
-// The sums along the diagonals of a 32 x 32 block whose row `lane` is s[32]:
-// before is the sum of column - row = lane - 31, after that of lane + 1.
-// Lane k reads column (k + 1 + row) mod 32 of every row: no bank conflict.
-__device__ __forceinline__ void diagonal_sums(float* buf, const float* s, int lane, float& before, float& after) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 4)
-    *reinterpret_cast<float4*>(buf + lane * kPitch + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
-  __syncwarp();
-  float x[32];
-#pragma unroll
-  for (int r = 0; r < 32; ++r) x[r] = buf[r * (kPitch + 1) + lane + 1 - (lane >= 31 - r ? 32 : 0)];
+// The sums along the diagonals of a 32 x 32 block (32 rows of 128 bytes under
+// the 128-byte swizzle): before is that of column - row = lane - 31, after
+// that of lane + 1.  Lane k reads column (k + 1 + row) mod 32 of every row: no
+// bank conflict.
+__device__ __forceinline__ void diagonal_sums(const float* block, int lane, float& before, float& after) {
   before = after = 0.f;
 #pragma unroll
-  for (int r = 0; r < 32; ++r) {
-    if (lane >= 31 - r)
-      before += x[r];
-    else
-      after += x[r];
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = block[(r0 + r) * 32 + (((lane + 1 + r0 + r) & 31) ^ ((r & 7) << 2))];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if (lane >= 31 - r0 - r)
+        before += x[r];
+      else
+        after += x[r];
+    }
   }
-  __syncwarp();
 }
 
 // The launches of a call overlap.  kForward and kDq start while split_kernel
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
   constexpr int kBlocks = kW / 32;
   constexpr bool kShared = KIND != kDv && kHalves == 2;      // a row's threads share a maximum
   constexpr int kRowThreadsTc = 128 * kHalves;
-  constexpr int kIssueWarp = kRowWarpsOf(P);                 // and the copy warp behind it; two more idle
+  constexpr int kIssueWarp = kRowWarpsOf(P);                 // then the copy warp and two for the table's gradient
   constexpr uint32_t kCols = 256 * P;
   constexpr uint32_t kColA2 = 64 * P;
   constexpr uint32_t kColS = kScores2 ? 128 * P : 64 * P;
@@ -399,9 +400,15 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     mbar_init(&sm.part_free, kRowThreadsTc);
     mbar_init(&sm.a_ready, kRowThreadsTc);
     for (int s = 0; s < kIssueWarp; ++s) mbar_init(&sm.rows_full[s], 1);
+    for (int s = 0; s < 8; ++s) {
+      mbar_init(&sm.ds_ready[s], 1);
+      mbar_init(&sm.ds_free[s], 1);
+    }
+    mbar_init(&sm.far_ready, kIssueWarp);
+    mbar_init(&sm.far_free, 1);
     for (int s = 0; s < kQueue; ++s) {
       mbar_init(&sm.u_full[s], 1);
-      mbar_init(&sm.u_free[s], kIssueWarp + 1);
+      mbar_init(&sm.u_free[s], kIssueWarp + (with_grad ? 3 : 1));
     }
     sm.abort_flag = 0;
     fence_mbar_init();
@@ -534,31 +541,29 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     Row r, nr;
     int G = 0;
     bool ok = true;  // the same on every lane of the warp
-    // The table's gradient: this warp's sums by distance, and of what lies
-    // beyond the last bucket's bound on either side.
-    float* const dist = !with_grad ? nullptr
-                        : c.dist   ? c.dist + (static_cast<size_t>(blockIdx.x) * kIssueWarp + warp) * c.slots
-                                   : reinterpret_cast<float*>(&sm + 1) + warp * c.slots;
+    int units = 0;
+    uint32_t ds_used = 0, ds_phase = 0;  // by block: whether it has been handed over, the parity of its next return
     ok = take_unit(u);
     if (u.n > 0) {
       fetch_rows(u, 0);
       ok = load_rows(u, r);
     }
-    while (ok && u.n > 0) {
+    for (;;) {
+      // Warps that meet at barriers of their own leave together.
+      const bool leave = !ok || u.n <= 0;
+      if (kShared ? bar_any(kPairBarrier + (warp & 3), 64, leave) : leave) break;
       const int row = u.r0 + rt;
       const size_t first_row = static_cast<size_t>(c.slice0 + u.local) * a.seq + u.r0;
       float far_before = 0.f, far_after = 0.f;
+      if (with_grad) {
+        if (ln == 0) tma_store_wait_read();  // the last unit's way out, before the blocks of ds
+        __syncwarp();
+      }
       float o[kOutCols];
 #pragma unroll
       for (int i = 0; i < kOutCols; ++i) o[i] = 0.f;
       float m_used = -INFINITY, m_true = -INFINITY, lsum = 0.f;
       float factor = 0.f;  // of the partial that is in flight
-      if (with_grad) {
-        for (int i = ln; i < c.slots; i += 32) dist[i] = 0.f;
-        if (ln == 0) tma_store_wait_read();  // the diagonal sums use the buffer
-        __syncwarp();
-      }
-
       // o += partial of tile g * factor, and the partial's columns are free.
       auto add_partial = [&](int g) {
         if (!warp_wait(&sm.part_full, g)) return false;
@@ -575,6 +580,14 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         mbar_arrive(&sm.part_free);
         return true;
       };
+      // Block q of the buffer is back from the table's warps.
+      auto ds_return = [&](int q) {
+        if (!(ds_used >> q & 1u)) return true;
+        if (!warp_wait(&sm.ds_free[warp * kBlocks + q], ds_phase >> q)) return false;
+        ds_phase ^= 1u << q;
+        ds_used &= ~(1u << q);
+        return true;
+      };
       // The larger of the row's two values x; false if either thread's warp gave up.
       auto share_max = [&](int g, float& x) {
         if constexpr (kHalves == 1) return ok;
@@ -585,13 +598,17 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       };
       nu.n = -1;
       // The next unit's rows: begun before the last tile (with the table's
-      // gradient behind it, since that uses the buffer), placed behind it.
+      // gradient behind it, when the buffer is back), placed behind it.
       auto begin_next = [&] {
         if (ok && take_unit(nu) && nu.n > 0) fetch_rows(nu, 0);
       };
       auto prepare_next = [&](int t) {
         if (t + 1 < u.n) return;
-        if (with_grad) begin_next();
+        if (with_grad) {
+#pragma unroll
+          for (int q = 0; q < kBlocks; ++q) ok = ok && ds_return(q);
+          begin_next();
+        }
         if (ok && nu.n > 0) ok = load_rows(nu, nr);
       };
 
@@ -721,7 +738,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
                 big = fmax3(big, fabsf(s[i + 2]), fabsf(s[i + 3]));
               }
               tmem_st32(scol + 32 * q, s);
-              if (with_grad) {
+              if (with_grad && ok) {
                 const int base = c0 + 32 * q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
                 if (base - 31 >= c.far || base + 31 <= -c.far) {          // all beyond the last bound
                   float x = 0.f;
@@ -732,12 +749,16 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
                   else
                     far_before += x;
                 } else {
-                  float before, after;
-                  diagonal_sums(reinterpret_cast<float*>(buf), s, ln, before, after);
-                  float* at = dist + base + c.far + 63;
-                  at[ln - 31] += before;
-                  at[ln + 1] += after;  // lane 31: 0, one slot past the block's distances
-                  __syncwarp();
+                  ok = ds_return(q);
+                  if (ok) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                      *reinterpret_cast<float4*>(buf + q * kBlockBytes + ln * 128 + (((i >> 2) ^ (ln & 7)) << 4)) =
+                          make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+                    __syncwarp();
+                    if (ln == 0) mbar_arrive(&sm.ds_ready[warp * kBlocks + q]);
+                    ds_used |= 1u << q;
+                  }
                 }
               }
             }
@@ -780,43 +801,23 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
                             : make_float2(-INFINITY, 0.f);
         __syncwarp();
       }
-      if (with_grad) {
-        // The warps' distances, bucket by bucket, in a fixed order.
-        dist[0] = dist[c.slots - 1] = 0.f;  // of no pair: the far sums go there
-        __syncwarp();
+      if (with_grad && ok) {
+        // The warp's sums beyond the last bound, to the table's warps.
+        if (units > 0) ok = warp_wait(&sm.far_free, units - 1);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
           far_before += __shfl_xor_sync(0xffffffffu, far_before, off);
           far_after += __shfl_xor_sync(0xffffffffu, far_after, off);
         }
         if (ln == 0) {
-          dist[0] = far_before;
-          dist[c.slots - 1] = far_after;
+          sm.far[warp][0] = far_before;
+          sm.far[warp][1] = far_after;
+          mbar_arrive(&sm.far_ready);
         }
         __syncwarp();
-        if (bar_any(kRowBarrier, kRowThreadsTc, !ok)) { ok = false; break; }
-        float* partial = c.t.part + (static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets;
-        const float* all = dist - warp * c.slots;
-        const int sides = c.t.buckets / 2;
-        for (int b = warp; b < c.t.buckets; b += kIssueWarp) {
-          const bool behind = b >= sides;  // keys after the query
-          const int k = behind ? b - sides : b;
-          const int from = max(c.bounds.at[k], behind ? 1 : 0);
-          const int end = behind ? c.far + 65 : c.far + 64;  // past the far sums' slot
-          const int to = k + 1 < sides ? min(c.bounds.at[k + 1], end) : end;
-          const int mid = c.far + 63;
-          float x = 0.f;
-          for (int i = from + ln; i < to; i += 32)
-            for (int w = 0; w < kIssueWarp; ++w) x += all[w * c.slots + mid + (behind ? i : -i)];
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-          if (ln == 0) partial[b] = x;
-        }
-        __syncwarp();
-        bar_named(kRowBarrier, kRowThreadsTc);
+        ++units;
       }
-      if (!ok) break;
-      {
+      if (ok) {
         const bool live = row < u.valid;
         const int wr0 = u.r0 + (warp & 3) * 32;
 #pragma unroll
@@ -939,6 +940,70 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
     }
     // Nothing arrives on a barrier after the CTA has ended.
     for (int g = max(0, committed - kStages); ok && g < committed; ++g) ok = warp_wait(&sm.freed[g % kStages], g / kStages);
+  } else if (with_grad && warp > kIssueWarp + 1) {
+    // ---------------- the table's gradient ----------------
+    // Two warps, each with the row warps of its parity: their near blocks of
+    // ds (some pair below the last bound) by distance, and at the unit's end
+    // the distances by bucket, everything in a fixed order.  Beside the row
+    // threads, whose own diagonal sums took 1.6k cycles a block and 7k a unit.
+    const int me = warp - (kIssueWarp + 2), ln = tid & 31;
+    float* const all = c.dist ? c.dist + static_cast<size_t>(blockIdx.x) * 2 * c.slots : reinterpret_cast<float*>(&sm + 1);
+    float* const dist = all + me * c.slots;
+    const int mid = c.far + 63;  // the slot of distance 0
+    uint32_t phase = 0;
+    bool ok = true;
+    TcUnit u;
+    for (int units = 0;; ++units) {
+      const bool got = take_unit(u);
+      if (bar_any(kTableBarrier, 64, !got) || u.n <= 0) break;  // both leave together
+      for (int i = ln; i < c.slots; i += 32) dist[i] = 0.f;
+      __syncwarp();
+      for (int t = 0; ok && t < u.n; ++t)
+        for (int w = me; ok && w < kIssueWarp; w += 2)
+          for (int q = 0; ok && q < kBlocks; ++q) {
+            const int base = (u.t0 + t) * kTileCols + kW * (w >> 2) + 32 * q - (u.r0 + (w & 3) * 32);
+            if (base - 31 >= c.far || base + 31 <= -c.far) continue;
+            const int i = w * kBlocks + q;
+            ok = warp_wait(&sm.ds_ready[i], phase >> i);
+            if (!ok) break;
+            phase ^= 1u << i;
+            float before, after;
+            diagonal_sums(reinterpret_cast<const float*>(row_bufs + w * kRowBuf + q * kBlockBytes), ln, before, after);
+            __syncwarp();
+            if (ln == 0) mbar_arrive(&sm.ds_free[i]);
+            dist[mid + base + ln - 31] += before;
+            __syncwarp();
+            dist[mid + base + ln + 1] += after;  // lane 31: 0, one slot past the block's distances
+            __syncwarp();
+          }
+      if (ok) ok = warp_wait(&sm.far_ready, units);
+      if (bar_any(kTableBarrier, 64, !ok)) break;
+      float* partial = c.t.part + (static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets;
+      const int sides = c.t.buckets / 2;
+      for (int b0 = 8 * me; b0 < c.t.buckets; b0 += 16) {  // four lanes to a bucket
+        const int b = b0 + (ln >> 2);
+        float x = 0.f;
+        if (b < c.t.buckets) {
+          const bool behind = b >= sides;  // keys after the query
+          const int k = behind ? b - sides : b;
+          const int from = max(c.bounds.at[k], behind ? 1 : 0);
+          const int to = k + 1 < sides ? min(c.bounds.at[k + 1], c.far + 64) : c.far + 64;
+#pragma unroll 4
+          for (int i = from + (ln & 3); i < to; i += 4) {
+            const int at = mid + (behind ? i : -i);
+            x += all[at] + all[c.slots + at];
+          }
+          if (k + 1 == sides && (ln & 3) == 0)
+            for (int w = 0; w < kIssueWarp; ++w) x += sm.far[w][behind];
+        }
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if (b < c.t.buckets && (ln & 3) == 0) partial[b] = x;
+      }
+      if (bar_any(kTableBarrier, 64, false)) break;  // both are done with the distances and the far sums
+      if (me == 0 && ln == 0) mbar_arrive(&sm.far_free);
+      __syncwarp();
+    }
   } else if (warp == kIssueWarp + 1) {
     // ---------------- units and bulk copies ----------------
     bool ok = true, first = true;
