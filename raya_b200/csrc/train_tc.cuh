@@ -277,6 +277,26 @@ __device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 
+// 32 columns from each of two places of this thread's TMEM lane, both on the
+// way at once (a round trip takes the row threads 200 cycles).  Loads and wait
+// in one statement, so that no use can be scheduled between them.
+__device__ __forceinline__ void tmem_ld32x2(uint32_t at0, float* v0, uint32_t at1, float* v1) {
+  uint32_t a[32], b[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(a[16]), "=r"(a[17]), "=r"(a[18]), "=r"(a[19]), "=r"(a[20]), "=r"(a[21]), "=r"(a[22]), "=r"(a[23]), "=r"(a[24]), "=r"(a[25]), "=r"(a[26]), "=r"(a[27]), "=r"(a[28]), "=r"(a[29]), "=r"(a[30]), "=r"(a[31]),
+        "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]), "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15]), "=r"(b[16]), "=r"(b[17]), "=r"(b[18]), "=r"(b[19]), "=r"(b[20]), "=r"(b[21]), "=r"(b[22]), "=r"(b[23]), "=r"(b[24]), "=r"(b[25]), "=r"(b[26]), "=r"(b[27]), "=r"(b[28]), "=r"(b[29]), "=r"(b[30]), "=r"(b[31])
+      : "r"(at0), "r"(at1)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    v0[i] = __uint_as_float(a[i]);
+    v1[i] = __uint_as_float(b[i]);
+  }
+}
+
 // Weights w[32] (fp32, already scaled) as fp16 hi and lo over their scores.
 __device__ __forceinline__ void store_weights(uint32_t taddr, const float* w) {
 #pragma unroll
@@ -568,16 +588,15 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       auto add_partial = [&](int g) {
         if (!warp_wait(&sm.part_full, g)) return false;
         tc_fence_after();
-        const float2 f2 = make_float2(factor, factor);
-#pragma unroll
-        for (int q = 0; q < kOutCols; q += 32) {
-          float x[32];
-          tmem_ld32(lane + kColPart + kOutCols * half + q, x);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) put2(o + q + i, __ffma2_rn(get2(x + i), f2, get2(o + q + i)));
-        }
+        static_assert(kOutCols == 64, "two loads of a thread's output columns");
+        const uint32_t at = lane + kColPart + kOutCols * half;
+        float x[64];
+        tmem_ld32x2(at, x, at + 32, x + 32);
         tc_fence_before();
         mbar_arrive(&sm.part_free);
+        const float2 f2 = make_float2(factor, factor);
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) put2(o + i, __ffma2_rn(get2(x + i), f2, get2(o + i)));
         return true;
       };
       // Block q of the buffer is back from the table's warps.
@@ -629,8 +648,11 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         // 32 columns at a time, in rolled loops (the loop over the tiles is to
         // fit the instruction cache nearest to the scheduler): block q's masked
         // scores, and back into tensor memory until the row's maximum is known.
-        auto block_scores = [&](int q, float* s) {
-          tmem_ld32(scol + 32 * q, s);
+        auto block_scores = [&](int q, float* s, float* dp) {
+          if constexpr (kScores2)
+            tmem_ld32x2(scol + 32 * q, s, lane + kColS2 + kW * half + 32 * q, dp);
+          else
+            tmem_ld32(scol + 32 * q, s);
           mask_scores<32, BIAS, kStep>(s, mult, vec + kStep * 32 * q, flat, mlo - 32 * q, mhi - 32 * q, inside);
         };
 
@@ -640,7 +662,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
 #pragma unroll 1
             for (int q = 0; q < kBlocks; ++q) {
               float s[32];
-              block_scores(q, s);
+              block_scores(q, s, nullptr);
 #pragma unroll
               for (int i = 0; i < 32; i += 2) mx = fmax3(mx, s[i], s[i + 1]);
               tmem_st32(scol + 32 * q, s);
@@ -690,7 +712,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
           for (int q = 0; q < kBlocks; ++q) {
             const float* off = sm.rows[st] + 64 + kW * half + 32 * q;
             float s[32];
-            block_scores(q, s);
+            block_scores(q, s, nullptr);
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               const float4 f = *reinterpret_cast<const float4*>(off + i);
@@ -716,8 +738,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
             for (int q = 0; q < kBlocks; ++q) {
               const float* off = sm.rows[st] + kW * half + 32 * q;
               float s[32], dp[32];
-              block_scores(q, s);
-              tmem_ld32(lane + kColS2 + kW * half + 32 * q, dp);
+              block_scores(q, s, dp);
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 float4 f, g;
@@ -906,11 +927,15 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       for (int t = 0; ok && t < n; ++t, ++G) {
         if constexpr (kScores2) {
           ok = warp_wait(&sm.full[G % kStages], G / kStages);
-          // The row threads have added the last partial, so its columns (dP's, for P = 1) and the weights' are free.
-          if (ok && G > 0) ok = warp_wait(&sm.part_free, G - 1);
+          // S takes the place of the last weights, whose product is complete,
+          // dP (for P = 1) that of its sum, which the row threads have added.
+          if (ok && G > 0) ok = warp_wait(&sm.part_full, G - 1);
           if (!ok) break;
           tc_fence_after();
           scores(kColS, 0, operand(G, 0));
+          if (G > 0) ok = warp_wait(&sm.part_free, G - 1);
+          if (!ok) break;
+          tc_fence_after();
           scores(kColS2, kColA2, operand(G, 1));
           commit(&sm.s_full[0], G);
         } else {
