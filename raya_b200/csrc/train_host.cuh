@@ -109,15 +109,15 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
     plan->rel_id = take(2 * static_cast<size_t>(plan->rel_half));
   }
   if (d->head_dim <= 128) {
-    const int tensors = backward ? 4 : 3;
     plan->panels = d->head_dim <= 64 ? 1 : 2;
+    const int first = !backward && plan->panels == 1 ? train::kImgK : train::kImgQ, last = backward ? 4 : 3;
     plan->tiles = static_cast<int>((d->seq + 127) / 128 * 2);
     plan->parts = plan->tiles / 2;
     const size_t image = static_cast<size_t>(plan->tiles) * 2 * plan->panels * train::kPanelBytes;
     // The grid of a chunk: three CTAs per 128-row tile and at most 2^31 in all.
-    plan->chunk = std::max<long long>(1, std::min<long long>({slices, static_cast<long long>(kMaxImageBytes / (tensors * image)),
+    plan->chunk = std::max<long long>(1, std::min<long long>({slices, static_cast<long long>(kMaxImageBytes / ((last - first) * image)),
                                                               0x7fffffffll / (2ll * plan->tiles)}));
-    for (int i = 0; i < tensors; ++i) plan->img[i] = take(plan->chunk * image);
+    for (int i = first; i < last; ++i) plan->img[i] = take(plan->chunk * image);
     plan->exps = take(plan->chunk * plan->tiles * sizeof(int4));
     if (backward) plan->rows = take(static_cast<size_t>(plan->chunk) * plan->tiles * train::kRowValues * sizeof(float));
     plan->next = take(4 * sizeof(unsigned));
@@ -189,21 +189,21 @@ raya_attn_status launch_rowwise(const TrainPlan& plan, train::TrainArgs t, const
   return check_launch("key gradient launch");
 }
 
-// A 3-D tensor map over a [slices][seq][head_dim] fp32 output with boxes of
+// A 3-D tensor map over a [slices][seq][head_dim] fp32 tensor with boxes of
 // [1][32 rows][32 floats], 128-byte swizzle: a store clips rows past seq and
-// columns past head_dim.
-raya_attn_status encode_out(CUtensorMap* map, float* base, uint64_t head_dim, uint64_t seq, uint64_t slices) {
+// columns past head_dim, a load gives zeros there.
+raya_attn_status encode_rows3d(CUtensorMap* map, const float* base, uint64_t head_dim, uint64_t seq, uint64_t slices) {
   raya_attn_status st = load_encoder();
   if (st != RAYA_ATTN_OK) return st;
   const cuuint64_t gdim[3] = {head_dim, seq, slices};
   const cuuint64_t gstride[2] = {head_dim * sizeof(float), seq * head_dim * sizeof(float)};
   const cuuint32_t box[3] = {32, 32, 1};
   const cuuint32_t estride[3] = {1, 1, 1};
-  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, gdim, gstride, box, estride,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), gdim, gstride, box, estride,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
-    return fail(RAYA_ATTN_ERR_CUDA, "cuda: cuTensorMapEncodeTiled (output) failed (%d)", static_cast<int>(r));
+    return fail(RAYA_ATTN_ERR_CUDA, "cuda: cuTensorMapEncodeTiled (rows) failed (%d)", static_cast<int>(r));
   return RAYA_ATTN_OK;
 }
 
@@ -215,7 +215,8 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   c.t = t;
   c.tiles = plan.tiles;
   c.backward = backward;
-  for (int i = 0; i < (backward ? 4 : 3); ++i) c.img[i] = at<uint8_t>(workspace, plan.img[i]);
+  c.first_image = !backward && P == 1 ? train::kImgK : train::kImgQ;
+  for (int i = c.first_image; i < (backward ? 4 : 3); ++i) c.img[i] = at<uint8_t>(workspace, plan.img[i]);
   c.exps = at<int4>(workspace, plan.exps);
   if (backward) c.rows = at<float>(workspace, plan.rows);
   c.next = at<unsigned>(workspace, plan.next);
@@ -238,12 +239,14 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   for (c.slice0 = 0; c.slice0 < slices; c.slice0 += plan.chunk) {
     const long long n = std::min(plan.chunk, slices - c.slice0) * plan.tiles;
     c.units = static_cast<unsigned>(n / 2);
-    train::split_kernel<P><<<dim3(static_cast<unsigned>(n), (backward ? 4 : 3) + (bias ? 1 : 0)), 256, 0, stream>>>(c);
+    train::split_kernel<P><<<dim3(static_cast<unsigned>(n), (backward ? 4 : 3) - c.first_image + (bias ? 1 : 0)), 256, 0, stream>>>(c);
     raya_attn_status st = check_launch("operand split launch");
     if (st != RAYA_ATTN_OK) return st;
-    auto launch_kind = [&](void (*fn)(train::TcArgs, CUtensorMap), size_t shared, float* out, const char* what) {
-      CUtensorMap map;
-      const raya_attn_status encoded = encode_out(&map, out, t.a.head_dim, t.a.seq, slices);
+    auto launch_kind = [&](void (*fn)(train::TcArgs, CUtensorMap, CUtensorMap), size_t shared, float* out, const char* what) {
+      CUtensorMap map, q_map{};
+      raya_attn_status encoded = encode_rows3d(&map, out, t.a.head_dim, t.a.seq, slices);
+      if (encoded == RAYA_ATTN_OK && c.first_image == train::kImgK)
+        encoded = encode_rows3d(&q_map, t.a.q, t.a.head_dim, t.a.seq, slices);
       if (encoded != RAYA_ATTN_OK) return encoded;
       cudaLaunchAttribute overlap{};  // with the end of the launch before (train_tc.cuh)
       overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -255,7 +258,7 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
       config.stream = stream;
       config.attrs = &overlap;
       config.numAttrs = 1;
-      const cudaError_t e = cudaLaunchKernelEx(&config, fn, c, map);
+      const cudaError_t e = cudaLaunchKernelEx(&config, fn, c, map, q_map);
       return e == cudaSuccess ? check_launch(what) : cuda_fail(e, what);
     };
     using train::tc_train;

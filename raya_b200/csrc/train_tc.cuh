@@ -18,7 +18,8 @@
 // per 64 columns of head_dim, zeros behind it).  One image serves as K-major
 // operand (scores) and as MN-major operand (sums over rows), so a tile needs
 // one plain bulk copy per operand and no warp of the product kernels splits
-// anything.  Rows at or past valid_len are zeros, so nothing there is ever
+// anything but its weights (and, in the forward pass with head_dim <= 64, q,
+// which only its own rows meet: a tensor less to write and read back).  Rows at or past valid_len are zeros, so nothing there is ever
 // multiplied.  1 / l goes into the rows of dout and into delta = dout . out:
 // with g_i = dout_i / l_i and w_ij = 2^(x_ij - m_i) <= 1,
 //   dv_j = sum_i w_ij g_i,   ds_ij = w_ij (g_i . v_j - g_i . out_i),
@@ -100,6 +101,7 @@ struct TcArgs {
   float* vec;          // where it goes by distance (t.rel_bias)
   int tiles;           // 64-row tiles per slice (even)
   bool backward;
+  int first_image;     // kImgK where the forward kernel splits q itself, else kImgQ
   long long slice0;
   unsigned units;      // 128-row tiles of the chunk
   unsigned* next;      // [4] by kind: units handed out beyond the first one of each CTA; split_kernel clears them
@@ -113,6 +115,14 @@ struct TcArgs {
 __device__ __forceinline__ int valid_of(const AttnArgs& a, long long bh) {
   const int v = a.valid_len ? a.valid_len[bh / a.heads] : a.seq;
   return v < 0 ? 0 : (v > a.seq ? a.seq : v);
+}
+
+// Two scaled values as fp16 hi (rounded to nearest) and lo (the rest).
+__device__ __forceinline__ void split_near(float x, float y, uint32_t& h, uint32_t& l) {
+  const __half2 hh = __floats2half2_rn(x, y);
+  const float2 back = __half22float2(hh);
+  h = *reinterpret_cast<const uint32_t*>(&hh);
+  l = tc16::pack_f16x2(x - back.x, y - back.y);
 }
 
 // Programmatic dependent launch.  A kernel that says launch_dependents lets the
@@ -130,7 +140,7 @@ template <int P>
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcArgs c) {
   __shared__ uint32_t red[8];
   const AttnArgs& a = c.t.a;
-  const int tid = threadIdx.x, which = blockIdx.y, d = a.head_dim;
+  const int tid = threadIdx.x, which = c.first_image + blockIdx.y, d = a.head_dim;
   launch_dependents();
   if (which == 4 || (which == 3 && !c.backward)) {
     rel_table(c.table, a.heads, c.t.buckets, c.t.rel_half, c.bounds, c.vec, nullptr, blockIdx.x * 256ll + tid,
@@ -139,17 +149,20 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   }
   const long long local = blockIdx.x / static_cast<unsigned>(c.tiles), bh = c.slice0 + local;
   const int tile = static_cast<int>(blockIdx.x - local * c.tiles);
-  if (blockIdx.x == 0 && which == 0 && tid < 4) c.next[tid] = 0;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid < 4) c.next[tid] = 0;
   const int valid = valid_of(a, bh);
   const int r0 = tile * 64;
   if (r0 >= (valid + 127) / 128 * 128) {  // no 128-row tile reads it: padding, whose results are zero
-    float* o = which == kImgQ ? (c.backward ? c.t.dq : a.out) : which == kImgK ? c.t.dk : which == kImgV ? c.t.dv : nullptr;
-    if (!c.backward && which != kImgQ) o = nullptr;
+    float* o = nullptr;
+    if (c.backward)
+      o = which == kImgQ ? c.t.dq : which == kImgK ? c.t.dk : which == kImgV ? c.t.dv : nullptr;
+    else if (which == kImgV)
+      o = a.out;
     const size_t first = static_cast<size_t>(bh) * a.seq + r0;
     const int rows = min(64, a.seq - r0);
     if (o)
       for (int i = tid; i < rows * d / 4; i += 256) st_stream(o + first * d + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f));
-    if (!c.backward && which == kImgQ && c.t.stats_out && tid < rows) c.t.stats_out[first + tid] = make_float2(-INFINITY, 0.f);
+    if (!c.backward && which == kImgV && c.t.stats_out && tid < rows) c.t.stats_out[first + tid] = make_float2(-INFINITY, 0.f);
     if (c.t.part && which == kImgQ && tile % 2 == 0 && tid < c.t.buckets)
       c.t.part[(static_cast<size_t>(bh) * c.t.parts + tile / 2) * c.t.buckets + tid] = 0.f;
     return;
@@ -211,13 +224,8 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
     for (int p = 0; p < P; ++p) {
       const float v[4] = {x[i][p].x * sc, x[i][p].y * sc, x[i][p].z * sc, x[i][p].w * sc};
       uint32_t h[2], l[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const __half2 hh = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-        const float2 back = __half22float2(hh);
-        h[k] = *reinterpret_cast<const uint32_t*>(&hh);
-        l[k] = tc16::pack_f16x2(v[2 * k] - back.x, v[2 * k + 1] - back.y);
-      }
+      split_near(v[0], v[1], h[0], l[0]);
+      split_near(v[2], v[3], h[1], l[1]);
       const uint32_t at = p * kPanelBytes + tc16::op_off(rr, c4 >> 3) + (c4 & 4) * 2;
       *reinterpret_cast<uint2*>(img + at) = make_uint2(h[0], h[1]);
       *reinterpret_cast<uint2*>(img + P * kPanelBytes + at) = make_uint2(l[0], l[1]);
@@ -273,6 +281,14 @@ static_assert(tc_smem<1>() <= kHalfSm && tc_smem<1>() > 233472 / 3 && tc_smem<2>
 // A product of scales that would be infinite, as the largest float: 0 times it is 0.
 __device__ __forceinline__ float finite(float x) { return fmaxf(fminf(x, 3.4028235e38f), -3.4028235e38f); }
 
+// One tensor-map tile into shared memory, completing on `bar`; zeros outside the tensor.
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 __device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
@@ -376,10 +392,13 @@ __device__ __forceinline__ void diagonal_sums(const float* block, int lane, floa
 // hands them to the other warps.  Every barrier and ring runs on across them:
 // G counts the CTA's 64-column tiles, U its units with any.
 template <int KIND, int P, bool BIAS>
-__global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const __grid_constant__ TcArgs c, const __grid_constant__ CUtensorMap out_map) {
+__global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
+    const __grid_constant__ TcArgs c, const __grid_constant__ CUtensorMap out_map,
+    const __grid_constant__ CUtensorMap q_map) {
   using namespace tc32;
   constexpr bool kScores2 = KIND == kDq || KIND == kDk;      // S and dP, serial
   constexpr bool kByKey = KIND == kDk || KIND == kDv;        // rows are keys, columns queries
+  constexpr bool kOwnRows = KIND == kForward && P == 1;      // q straight from its tensor, split by its row threads
   constexpr bool kBehindSplit = !kByKey;                     // the launch before is split_kernel
   constexpr int kHalves = P;                                 // threads per row
   constexpr int kW = 64 / kHalves;                           // score columns of a thread
@@ -502,8 +521,14 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         tma_store_wait_read();  // and the last unit's way out
         const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64 + ((warp & 3) >> 1);
         mbar_arrive_expect_tx(&sm.rows_full[warp], kRowBuf);
+        if constexpr (kOwnRows) {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+          for (int p = 0; p < 2; ++p)
+            tma_load_3d(buf + p * kBlockBytes, &q_map, 32 * p, u.r0 + warp * 32, static_cast<int>(c.slice0 + u.local),
+                        &sm.rows_full[warp]);
+        }
+#pragma unroll
+        for (int p = 0; p < 2 && !kOwnRows; ++p) {
           const int piece = (half * kRounds + round) * 2 + p;
           tma_load_1d(buf + p * kBlockBytes,
                       c.img[piece < 2 * P ? kA1 : kA2] + tile * static_cast<long long>(kOp) +
@@ -514,32 +539,67 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       __syncwarp();
       in_flight = true;
     };
+    // Piece p of the buffer: this lane's row of block p.
+    auto buffered = [&](int p, float* w) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(buf + p * kBlockBytes + ln * 128 + ((k ^ (ln & 7)) << 4));
+        w[4 * k] = x.x;
+        w[4 * k + 1] = x.y;
+        w[4 * k + 2] = x.z;
+        w[4 * k + 3] = x.w;
+      }
+    };
     auto place_rows = [&](int round) {
       if (!warp_wait(&sm.rows_full[warp], fetched)) return false;
       in_flight = false;
       ++fetched;
+      if constexpr (!kOwnRows) {
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        float w[32];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float4 x = *reinterpret_cast<const float4*>(buf + p * kBlockBytes + ln * 128 + ((k ^ (ln & 7)) << 4));
-          w[4 * k] = x.x;
-          w[4 * k + 1] = x.y;
-          w[4 * k + 2] = x.z;
-          w[4 * k + 3] = x.w;
+        for (int p = 0; p < 2; ++p) {
+          float w[32];
+          buffered(p, w);
+          tmem_st32(lane + 32 * ((half * kRounds + round) * 2 + p), w);
         }
-        tmem_st32(lane + 32 * ((half * kRounds + round) * 2 + p), w);
       }
       return true;
+    };
+    // kOwnRows: the row of q in the buffer, scaled by an exponent of its own,
+    // hi and lo into tensor memory (columns k / 2 and 32 + k / 2).  Returns 2^-e.
+    auto split_row = [&](bool live) {
+      float w[64];
+      buffered(0, w);
+      buffered(1, w + 32);
+      float big = 0.f;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {
+        if (!live) w[i] = 0.f;  // padding may hold anything
+        if (fabsf(w[i]) < INFINITY) big = fmaxf(big, fabsf(w[i]));
+      }
+      const int e = tc16::scale_exp(__float_as_uint(big));
+      const float2 up = make_float2(tc16::pow2(e), tc16::pow2(e));
+#pragma unroll
+      for (int q = 0; q < 64; q += 16) {
+        uint32_t h[8], l[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float2 x = __fmul2_rn(get2(w + q + 2 * k), up);
+          split_near(x.x, x.y, h[k], l[k]);
+        }
+        tc16::tmem_st8u(lane + q / 2, h);
+        tc16::tmem_st8u(lane + 32 + q / 2, l);
+      }
+      return tc16::pow2(-e);
     };
     // The rest of a unit's rows (its first round is on the way) and what goes
     // with them.  Called when the scores of the unit before are complete.
     auto load_rows = [&](const TcUnit& u, Row& r) {
       const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64 + ((warp & 3) >> 1);
-      const int4 e = c.exps[tile];
-      r.qmul = a.qscale * tc16::pow2(-(kByKey ? e.y : e.x));
-      r.unit = kScores2 ? tc16::pow2(-(kByKey ? e.z : e.w)) : 0.f;
+      if constexpr (!kOwnRows) {
+        const int4 e = c.exps[tile];
+        r.qmul = a.qscale * tc16::pow2(-(kByKey ? e.y : e.x));
+        r.unit = kScores2 ? tc16::pow2(-(kByKey ? e.z : e.w)) : 0.f;
+      }
       r.off = r.delta = 0.f;
       if constexpr (KIND == kDq) {
         r.off = c.rows[tile * kRowValues + (rt & 63)];
@@ -551,6 +611,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
         if (round > 0) fetch_rows(u, round);
         if (!place_rows(round)) return false;
       }
+      if constexpr (kOwnRows) r.qmul = a.qscale * split_row(u.r0 + rt < u.valid);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&sm.a_ready);
@@ -1063,7 +1124,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(const 
       if ((tid & 31) == 0) {
         sm.unit[k % kQueue] = u;
         mbar_arrive(&sm.u_full[k % kQueue]);
-        if (u.n > 0) {  // its rows, a unit ahead of their use
+        if (!kOwnRows && u.n > 0) {  // its rows, a unit ahead of their use
           const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64;
           prefetch_l2(c.img[kA1] + tile * static_cast<long long>(kOp), 2 * kOp);
           if constexpr (kScores2) prefetch_l2(c.img[kA2] + tile * static_cast<long long>(kOp), 2 * kOp);
