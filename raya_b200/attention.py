@@ -470,16 +470,15 @@ def _train_call(call, backward, shape, params, tensors, stats, more, bias, dtabl
     one sequence takes the GPU about 20 us."""
     import torch
 
+    tensor, float32 = torch.Tensor, torch.float32
     q = tensors[0][1]
-    if not isinstance(q, torch.Tensor) or not q.is_cuda:
-        raise TypeError("`q` must be a contiguous CUDA torch.float32 tensor")
-    device = q.device
+    at = q.get_device() if isinstance(q, tensor) else -1
 
-    def ptr(name, x, numel, dtype=torch.float32):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype is not dtype or not x.is_contiguous():
+    def ptr(name, x, numel, dtype=float32):
+        if not isinstance(x, tensor) or x.dtype is not dtype or not x.is_contiguous() or x.get_device() < 0:
             raise TypeError(f"`{name}` must be a contiguous CUDA {dtype} tensor")
-        if x.device != device:
-            raise TypeError(f"`{name}` is on {x.device}, the other tensors are on {device}")
+        if x.get_device() != at:
+            raise TypeError(f"`{name}` is on {x.device}, the other tensors are on cuda:{at}")
         if x.numel() != numel:
             raise LengthError(f"buffer `{name}` has length {x.numel()}, expected {numel}", name=name, got=x.numel(),
                               expected=numel)
@@ -505,35 +504,35 @@ def _train_call(call, backward, shape, params, tensors, stats, more, bias, dtabl
         if (host < 0).any() or (host > shape.seq).any():
             raise ShapeError(f"invalid shape: valid_len outside [0, {shape.seq}]")
         if (host != shape.seq).any():
-            keep = valid_len = torch.from_numpy(host).to(device)
+            keep = valid_len = torch.from_numpy(host).to(q.device)
     args.append(None if valid_len is None else ptr("valid_len", valid_len, shape.batch, torch.int32))
     args.append(b)
     if backward:
         args.append(dtable_ptr)
-    if workspace is not None and (not isinstance(workspace, torch.Tensor) or not workspace.is_contiguous()
-                                  or workspace.device != device):
+    if workspace is not None and (not isinstance(workspace, tensor) or not workspace.is_contiguous()
+                                  or workspace.get_device() != at):
         raise TypeError("the workspace must be a contiguous CUDA tensor on the tensors' device")
 
     def launch(handle):
         # Memory that is taken here is taken on the call's stream, so the allocator orders its next use.
         ws = workspace
         if ws is None:
-            ws = torch.empty(_train_bytes(d, b, backward), dtype=torch.uint8, device=device)
+            ws = torch.empty(_train_bytes(d, b, backward), dtype=torch.uint8, device=q.device)
         status = call(d, *args, ws.data_ptr() or None, ws.numel() * ws.element_size(), handle)
         if status != _lib.OK:
             _check(status)
         if keep is not None:  # keep the uploaded lengths alive until the kernels have run
             _sync(handle)
 
-    if stream is None and device.index == torch.cuda.current_device():
-        launch(torch.cuda.current_stream(device.index).cuda_stream)
+    if stream is None and at == torch.cuda.current_device():
+        launch(torch.cuda.current_stream(at).cuda_stream)
         return
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        stream = torch.cuda.current_stream(at)
     elif not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(int(stream), device=device)
-    if stream.device != device:
-        raise TypeError(f"the stream is on {stream.device}, the tensors are on {device}")
+        stream = torch.cuda.ExternalStream(int(stream), device=q.device)
+    if stream.device != q.device:
+        raise TypeError(f"the stream is on {stream.device}, the tensors are on {q.device}")
     with torch.cuda.stream(stream):
         launch(stream.cuda_stream)
 

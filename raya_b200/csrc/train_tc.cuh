@@ -19,36 +19,41 @@
 // operand (scores) and as MN-major operand (sums over rows), so a tile needs
 // one plain bulk copy per operand and no warp of the product kernels splits
 // anything but its weights (and, in the forward pass with head_dim <= 64, q,
-// which only its own rows meet: a tensor less to write and read back).  Rows at or past valid_len are zeros, so nothing there is ever
-// multiplied.  1 / l goes into the rows of dout and into delta = dout . out:
+// which only its own rows meet: a tensor less to write and read back, 10%).
+// Rows at or past valid_len are zeros, so nothing there is ever multiplied.
+// What is not finite stays in the products of its own row with every row of
+// the tiles that see it.  1 / l goes into the rows of dout and into delta = dout . out:
 // with g_i = dout_i / l_i and w_ij = 2^(x_ij - m_i) <= 1,
 //   dv_j = sum_i w_ij g_i,   ds_ij = w_ij (g_i . v_j - g_i . out_i),
 // so no product multiplies by it, and the exponent's argument stays a small
 // difference (m and log2(l) in one fp32 offset cost 6e-7 of every p).
 //
-// A CTA computes one 128-row tile of one output; with the rows R, the
-// columns C (64 per step) and the second operand X of its kind:
+// A unit of work is one 128-row tile of one output; with the rows R, the
+// columns C (64 per step) and the second operand of its kind:
 //   kForward: R = q,      C = k,  out  = softmax(R C^T) v
 //   kDv:      R = k,      C = q,  dv   = W^T g
 //   kDq:      R = q, g    C = k, v  dq = dS k,   dS = W * (g v^T - delta)
 //   kDk:      R = k, v    C = q, g  dk = dS^T q
-// 7 products where a single pass over the pairs would take 5, but every sum
-// stays in its own CTA: no atomics, the same bits on every run.  Per 128x64
-// tile and kind: 12 MMAs (M 128, N 64, K 16) per product, ~32 cycles each.
+// 7 products where a single pass over the pairs would take 5 (dk and dv in
+// one CTA would need 384 columns of tensor memory and could not share an SM),
+// but every sum stays in its own CTA: no atomics, the same bits on every run.
+// Per 128x64 tile and kind: 12 MMAs (M 128, N 64, K 16) per product and
+// panel, ~32 cycles each.
 //
 // Two CTAs share an SM (head_dim <= 64: 256 tensor-memory columns each; one
 // CTA of 512 columns above), so one's softmax runs beside the other's
-// products and its start and end beside the other's middle.  Within a CTA
-// the steps are serial, except that kForward and kDv compute the next scores
-// during the softmax (two score buffers).
+// products: 1.6 times one CTA's rate.  Within a CTA the steps follow one
+// another, except that kForward and kDv compute the next scores during the
+// softmax (two score buffers).  The CTAs are persistent and take units from a
+// queue; the next unit's rows are on their way before the last tile of this.
 //
-// Roles (320 threads): warps 0-7 the rows (TMEM lane = row), warps 0-3 the
-// first and 4-7 the second half of the columns of the scores and of the
-// output; what a row's two threads share (its maximum) passes through shared
-// memory at a barrier of their two warps.  Warp 8 issues the MMAs, warp 9 the
-// bulk copies; both run their loops on the whole warp and issue from one
-// lane.  With one thread per row (192 threads) the softmax's own latencies
-// set the pace: 3.4k cycles per tile and 31% of the issue slots used.
+// Roles (256 threads; 384 for two panels): warps 0-3 one row per thread (TMEM
+// lane = row), for two panels warps 4-7 the second half of the columns of
+// the scores and of the output (what a row's two threads share, its maximum,
+// passes through shared memory).  Then one warp that issues the MMAs, one
+// that takes the units and issues the bulk copies, and two that sum the
+// table's gradient; the first two run their loops on the whole warp and issue
+// from one lane.
 //
 // Tensor memory, columns (P = panels): rows' operands (hi 32 P, lo 32 P,
 // twice for kDq and kDk), then scores: kForward and kDv two buffers of 64 and
@@ -56,6 +61,16 @@
 // P = 1 takes dP's place once that has been read.  The weights overwrite
 // their scores: k-step s (16 columns) has its hi part in columns 32 (s / 2) +
 // 8 (s % 2) and lo 16 further.
+//
+// What bounds it.  The chain of a tile: scores, a round trip through the row
+// threads (tensor memory to registers and back), the second product, its
+// sum.  One CTA alone takes 3.5k cycles a tile (kForward), two on an SM 2.1k
+// each tile of either, of which the tensor core works 37%, the issue slots
+// 44%.  Taking two thirds of the MMAs out changed 8 to 17%, all exponentials 5%, the
+// split of the weights 4%, the bulk copies nothing.  Measured and left: two
+// threads per row (the same time with 30% more instructions), unrolled 64-column
+// code (instruction fetch: 419 against 314 us), a grid of all three gradients
+// (likewise), a workspace that stays in L2 (each chunk's tail costs more).
 //
 // Every wait is bounded, as in the forward kernels.
 #pragma once
@@ -78,7 +93,8 @@ constexpr int tc_threads(int panels) { return 128 * panels + 128; }
 constexpr int row_regs(int panels) { return panels == 1 ? 192 : 208; }
 constexpr int other_regs(int panels) { return panels == 1 ? 64 : 88; }
 static_assert(row_regs(1) + other_regs(1) <= 2 * 128 && 2 * row_regs(2) + other_regs(2) <= 3 * 168, "register shares");
-constexpr int kPairBarrier = 1, kRowBarrier = 5, kTableBarrier = 6;  // named barriers: 1-4 the warps of the same rows, 5 all row warps, 6 the table's
+// Named barriers: 1-4 the two warps of the same rows, 5 all row warps, 6 the table's.
+constexpr int kPairBarrier = 1, kRowBarrier = 5, kTableBarrier = 6;
 constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
@@ -113,7 +129,7 @@ struct TcArgs {
 };
 
 __device__ __forceinline__ int valid_of(const AttnArgs& a, long long bh) {
-  const int v = a.valid_len ? a.valid_len[bh / a.heads] : a.seq;
+  const int v = a.valid_len ? a.valid_len[static_cast<unsigned>(bh) / static_cast<unsigned>(a.heads)] : a.seq;  // bh < 2^31
   return v < 0 ? 0 : (v > a.seq ? a.seq : v);
 }
 
@@ -134,8 +150,9 @@ __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontro
 // 64 rows of one tensor into their image.  256 threads: 16 lanes take a row's
 // 64 columns of a panel (16-byte loads, 8-byte stores), 16 rows at a time.
 // blockIdx.y: the tensor, and behind them the bias by distance.  Tiles of padding write the zeros of the results
-// there instead.  Bound by HBM: 4 bytes read and 4 written per
-// element (dout: 8 read).
+// there instead.  Bound by HBM: 4 bytes read and 4 written per element
+// (dout: 8 read), 75 to 80% of the copy rate (8 x 16 x 8192, backward: 2.0 GB
+// in 388 us).
 template <int P>
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcArgs c) {
   __shared__ uint32_t red[8];
@@ -147,18 +164,19 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
               gridDim.x * 256ll);
     return;
   }
-  const long long local = blockIdx.x / static_cast<unsigned>(c.tiles), bh = c.slice0 + local;
-  const int tile = static_cast<int>(blockIdx.x - local * c.tiles);
+  const unsigned local = blockIdx.x / static_cast<unsigned>(c.tiles);
+  const long long bh = c.slice0 + local;
+  const int tile = static_cast<int>(blockIdx.x - local * static_cast<unsigned>(c.tiles));
   if (blockIdx.x == 0 && blockIdx.y == 0 && tid < 4) c.next[tid] = 0;
   const int valid = valid_of(a, bh);
   const int r0 = tile * 64;
+  const size_t first = static_cast<size_t>(bh) * a.seq + r0;
   if (r0 >= (valid + 127) / 128 * 128) {  // no 128-row tile reads it: padding, whose results are zero
     float* o = nullptr;
     if (c.backward)
       o = which == kImgQ ? c.t.dq : which == kImgK ? c.t.dk : which == kImgV ? c.t.dv : nullptr;
     else if (which == kImgV)
       o = a.out;
-    const size_t first = static_cast<size_t>(bh) * a.seq + r0;
     const int rows = min(64, a.seq - r0);
     if (o)
       for (int i = tid; i < rows * d / 4; i += 256) st_stream(o + first * d + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f));
@@ -167,46 +185,60 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
       c.t.part[(static_cast<size_t>(bh) * c.t.parts + tile / 2) * c.t.buckets + tid] = 0.f;
     return;
   }
-  const float* src = which == kImgQ ? a.q : which == kImgK ? a.k : which == kImgV ? a.v : c.t.dout;
-  src += static_cast<size_t>(bh) * a.seq * d;
-  const float* out = a.out + static_cast<size_t>(bh) * a.seq * d;
-  const int c4 = (tid & 15) * 4, r = tid >> 4;
-  float4 x[4][P];
-  float big = 0.f;
+  const float* __restrict__ src = (which == kImgQ ? a.q : which == kImgK ? a.k : which == kImgV ? a.v : c.t.dout) + first * d;
+  const float* __restrict__ out = a.out + first * d;
+  const bool grad = which == kImgG;
+  const int c4 = (tid & 15) * 4, r = tid >> 4, live = valid - r0;  // rows below `live` are read
+  float4 x[4][P], y[4][P];
+  float2 st[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = r0 + r + 16 * i;
-    float m2 = 0.f, linv = 0.f, dot = 0.f;
-    if (which == kImgG && row < valid) row_stats(c.t.stats[static_cast<size_t>(bh) * a.seq + row], m2, linv);
+    const int row = r + 16 * i;
+    st[i] = make_float2(0.f, 0.f);
+    if (grad && row < live) st[i] = __ldg(c.t.stats + first + row);
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int col = 64 * p + c4;
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < valid && col < d) {
-        y = *reinterpret_cast<const float4*>(src + static_cast<size_t>(row) * d + col);
-        if (which == kImgG) {
-          y = make_float4(y.x * linv, y.y * linv, y.z * linv, y.w * linv);
-          const float4 o = *reinterpret_cast<const float4*>(out + static_cast<size_t>(row) * d + col);
-          dot = fmaf(y.x, o.x, fmaf(y.y, o.y, fmaf(y.z, o.z, fmaf(y.w, o.w, dot))));
-        }
-      }
-      x[i][p] = y;
-      // Infinities and NaN stay out of the exponent: they spoil their own products only.
-      const float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
-      if (m < INFINITY) big = fmaxf(big, m);
-    }
-    if (which == kImgG) {
-#pragma unroll
-      for (int off = 8; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-      if ((tid & 15) == 0) {
-        float* rows = c.rows + (local * c.tiles + tile) * kRowValues;
-        const float off = linv != 0.f ? m2 : INFINITY;  // 2^(x - inf) = 0: no key, or past valid_len
-        rows[r + 16 * i] = off;
-        rows[64 + r + 16 * i] = off - kWeightLog2;
-        rows[128 + r + 16 * i] = dot;
+      x[i][p] = y[i][p] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < live && col < d) {
+        x[i][p] = __ldcs(reinterpret_cast<const float4*>(src + static_cast<size_t>(row) * d + col));
+        if (grad) y[i][p] = __ldcs(reinterpret_cast<const float4*>(out + static_cast<size_t>(row) * d + col));
       }
     }
   }
+  if (grad) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float m2, linv, dot = 0.f;
+      row_stats(st[i], m2, linv);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        float4& g = x[i][p];
+        const float4 o = y[i][p];
+        g = make_float4(g.x * linv, g.y * linv, g.z * linv, g.w * linv);
+        dot = fmaf(g.x, o.x, fmaf(g.y, o.y, fmaf(g.z, o.z, fmaf(g.w, o.w, dot))));
+      }
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+      if ((tid & 15) == 0) {
+        float* rows = c.rows + (static_cast<size_t>(local) * c.tiles + tile) * kRowValues + r + 16 * i;
+        const float off = linv != 0.f ? m2 : INFINITY;  // 2^(x - inf) = 0: no key, or past valid_len
+        rows[0] = off;
+        rows[64] = off - kWeightLog2;
+        rows[128] = dot;
+      }
+    }
+  }
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      // Infinities and NaN stay out of the exponent: they spoil their own products only.
+      const float4 g = x[i][p];
+      const float m = fmaxf(fmaxf(fabsf(g.x), fabsf(g.y)), fmaxf(fabsf(g.z), fabsf(g.w)));
+      if (m < INFINITY) big = fmaxf(big, m);
+    }
   const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
   if ((tid & 31) == 0) red[tid >> 5] = bits;
   __syncthreads();
@@ -215,22 +247,21 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   for (int w = 1; w < 8; ++w) most = max(most, red[w]);
   const int e = tc16::scale_exp(most);
   const float sc = tc16::pow2(e);
-  if (tid == 0) reinterpret_cast<int*>(c.exps + local * c.tiles + tile)[which] = e;
-  uint8_t* img = c.img[which] + (local * c.tiles + tile) * (2ll * P * kPanelBytes);
+  const size_t at_tile = static_cast<size_t>(local) * c.tiles + tile;
+  if (tid == 0) reinterpret_cast<int*>(c.exps + at_tile)[which] = e;
+  uint8_t* img = c.img[which] + at_tile * (2 * P * kPanelBytes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int rr = r + 16 * i;
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const float v[4] = {x[i][p].x * sc, x[i][p].y * sc, x[i][p].z * sc, x[i][p].w * sc};
+      const float4 g = x[i][p];
       uint32_t h[2], l[2];
-      split_near(v[0], v[1], h[0], l[0]);
-      split_near(v[2], v[3], h[1], l[1]);
-      const uint32_t at = p * kPanelBytes + tc16::op_off(rr, c4 >> 3) + (c4 & 4) * 2;
+      split_near(g.x * sc, g.y * sc, h[0], l[0]);
+      split_near(g.z * sc, g.w * sc, h[1], l[1]);
+      const uint32_t at = p * kPanelBytes + tc16::op_off(r + 16 * i, c4 >> 3) + (c4 & 4) * 2;
       *reinterpret_cast<uint2*>(img + at) = make_uint2(h[0], h[1]);
       *reinterpret_cast<uint2*>(img + P * kPanelBytes + at) = make_uint2(l[0], l[1]);
     }
-  }
 }
 
 // One unit of work: a 128-row tile of one slice.

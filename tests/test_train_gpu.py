@@ -392,3 +392,72 @@ def test_a_training_step(cuda_device):
     # L(+s) - L(-s) = 2 s g.g plus odd terms from s^3 on: the even ones cancel.  The table's gradient sums thousands of
     # pairs, so the quadratic term alone is ~0.08 of s g.g here, and the cubic one is of the order of its square.
     assert abs((at[0] - at[1]) / (2 * step) - square) < 0.05 * square, (at, square)
+
+
+@pytest.mark.parametrize("heads,seq,d,far", [(2, 1500, 64, 4096), (1, 2000, 96, 4096), (1, 700, 64, 600)])
+def test_distances_that_shared_memory_does_not_hold(cuda_device, heads, seq, d, far):
+    """Bias tables whose distances are too many for a block's shared memory."""
+    x, valid = make(1, heads, seq, d, [seq - 77], 23, 64)
+    check(x, valid, rb.Mask.FULL, 128, max_distance=far)
+
+
+def test_more_slices_than_one_chunk_of_the_workspace(cuda_device):
+    """Images of more than the workspace holds at a time: every sequence as when called alone."""
+    import torch
+
+    batch, heads, seq = 20, 16, 8192  # 8 MB of images per slice, 2 GiB at a time
+    shape = rb.AttnShape(heads=heads, seq=seq, head_dim=64, batch=batch)
+    params = rb.AttnParams(BLOCK3, 128, seq, 0.125)
+    g = torch.Generator(device="cuda").manual_seed(24)
+    t = {n: torch.randn(batch, heads, seq, 64, generator=g, device="cuda") for n in ("q", "k", "v", "dout")}
+    bias = rb.RelativeBias(torch.randn(heads, 32, generator=g, device="cuda"))
+    valid = torch.randint(1000, seq + 1, (batch,), generator=g, device="cuda", dtype=torch.int32)
+
+    def run(at):
+        x = {n: y[at] for n, y in t.items()}
+        sh = rb.AttnShape(heads=heads, seq=seq, head_dim=64, batch=x["q"].shape[0])
+        out, stats = torch.empty_like(x["q"]), torch.empty(*x["q"].shape[:3], 2, device="cuda")
+        rb.Cuda().attend_bias(sh, params, x["q"], x["k"], x["v"], out, stats=stats, bias=bias, valid_len=valid[at])
+        grads = [torch.empty_like(out) for _ in range(3)]
+        dtable = torch.empty_like(bias.table)
+        rb.Cuda().attend_backward(sh, params, x["q"], x["k"], x["v"], out, stats, x["dout"], *grads, bias=bias, dtable=dtable,
+                                  valid_len=valid[at])
+        return [out, stats, *grads, dtable]
+
+    need = rb.train_workspace(shape, params, bias, backward=True)
+    assert need < 3 << 30 and need < batch * heads * 8 << 20  # one chunk at a time
+    whole = run(slice(0, batch))
+    table = torch.zeros_like(bias.table, dtype=torch.float64)
+    for b in range(batch):
+        one = run(slice(b, b + 1))
+        for x, y in zip(whole[:-1], one[:-1]):
+            assert torch.equal(x[b : b + 1], y), b
+        table += one[-1].double()
+    # each sequence's gradient is rounded to fp32 once, and the whole's
+    assert ((whole[-1] - table).abs() <= 2.0 ** -24 * (batch + 1) * table.abs().max()).all()
+    rb.sync_status()
+
+
+@pytest.mark.parametrize("d", [64, 96, 136])
+def test_two_calls_at_once(cuda_device, d):
+    """Calls on two streams, each with a workspace of its own, in each other's way on the SMs."""
+    import torch
+
+    inputs = [make(2, 4, 700, d, [700, 401], 25, 32), make(3, 2, 500, d, [500, 33, 444], 26)]
+    want = []
+    for x, valid in inputs:
+        c = Call(x, valid, BLOCK3, 64)
+        c.forward()
+        c.backward()
+        want.append(c.results())
+    streams = [torch.cuda.Stream() for _ in inputs]
+    calls = [Call(x, valid, BLOCK3, 64, stream=s) for (x, valid), s in zip(inputs, streams)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c in calls:
+            c.forward()
+            c.backward()
+    for c, w in zip(calls, want):
+        got = c.results()
+        for n in w:
+            assert np.array_equal(got[n], w[n]), n
