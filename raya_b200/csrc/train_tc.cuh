@@ -93,8 +93,9 @@ constexpr int tc_threads(int panels) { return 128 * panels + 128; }
 constexpr int row_regs(int panels) { return panels == 1 ? 192 : 208; }
 constexpr int other_regs(int panels) { return panels == 1 ? 64 : 88; }
 static_assert(row_regs(1) + other_regs(1) <= 2 * 128 && 2 * row_regs(2) + other_regs(2) <= 3 * 168, "register shares");
-// Named barriers: 1-4 the two warps of the same rows, 5 all row warps, 6 the table's.
-constexpr int kPairBarrier = 1, kRowBarrier = 5, kTableBarrier = 6;
+// Named barriers, which have no bound: between warps that leave together only.
+// 1-4 the two warps of the same rows, 5 the table's.
+constexpr int kPairBarrier = 1, kTableBarrier = 5;
 constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
@@ -903,9 +904,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
       if constexpr (KIND == kForward) {
         if constexpr (kHalves == 2) {  // the row's sum: first half + second half
           sm.red[0][half][rt] = lsum;  // the last exchange is read: part_full follows both threads' w_ready
-          if (bar_any(kRowBarrier, kRowThreadsTc, !ok)) { ok = false; break; }
-          lsum = sm.red[0][0][rt] + sm.red[0][1][rt];
-          bar_named(kRowBarrier, kRowThreadsTc);  // read before the next unit's exchange
+          if (bar_any(kPairBarrier + (warp & 3), 64, !ok)) { ok = false; break; }
+          lsum = sm.red[0][0][rt] + sm.red[0][1][rt];  // and read before the pair meets at the loop's top
         }
         f = lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f;
         if (ok && c.t.stats_out && half == 0 && row < a.seq)
