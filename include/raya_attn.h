@@ -251,8 +251,12 @@ raya_attn_status raya_attn_forward_packed_noalloc(const raya_attn_desc* desc, co
  * row statistics stats[row] = (m, l): the largest score m_i = max_j x_ij and
  * l_i = sum_j exp(x_ij - m_i) over the allowed keys; (-inf, 0) for a row
  * without keys.  `stats` is a DEVICE array of batch*heads*seq pairs of
- * floats, and log(l) + m is the row's log-sum-exp.  The score accuracy is
- * that of fp32 (3xFP16 products on the tensor cores for head_dim <= 128).
+ * floats, and log(l) + m is the row's log-sum-exp.  Products are as good as
+ * fp32's (3xFP16 on the tensor cores for head_dim <= 128: to 2^-22 of an
+ * element, and absolutely to 2^-40 of the largest of its 64 rows).  An
+ * infinity or NaN at or past valid_len is never read; one in a valid row
+ * spoils what the plain formulas spoil, where a weight of 0 times it counts
+ * as NaN, also for pairs that the mask or the bias excludes.
  *
  * raya_attn_backward takes q, k, v, out and stats of such a forward pass
  * with the same descriptor, valid_len and bias, and dout, the gradient of

@@ -159,9 +159,10 @@ __global__ void __launch_bounds__(kRowThreads) rowwise_train_dq(const __grid_con
           if (lane + 32 * u < d) o[u] = fmaf(w, krow[lane + 32 * u], o[u]);
       }
     }
+    const float f = i < job.valid ? t.scale : 1.f;  // padded rows stay +0 under a negative scale
 #pragma unroll
     for (int u = 0; u < kRowCols; ++u)
-      if (lane + 32 * u < d) dqrow[lane + 32 * u] = o[u] * t.scale;
+      if (lane + 32 * u < d) dqrow[lane + 32 * u] = o[u] * f;
     __syncwarp();
   }
   if (t.part) {
@@ -218,10 +219,11 @@ __global__ void __launch_bounds__(kRowThreads) rowwise_train_dkv(const __grid_co
           }
       }
     }
+    const float f = j < job.valid ? t.scale : 1.f;  // as in rowwise_train_dq
 #pragma unroll
     for (int u = 0; u < kRowCols; ++u)
       if (lane + 32 * u < d) {
-        t.dk[(base + j) * d + lane + 32 * u] = ok[u] * t.scale;
+        t.dk[(base + j) * d + lane + 32 * u] = ok[u] * f;
         t.dv[(base + j) * d + lane + 32 * u] = ov[u];
       }
     __syncwarp();

@@ -4,7 +4,10 @@ kernels may be off, element by element, from the arithmetic they do.
 Products.  The tensor-core kernels take a product of two fp32 numbers as three
 products of their fp16 halves (hi rounded to nearest, lo the rest rounded to
 nearest): each operand is represented to 2^-22 of its value, so two cost
-2^-21, and the dropped lo * lo is at most 2^-22.  A sum over head_dim or over
+2^-21, and the dropped lo * lo is at most 2^-22.  (The weights' hi is
+truncated, so theirs are represented to 2^-21; the chain below is counted long
+enough for that: 12 accumulations follow one another per 64 columns, 24 in all
+for 128, of which the weights' products take 12.)  A sum over head_dim or over
 64 partners is a chain of at most 24 accumulations in fp32 that truncate, 2^-23
 of the running sum of magnitudes each.  The row-wise kernels round d products
 and sums in fp32, 2^-24 each.  So a dot product is off by at most
@@ -89,7 +92,7 @@ def reference(mask, block, scale, valid, q, k, v, dout=None, table=None, max_dis
     w = np.exp(x - m0)
     l = w.sum(-1, keepdims=True)
     p = w / np.where(l > 0, l, 1)
-    a = scale * ((np.abs(q) + small(q)) @ (np.abs(k) + small(k)).swapaxes(-1, -2))
+    a = abs(scale) * ((np.abs(q) + small(q)) @ (np.abs(k) + small(k)).swapaxes(-1, -2))
     dx = np.where(see, e * a + 4 * U * (a + np.abs(bias) + np.abs(m0)), 0.0)
     dxm = dx.max(-1, keepdims=True) if s else dx.sum(-1, keepdims=True)
     n = see.sum(-1, keepdims=True)
@@ -112,8 +115,8 @@ def reference(mask, block, scale, valid, q, k, v, dout=None, table=None, max_dis
     pe = p * dp_rel + 2.0 ** -30 * p.max(-1, keepdims=True, initial=0) * see
     dse = p * (e * da + ddelta + 2 * U * (np.abs(dp) + np.abs(delta))) + pe * (np.abs(dp) + np.abs(delta))
     ta = dse + (e + (n.max(initial=0) + 8) * U) * np.abs(ds)
-    got["dq"] = (scale * (ds @ k), scale * (ta @ (np.abs(k) + small(k))))
-    got["dk"] = (scale * (ds.swapaxes(-1, -2) @ q), scale * (ta.swapaxes(-1, -2) @ (np.abs(q) + small(q))))
+    got["dq"] = (scale * (ds @ k), abs(scale) * (ta @ (np.abs(k) + small(k))))
+    got["dk"] = (scale * (ds.swapaxes(-1, -2) @ q), abs(scale) * (ta.swapaxes(-1, -2) @ (np.abs(q) + small(q))))
     got["dv"] = (p.swapaxes(-1, -2) @ g, (pe + (e + (s + 8) * U) * p).swapaxes(-1, -2) @ ga)
     if table is not None:
         t, tb = np.zeros((2,) + table.shape)

@@ -461,3 +461,83 @@ def test_two_calls_at_once(cuda_device, d):
         got = c.results()
         for n in w:
             assert np.array_equal(got[n], w[n]), n
+
+
+@pytest.mark.parametrize("d", [64, 96, 136])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_scales_that_turn_or_drop_the_scores(cuda_device, d, scale):
+    x, valid = make(2, 2, 150, d, [150, 65], 27, 32)
+    check(x, valid, BLOCK3, 64, scale=scale)
+
+
+@pytest.mark.parametrize("d", [64, 96, 136])
+def test_lengths_outside_the_sequence_are_clamped(cuda_device, d):
+    import torch
+
+    x, valid = make(3, 2, 140, d, [140, 0, 77], 28, 32)
+    calls = [Call(x, valid, BLOCK3, 64) for _ in range(2)]
+    calls[1].valid = torch.tensor([2 ** 31 - 1, -5, 77], dtype=torch.int32, device="cuda")
+    for c in calls:
+        c.forward()
+        c.backward()
+    want, got = (c.results() for c in calls)
+    for n in want:
+        assert np.array_equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("d", [64, 136])
+@pytest.mark.parametrize("mask,block", [(rb.Mask.block(2 ** 31 - 1), 64), (rb.Mask.block(0), 2 ** 31 - 1),
+                                        (rb.Mask.sliding(2 ** 31 - 1), 128), (rb.Mask.block(1), 1)])
+def test_masks_at_their_limits(cuda_device, mask, block, d):
+    x, valid = make(2, 2, 200, d, [200, 131], 29, 32)
+    check(x, valid, mask, block)
+
+
+@pytest.mark.parametrize("batch,heads,seq", [(300, 1, 70), (1, 200, 3), (40, 5, 1)])
+def test_many_short_slices(cuda_device, batch, heads, seq):
+    x, valid = make(batch, heads, seq, 64, None, 30, 32)
+    valid = np.random.default_rng(31).integers(0, seq + 1, batch)
+    check(x, valid, BLOCK3, 64)
+
+
+@pytest.mark.parametrize("d", [64, 96, 136])
+def test_one_tensor_in_several_places(cuda_device, d):
+    """q, k and v (and dout and out) may be the same tensor: nothing reads what another has written."""
+    x, valid = make(1, 2, 190, d, None, 32, 32)
+    x["k"] = x["v"] = x["q"]
+    c = Call(x, valid, BLOCK3, 64)
+    c.t["k"] = c.t["v"] = c.t["q"]
+    c.forward()
+    c.x["dout"] = c.t["out"].cpu().numpy()
+    c.t["dout"] = c.t["out"]
+    c.backward()
+    got, want = c.results(), c.want()
+    for n in want:
+        close(got[n], want[n], n)
+
+
+def test_a_stream_handle_and_a_workspace_of_floats(cuda_device):
+    """The stream as the integer that other libraries hand out, views that start past their storage, a larger workspace
+    of another type, and a bias whose gradient nobody asks for."""
+    import torch
+
+    x, valid = make(2, 2, 200, 64, [200, 77], 33, 32)
+    c = Call(x, valid, BLOCK3, 64)
+    c.forward()
+    c.backward()
+    want = c.results()
+    s = torch.cuda.Stream()
+    size = rb.train_workspace(c.shape, c.params, c.bias, backward=True)
+    ws = torch.empty(size // 4 + 1000, device="cuda")
+    d = Call(x, valid, BLOCK3, 64, stream=s.cuda_stream)
+    for n, y in d.t.items():
+        room = torch.empty(y.numel() + 4, device="cuda")
+        room[4:].copy_(y.reshape(-1))
+        d.t[n] = room[4:].view(y.shape)
+    torch.cuda.synchronize()
+    d.forward(ws)
+    d.dtable = None
+    d.backward(ws)
+    got = d.results()
+    for n in got:
+        assert np.array_equal(got[n], want[n]), n
