@@ -75,7 +75,7 @@ struct TrainPlan {
   int tiles = 0;     // 64-row tiles per slice, an even number
   long long chunk = 0;  // slices whose images the workspace holds at a time
   size_t rel_bias = 0, rel_id = 0, delta = 0, part = 0;
-  size_t img[4] = {}, exps = 0, rows = 0, next = 0;
+  size_t img[4] = {}, scales = 0, rows = 0, next = 0;
   int far = 0, slots = 0;           // the table's gradient by distance (train_tc.cuh)
   size_t dist = 0, dist_bytes = 0;  // where it does not fit into shared memory
   size_t bytes = 0;
@@ -119,7 +119,7 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
     plan->chunk = std::max<long long>(1, std::min<long long>({slices, static_cast<long long>(kMaxImageBytes / ((last - first) * image)),
                                                               0x7fffffffll / (2ll * plan->tiles)}));
     for (int i = first; i < last; ++i) plan->img[i] = take(plan->chunk * image);
-    plan->exps = take(plan->chunk * plan->tiles * sizeof(int4));
+    plan->scales = take(plan->chunk * plan->tiles * sizeof(train::TileScale));
     if (backward) plan->rows = take(static_cast<size_t>(plan->chunk) * plan->tiles * train::kRowValues * sizeof(float));
     plan->next = take(4 * sizeof(unsigned));
     if (bias)  // distances beyond seq do not occur
@@ -218,7 +218,7 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   c.backward = backward;
   c.first_image = !backward && P == 1 ? train::kImgK : train::kImgQ;
   for (int i = c.first_image; i < (backward ? 4 : 3); ++i) c.img[i] = at<uint8_t>(workspace, plan.img[i]);
-  c.exps = at<int4>(workspace, plan.exps);
+  c.scales = at<train::TileScale>(workspace, plan.scales);
   if (backward) c.rows = at<float>(workspace, plan.rows);
   c.next = at<unsigned>(workspace, plan.next);
   c.table = table;

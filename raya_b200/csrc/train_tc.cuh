@@ -7,8 +7,8 @@
 // lo*hi + hi*hi into fp32, and the softmax threads take the exponents off
 // with the factor that they multiply by anyway.  An operand is good to 2^-22
 // of its value, and absolutely to 2^-40 of its tile's largest.  The weights
-// that meet the second operand (w, ds) are scaled per row: w by a constant,
-// ds by an exponent of its own for each row and tile.  Every tile's product
+// that meet the second operand (w, ds) are scaled too: w by a constant, ds by
+// an exponent from a bound for each row and tile.  Every tile's product
 // is added into fp32 registers with rounding to nearest, since the tensor
 // core's accumulation truncates.
 //
@@ -100,11 +100,19 @@ constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
 constexpr float kWeightLog2 = 14.f;                // kDv: w enters as w * 2^14, so that small ones keep their bits
-constexpr int kRowValues = 3 * 64;                 // values per 64 rows of dout
+constexpr int kRowValues = 4 * 64;                 // values per 64 rows of dout; kDk and kDv read the first three of each
 constexpr float kRescale = 8.f, kForwardLog2 = 7.f;  // kForward: p <= 2^8 of the kept maximum, times 2^7
 
 enum TcKind { kForward = 0, kDq = 1, kDk = 2, kDv = 3 };
 enum { kImgQ = 0, kImgK = 1, kImgV = 2, kImgG = 3 };
+
+// What goes with 64 rows of a slice's images: their exponents by tensor, and
+// in units of these (2^e times the value) the longest row of v and of g; the
+// largest |delta|.  Rows that are not finite do not count.
+struct alignas(16) TileScale {
+  int e[4];
+  float v_norm, g_norm, delta, unused;
+};
 
 // What the tensor-core kernels read besides TrainArgs.  The workspace holds
 // one chunk of slices at a time: images, exponents and row values are
@@ -112,8 +120,8 @@ enum { kImgQ = 0, kImgK = 1, kImgV = 2, kImgG = 3 };
 struct TcArgs {
   TrainArgs t;
   uint8_t* img[4];     // [chunk slices][tiles][2 P panels]: q, k, v, dout
-  int4* exps;          // [chunk slices][tiles]: their exponents
-  float* rows;         // [chunk slices][tiles][3][64]: m * log2(e) (inf: no key), that - kWeightLog2, and delta / l
+  TileScale* scales;   // [chunk slices][tiles]
+  float* rows;         // [chunk slices][tiles][4][64]: m * log2(e) (inf: no key), that - kWeightLog2, delta = g . out, |g| 2^e
   const float* table;  // the bias, or nullptr
   float* vec;          // where it goes by distance (t.rel_bias)
   int tiles;           // 64-row tiles per slice (even)
@@ -157,6 +165,7 @@ __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontro
 template <int P>
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcArgs c) {
   __shared__ uint32_t red[8];
+  __shared__ float norms[8], deltas[8];
   const AttnArgs& a = c.t.a;
   const int tid = threadIdx.x, which = c.first_image + blockIdx.y, d = a.head_dim;
   launch_dependents();
@@ -192,6 +201,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   const int c4 = (tid & 15) * 4, r = tid >> 4, live = valid - r0;  // rows below `live` are read
   float4 x[4][P], y[4][P];
   float2 st[4];
+  float delta = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = r + 16 * i;
@@ -228,6 +238,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
         rows[64] = off - kWeightLog2;
         rows[128] = dot;
       }
+      if (fabsf(dot) < INFINITY) delta = fmaxf(delta, fabsf(dot));
     }
   }
   float big = 0.f;
@@ -249,7 +260,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   const int e = tc16::scale_exp(most);
   const float sc = tc16::pow2(e);
   const size_t at_tile = static_cast<size_t>(local) * c.tiles + tile;
-  if (tid == 0) reinterpret_cast<int*>(c.exps + at_tile)[which] = e;
+  if (tid == 0) c.scales[at_tile].e[which] = e;
   uint8_t* img = c.img[which] + at_tile * (2 * P * kPanelBytes);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -263,6 +274,44 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
       *reinterpret_cast<uint2*>(img + at) = make_uint2(h[0], h[1]);
       *reinterpret_cast<uint2*>(img + P * kPanelBytes + at) = make_uint2(l[0], l[1]);
     }
+  if (!c.backward || which < kImgV) return;
+  // The rows' lengths, for the bound on ds (kDq, kDk).
+  float longest = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float square = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const float4 g = make_float4(x[i][p].x * sc, x[i][p].y * sc, x[i][p].z * sc, x[i][p].w * sc);
+      square = fmaf(g.x, g.x, fmaf(g.y, g.y, fmaf(g.z, g.z, fmaf(g.w, g.w, square))));
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) square += __shfl_xor_sync(0xffffffffu, square, off);
+    const float norm = square < INFINITY ? sqrtf(square) : 0.f;
+    longest = fmaxf(longest, norm);
+    if (grad && (tid & 15) == 0) c.rows[at_tile * kRowValues + 192 + r + 16 * i] = norm;
+  }
+  longest = fmaxf(longest, __shfl_xor_sync(0xffffffffu, longest, 16));
+  delta = fmaxf(delta, __shfl_xor_sync(0xffffffffu, delta, 16));
+  if ((tid & 31) == 0) {
+    norms[tid >> 5] = longest;
+    deltas[tid >> 5] = delta;
+  }
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      longest = fmaxf(longest, norms[w]);
+      delta = fmaxf(delta, deltas[w]);
+    }
+    TileScale& t = c.scales[at_tile];
+    if (grad) {
+      t.g_norm = longest;
+      t.delta = delta;
+    } else {
+      t.v_norm = longest;
+    }
+  }
 }
 
 // One unit of work: a 128-row tile of one slice.
@@ -276,8 +325,8 @@ struct TcUnit {
 constexpr int kQueue = 2;
 struct alignas(16) TcTail {
   float vec[kStages][kVec];       // bias * log2(e) by distance
-  float rows[kStages][kRowValues];  // kDk, kDv: the columns' exponents and delta
-  int exps[kStages][4];           // exponents of the columns' 64 rows, by tensor
+  float rows[kStages][192];       // kDk, kDv: the columns' exponents and delta
+  TileScale scales[kStages];      // of the columns' 64 rows
   int flat[kStages];              // the tile's pairs all lie in one distance bucket
   float red[2][2][kTileRows];     // [tile parity][half]: what a row's threads exchange
   TcUnit unit[kQueue];            // the units that the copy warp has begun
@@ -435,7 +484,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
   constexpr int kHalves = P;                                 // threads per row
   constexpr int kW = 64 / kHalves;                           // score columns of a thread
   constexpr int kBlocks = kW / 32;
-  constexpr bool kShared = KIND != kDv && kHalves == 2;      // a row's threads share a maximum
+  constexpr bool kShared = KIND == kForward && kHalves == 2; // a row's threads share a maximum
   constexpr int kRowThreadsTc = 128 * kHalves;
   constexpr int kIssueWarp = kRowWarpsOf(P);                 // then the copy warp and two for the table's gradient
   constexpr uint32_t kCols = 256 * P;
@@ -535,9 +584,10 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     const int vec_at = (kByKey ? rt + 64 : 128 - rt) + kStep * kW * half;
 
     // What a row needs besides its operands: 2^-e of these, the columns that
-    // it sees, and for kDq its exponent and delta.
+    // it sees, for kDq and kDk the (longest) length of the second, and for
+    // kDq its exponent and delta.
     struct Row {
-      float qmul, unit, off, delta;
+      float qmul, unit, off, delta, norm;
       int lo, hi;
     };
     // Unit u's rows, in rounds of two 32-word pieces of a thread (hi and lo
@@ -628,14 +678,16 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     auto load_rows = [&](const TcUnit& u, Row& r) {
       const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64 + ((warp & 3) >> 1);
       if constexpr (!kOwnRows) {
-        const int4 e = c.exps[tile];
-        r.qmul = a.qscale * tc16::pow2(-(kByKey ? e.y : e.x));
-        r.unit = kScores2 ? tc16::pow2(-(kByKey ? e.z : e.w)) : 0.f;
+        const TileScale& s = c.scales[tile];
+        r.qmul = a.qscale * tc16::pow2(-s.e[kA1]);
+        r.unit = kScores2 ? tc16::pow2(-s.e[kA2]) : 0.f;
+        r.norm = KIND == kDk ? s.v_norm : 0.f;
       }
       r.off = r.delta = 0.f;
       if constexpr (KIND == kDq) {
         r.off = c.rows[tile * kRowValues + (rt & 63)];
         r.delta = c.rows[tile * kRowValues + 128 + (rt & 63)];
+        r.norm = c.rows[tile * kRowValues + 192 + (rt & 63)];
       }
       key_range(a, min(u.r0 + rt, u.valid - 1), u.valid, r.lo, r.hi);
 #pragma unroll 1
@@ -732,7 +784,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
         if (!kShared && !ok) break;
         tc_fence_after();
         const uint32_t scol = lane + kColS + 64 * sb + kW * half;
-        const int e1 = sm.exps[st][kB1], e2 = sm.exps[st][kB2];
+        const int e1 = sm.scales[st].e[kB1], e2 = sm.scales[st].e[kB2];
         const int mlo = r.lo - c0, mhi = r.hi - c0;
         const bool inside = __all_sync(0xffffffffu, mlo <= 0 && mhi >= kW);
         const float mult = finite(r.qmul * tc16::pow2(-e1));
@@ -822,72 +874,68 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           factor = tc16::pow2(-e2) * 6.103515625e-05f;  // 2^-14
           prepare_next(t);
         } else {
-          // ds = w (dP - delta), then an exponent for the row: its largest |ds| to [2^14, 2^15)
-          float big = 0.f;
-          if (ok) {
-            const float unit = finite(r.unit * tc16::pow2(-e2));
-            const float2 unit2 = make_float2(unit, unit);
+          // ds = w (g . v - delta) times 2^e, which brings the bound |g| |v| +
+          // |delta| (w <= 1, the column's or the row's longest vector) to
+          // [2^13, 2^14): four times that still fit, should rounding bring a
+          // weight above 1.  fp16 holds what is 2^-38 of the bound; a pass
+          // for the largest |ds| itself would gain a few bits for 9% of the time.
+          const float unit = finite(r.unit * tc16::pow2(-e2));
+          const float bound = KIND == kDq ? fmaf(r.norm * sm.scales[st].v_norm, unit, fabsf(r.delta))
+                                          : fmaf(r.norm * sm.scales[st].g_norm, unit, sm.scales[st].delta);
+          const int e = tc16::scale_exp(__float_as_uint(finite(bound))) - 1;
+          const float up = tc16::pow2(e), down = tc16::pow2(-e);
+          const float unit_up = finite(unit * up), minus_up = KIND == kDq ? -r.delta * up : -up;
+          const float2 unit2 = make_float2(unit_up, unit_up), minus2 = make_float2(minus_up, minus_up);
 #pragma unroll 1
-            for (int q = 0; q < kBlocks; ++q) {
-              const float* off = sm.rows[st] + kW * half + 32 * q;
-              float s[32], dp[32];
-              block_scores(q, s, dp);
+          for (int q = 0; q < kBlocks; ++q) {
+            const float* off = sm.rows[st] + kW * half + 32 * q;
+            float s[32], dp[32];
+            block_scores(q, s, dp);
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                float4 f, g;
-                if constexpr (KIND == kDk) {
-                  f = *reinterpret_cast<const float4*>(off + i);
-                  g = *reinterpret_cast<const float4*>(off + 128 + i);
-                } else {
-                  f = make_float4(r.off, r.off, r.off, r.off);
-                  g = make_float4(r.delta, r.delta, r.delta, r.delta);
-                }
-                const float2 x = sub2(get2(s + i), make_float2(f.x, f.y));
-                const float2 y = sub2(get2(s + i + 2), make_float2(f.z, f.w));
-                put2(s + i, __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)),
-                                       __ffma2_rn(get2(dp + i), unit2, make_float2(-g.x, -g.y))));
-                put2(s + i + 2, __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)),
-                                           __ffma2_rn(get2(dp + i + 2), unit2, make_float2(-g.z, -g.w))));
-                big = fmax3(big, fabsf(s[i]), fabsf(s[i + 1]));
-                big = fmax3(big, fabsf(s[i + 2]), fabsf(s[i + 3]));
+            for (int i = 0; i < 32; i += 4) {
+              float4 f;
+              float2 g0 = minus2, g1 = minus2;
+              if constexpr (KIND == kDk) {
+                f = *reinterpret_cast<const float4*>(off + i);
+                const float4 g = *reinterpret_cast<const float4*>(off + 128 + i);
+                g0 = __fmul2_rn(make_float2(g.x, g.y), minus2);
+                g1 = __fmul2_rn(make_float2(g.z, g.w), minus2);
+              } else {
+                f = make_float4(r.off, r.off, r.off, r.off);
               }
-              tmem_st32(scol + 32 * q, s);
-              if (with_grad && ok) {
-                const int base = c0 + 32 * q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
-                if (base - 31 >= c.far || base + 31 <= -c.far) {          // all beyond the last bound
-                  float x = 0.f;
+              const float2 x = sub2(get2(s + i), make_float2(f.x, f.y));
+              const float2 y = sub2(get2(s + i + 2), make_float2(f.z, f.w));
+              put2(s + i, __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)), __ffma2_rn(get2(dp + i), unit2, g0)));
+              put2(s + i + 2, __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(get2(dp + i + 2), unit2, g1)));
+            }
+            store_weights(scol + 32 * q, s);
+            if (with_grad) {
+              const int base = c0 + 32 * q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
+              if (base - 31 >= c.far || base + 31 <= -c.far) {          // all beyond the last bound
+                float2 x = get2(s), y = get2(s + 2);
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) x += s[i];
-                  if (base > 0)
-                    far_after += x;
-                  else
-                    far_before += x;
-                } else {
-                  ok = ds_return(q);
-                  if (ok) {
+                for (int i = 4; i < 32; i += 4) {
+                  x = __fadd2_rn(x, get2(s + i));
+                  y = __fadd2_rn(y, get2(s + i + 2));
+                }
+                const float sum = (x.x + x.y) + (y.x + y.y);
+                if (base > 0)
+                  far_after = fmaf(sum, down, far_after);
+                else
+                  far_before = fmaf(sum, down, far_before);
+              } else {
+                ok = ok && ds_return(q);
+                if (ok) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                      *reinterpret_cast<float4*>(buf + q * kBlockBytes + ln * 128 + (((i >> 2) ^ (ln & 7)) << 4)) =
-                          make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
-                    __syncwarp();
-                    if (ln == 0) mbar_arrive(&sm.ds_ready[warp * kBlocks + q]);
-                    ds_used |= 1u << q;
-                  }
+                  for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<float4*>(buf + q * kBlockBytes + ln * 128 + (((i >> 2) ^ (ln & 7)) << 4)) =
+                        make_float4(s[i] * down, s[i + 1] * down, s[i + 2] * down, s[i + 3] * down);
+                  __syncwarp();
+                  if (ln == 0) mbar_arrive(&sm.ds_ready[warp * kBlocks + q]);
+                  ds_used |= 1u << q;
                 }
               }
             }
-            tmem_wait_st();
-          }
-          if (!share_max(G, big)) { ok = false; break; }
-          const int e = tc16::scale_exp(__float_as_uint(big));
-          const float2 up = make_float2(tc16::pow2(e), tc16::pow2(e));
-#pragma unroll 1
-          for (int q = 0; q < kBlocks; ++q) {
-            float s[32];
-            tmem_ld32(scol + 32 * q, s);
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) put2(s + i, __fmul2_rn(get2(s + i), up));
-            store_weights(scol + 32 * q, s);
           }
           tmem_wait_st();
           tc_fence_before();
@@ -1177,13 +1225,14 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           unsigned char* op = smem + st * stage_bytes<P>();
           uint64_t* bar = &sm.full[st];
           if constexpr (BIAS) sm.flat[st] = rel + 1 >= c.far || rel + kVec - 1 <= -c.far;
-          mbar_arrive_expect_tx(bar, 2 * kOp + 16u + (BIAS ? kVec * 4u : 0u) + (kByKey ? kRowValues * 4u : 0u));
+          constexpr uint32_t kScaleBytes = sizeof(TileScale), kRowBytes = 192 * 4;
+          mbar_arrive_expect_tx(bar, 2 * kOp + kScaleBytes + (BIAS ? kVec * 4u : 0u) + (kByKey ? kRowBytes : 0u));
           tma_load_1d(op, c.img[kB1] + tile * static_cast<long long>(kOp), kOp, bar);
           tma_load_1d(op + kOp, c.img[kB2] + tile * static_cast<long long>(kOp), kOp, bar);
-          tma_load_1d(sm.exps[st], c.exps + tile, 16u, bar);
+          tma_load_1d(&sm.scales[st], c.scales + tile, kScaleBytes, bar);
           if constexpr (BIAS)
             tma_load_1d(sm.vec[st], c.t.rel_bias + (2ll * head + 1) * c.t.rel_half + rel, kVec * 4u, bar);
-          if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * kRowValues, kRowValues * 4u, bar);
+          if constexpr (kByKey) tma_load_1d(sm.rows[st], c.rows + tile * kRowValues, kRowBytes, bar);
         }
         __syncwarp();
         ++copied;

@@ -115,8 +115,13 @@ def reference(mask, block, scale, valid, q, k, v, dout=None, table=None, max_dis
     pe = p * dp_rel + 2.0 ** -30 * p.max(-1, keepdims=True, initial=0) * see
     dse = p * (e * da + ddelta + 2 * U * (np.abs(dp) + np.abs(delta))) + pe * (np.abs(dp) + np.abs(delta))
     ta = dse + (e + (n.max(initial=0) + 8) * U) * np.abs(ds)
-    got["dq"] = (scale * (ds @ k), abs(scale) * (ta @ (np.abs(k) + small(k))))
-    got["dk"] = (scale * (ds.swapaxes(-1, -2) @ q), abs(scale) * (ta.swapaxes(-1, -2) @ (np.abs(q) + small(q))))
+    # ds is held in fp16 halves to 2^-38 of the bound on it, |g_i| max |v_j| + |delta_i| with g = dout / l
+    most = np.where(n > 0, (np.sqrt((g * g).sum(-1, keepdims=True)) * np.sqrt((v * v).sum(-1)).max(-1, initial=0)[..., None, None] + np.abs(delta))
+                    / np.where(l > 0, l, 1), 0.0)
+    lost = 2.0 ** -38
+    taq, tak = ta + lost * most * see, ta + lost * most.max(-2, initial=0, keepdims=True) * see
+    got["dq"] = (scale * (ds @ k), abs(scale) * (taq @ (np.abs(k) + small(k))))
+    got["dk"] = (scale * (ds.swapaxes(-1, -2) @ q), abs(scale) * (tak.swapaxes(-1, -2) @ (np.abs(q) + small(q))))
     got["dv"] = (p.swapaxes(-1, -2) @ g, (pe + (e + (s + 8) * U) * p).swapaxes(-1, -2) @ ga)
     if table is not None:
         t, tb = np.zeros((2,) + table.shape)
