@@ -249,7 +249,8 @@ raya_attn_status ensure_ready(int dev, DeviceCtx** out) {
     for (auto fn : {tc_train<train::kForward, 1, false>, tc_train<train::kForward, 1, true>,
                     tc_train<train::kForward, 2, false>, tc_train<train::kForward, 2, true>,
                     tc_train<train::kDq, 1, false>, tc_train<train::kDq, 1, true>, tc_train<train::kDq, 2, false>,
-                    tc_train<train::kDq, 2, true>, tc_train<train::kDk, 1, false>, tc_train<train::kDk, 1, true>,
+                    tc_train<train::kDq, 2, true>, tc_train<train::kDq, 1, true, true>,
+                    tc_train<train::kDq, 2, true, true>, tc_train<train::kDk, 1, false>, tc_train<train::kDk, 1, true>,
                     tc_train<train::kDk, 2, false>, tc_train<train::kDk, 2, true>, tc_train<train::kDv, 1, false>,
                     tc_train<train::kDv, 1, true>, tc_train<train::kDv, 2, false>, tc_train<train::kDv, 2, true>}) {
       e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -77,7 +77,8 @@ struct TrainPlan {
   size_t rel_bias = 0, rel_id = 0, delta = 0, part = 0;
   size_t img[4] = {}, scales = 0, rows = 0, next = 0;
   int far = 0, slots = 0;           // the table's gradient by distance (train_tc.cuh)
-  size_t dist = 0, dist_bytes = 0;  // where it does not fit into shared memory
+  size_t dist = 0;                  // where it does not fit into shared memory,
+  long long dist_ctas = 0;          // for that many CTAs (0: it fits)
   size_t bytes = 0;
 };
 
@@ -125,12 +126,13 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
     if (bias)  // distances beyond seq do not occur
       plan->far = static_cast<int>(std::min<int64_t>(bucket_bounds(bias->buckets, bias->max_distance).at[bias->buckets / 2 - 1], d->seq));
     if (backward && bias) {
-      plan->slots = 2 * plan->far + 128;
-      const size_t bytes = size_t{2} * plan->slots * sizeof(float);
+      plan->slots = train::dist_slots(plan->far);
+      const size_t bytes = size_t{8} * plan->slots * sizeof(float);
       const size_t spare = plan->panels == 1 ? train::kHalfSm - train::tc_smem<1>() : train::kWholeSm - train::tc_smem<2>();
       if (bytes > spare) {
-        plan->dist_bytes = kMaxResident * bytes;
-        plan->dist = take(plan->dist_bytes);
+        // Tables of very many distances: fewer CTAs rather than more than 1 GiB.
+        plan->dist_ctas = std::max<long long>(1, std::min<long long>(kMaxResident, (1ll << 30) / static_cast<long long>(bytes)));
+        plan->dist = take(plan->dist_ctas * bytes);
       }
     }
   } else {
@@ -229,10 +231,10 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   size_t dist = 0;
   if (t.part) {
     c.slots = plan.slots;
-    if (plan.dist_bytes > 0)
+    if (plan.dist_ctas > 0)
       c.dist = at<float>(workspace, plan.dist);
     else
-      dist = size_t{2} * plan.slots * sizeof(float);
+      dist = size_t{8} * plan.slots * sizeof(float);
   }
   const long long resident = std::min(kMaxResident, static_cast<long long>(sms) * (P == 1 ? 2 : 1));
   const bool bias = t.rel_bias != nullptr;
@@ -243,7 +245,7 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
     train::split_kernel<P><<<dim3(static_cast<unsigned>(n), (backward ? 4 : 3) - c.first_image + (bias ? 1 : 0)), 256, 0, stream>>>(c);
     raya_attn_status st = check_launch("operand split launch");
     if (st != RAYA_ATTN_OK) return st;
-    auto launch_kind = [&](void (*fn)(train::TcArgs, CUtensorMap, CUtensorMap), size_t shared, float* out, const char* what) {
+    auto launch_kind = [&](void (*fn)(train::TcArgs, CUtensorMap, CUtensorMap), size_t shared, long long ctas, float* out, const char* what) {
       CUtensorMap map, q_map{};
       raya_attn_status encoded = encode_rows3d(&map, out, t.a.head_dim, t.a.seq, slices);
       if (encoded == RAYA_ATTN_OK && c.first_image == train::kImgK)
@@ -253,7 +255,7 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
       overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
       overlap.val.programmaticStreamSerializationAllowed = 1;
       cudaLaunchConfig_t config{};
-      config.gridDim = dim3(static_cast<unsigned>(std::min(n / 2, resident)));
+      config.gridDim = dim3(static_cast<unsigned>(std::min(n / 2, ctas)));
       config.blockDim = dim3(train::tc_threads(P));
       config.dynamicSmemBytes = shared;
       config.stream = stream;
@@ -264,15 +266,18 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
     };
     using train::tc_train;
     if (!backward) {
-      st = launch_kind(bias ? tc_train<train::kForward, P, true> : tc_train<train::kForward, P, false>, smem, t.a.out, "forward launch");
+      st = launch_kind(bias ? tc_train<train::kForward, P, true> : tc_train<train::kForward, P, false>, smem, resident, t.a.out, "forward launch");
       if (st != RAYA_ATTN_OK) return st;
       continue;
     }
-    st = launch_kind(bias ? tc_train<train::kDq, P, true> : tc_train<train::kDq, P, false>, smem + dist, t.dq, "query gradient launch");
+    st = launch_kind(t.part  ? tc_train<train::kDq, P, true, true>
+                     : bias ? tc_train<train::kDq, P, true>
+                            : tc_train<train::kDq, P, false>,
+                     smem + dist, c.dist ? std::min(resident, plan.dist_ctas) : resident, t.dq, "query gradient launch");
     if (st == RAYA_ATTN_OK)
-      st = launch_kind(bias ? tc_train<train::kDk, P, true> : tc_train<train::kDk, P, false>, smem, t.dk, "key gradient launch");
+      st = launch_kind(bias ? tc_train<train::kDk, P, true> : tc_train<train::kDk, P, false>, smem, resident, t.dk, "key gradient launch");
     if (st == RAYA_ATTN_OK)
-      st = launch_kind(bias ? tc_train<train::kDv, P, true> : tc_train<train::kDv, P, false>, smem, t.dv, "value gradient launch");
+      st = launch_kind(bias ? tc_train<train::kDv, P, true> : tc_train<train::kDv, P, false>, smem, resident, t.dv, "value gradient launch");
     if (st != RAYA_ATTN_OK) return st;
   }
   return RAYA_ATTN_OK;

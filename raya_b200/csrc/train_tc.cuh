@@ -132,9 +132,9 @@ struct TcArgs {
   unsigned* next;      // [4] by kind: units handed out beyond the first one of each CTA; split_kernel clears them
   BucketBounds bounds;
   int far;             // the last bucket's first distance
-  // With t.part, the table's gradient:
-  int slots;           // distances kept apart: -far - 63 ... far + 64 (a near block reaches 62 beyond the last bound)
-  float* dist;         // [CTAs][2][slots] where shared memory does not hold them, or nullptr
+  // With t.part, the table's gradient by distance:
+  int slots;           // dist_slots(far)
+  float* dist;         // [CTAs][8][slots] where shared memory does not hold them, or nullptr
 };
 
 __device__ __forceinline__ int valid_of(const AttnArgs& a, long long bh) {
@@ -323,21 +323,22 @@ struct TcUnit {
 
 // Shared memory behind the operand stages.
 constexpr int kQueue = 2;
+template <int P>
 struct alignas(16) TcTail {
   float vec[kStages][kVec];       // bias * log2(e) by distance
   float rows[kStages][192];       // kDk, kDv: the columns' exponents and delta
   TileScale scales[kStages];      // of the columns' 64 rows
   int flat[kStages];              // the tile's pairs all lie in one distance bucket
-  float red[2][2][kTileRows];     // [tile parity][half]: what a row's threads exchange
+  float red[2][2][P == 2 ? kTileRows : 1];  // [tile parity][half]: what a row's threads exchange
   TcUnit unit[kQueue];            // the units that the copy warp has begun
   uint64_t u_full[kQueue], u_free[kQueue];
   uint64_t full[kStages], freed[kStages];
   uint64_t s_full[2], w_ready[2], part_full, part_free, a_ready;
   uint64_t rows_full[8];          // by row warp
   // The table's gradient: each row warp's blocks of ds in its buffer, and at a
-  // unit's end its sums beyond the last bound on either side.
+  // unit's end each row's sums beyond the last bound on either side.
   uint64_t ds_ready[8], ds_free[8], far_ready, far_free;
-  float far[8][2];
+  float2 far[4 * P][32];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -352,7 +353,7 @@ constexpr size_t stage_bytes() { return 2ull * 2 * P * kPanelBytes; }
 constexpr int kBlockBytes = 32 * 128, kRowBuf = 2 * kBlockBytes;
 template <int P>
 constexpr size_t tc_smem() {
-  return 1024 + kStages * stage_bytes<P>() + kRowWarpsOf(P) * kRowBuf + sizeof(TcTail);
+  return 1024 + kStages * stage_bytes<P>() + kRowWarpsOf(P) * kRowBuf + sizeof(TcTail<P>);
 }
 // head_dim <= 64: two CTAs (2 x 256 tensor-memory columns) share an SM and a
 // third does not fit beside them.
@@ -442,25 +443,37 @@ __device__ __forceinline__ void mask_scores(float* s, float mult, const float* v
 }
 
 // The sums along the diagonals of a 32 x 32 block (32 rows of 128 bytes under
-// the 128-byte swizzle): before is that of column - row = lane - 31, after
-// that of lane + 1.  Lane k reads column (k + 1 + row) mod 32 of every row: no
-// bank conflict.
-__device__ __forceinline__ void diagonal_sums(const float* block, int lane, float& before, float& after) {
-  before = after = 0.f;
+// the 128-byte swizzle).  Lane (a, b) = (lane / 8, lane % 8) takes row 4 m + a,
+// columns 4 ((m + b) mod 8) ... + 3 for m = 0 ... 7: column - row + a is 4 b ...
+// + 3 while m + b < 8 (in `upper`), 32 less behind that (in `lower`).
+// 16-byte loads without a bank conflict, and half the instructions of one
+// column per lane and row.
+__device__ __forceinline__ void diagonal_sums(const float* block, int lane, float2* upper, float2* lower) {
+  const int a = lane >> 3, b = lane & 7;
+  float4 x[8];
 #pragma unroll
-  for (int r0 = 0; r0 < 32; r0 += 16) {
-    float x[16];
+  for (int m = 0; m < 8; ++m)
+    x[m] = *reinterpret_cast<const float4*>(block + (4 * m + a) * 32 + ((((m + b) & 7) ^ ((4 * m + a) & 7)) << 2));
+  upper[0] = upper[1] = lower[0] = lower[1] = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = block[(r0 + r) * 32 + (((lane + 1 + r0 + r) & 31) ^ ((r & 7) << 2))];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      if (lane >= 31 - r0 - r)
-        before += x[r];
-      else
-        after += x[r];
+  for (int m = 0; m < 8; ++m) {
+    if (m + b < 8) {
+      upper[0] = __fadd2_rn(upper[0], make_float2(x[m].x, x[m].y));
+      upper[1] = __fadd2_rn(upper[1], make_float2(x[m].z, x[m].w));
+    } else {
+      lower[0] = __fadd2_rn(lower[0], make_float2(x[m].x, x[m].y));
+      lower[1] = __fadd2_rn(lower[1], make_float2(x[m].z, x[m].w));
     }
   }
 }
+
+// Whether some pair of a block of 32 x 32 lies below the last bucket's bound;
+// base: column - row of its first pair.
+__device__ __forceinline__ bool near_block(int base, int far) { return base - 31 < far && base + 31 > -far; }
+// Distances are kept in four copies by a, that of D at slot mid + D + a.  Near
+// blocks have -far - 61 ... far + 61 and touch 64 slots from mid + base - 32.
+constexpr int dist_mid(int far) { return (far + 67) / 4 * 4; }
+constexpr int dist_slots(int far) { return (dist_mid(far) + far + 68) / 4 * 4; }
 
 // The launches of a call overlap.  kForward and kDq start while split_kernel
 // ends and wait for it before they read what it wrote; kDk and kDv start
@@ -471,8 +484,9 @@ __device__ __forceinline__ void diagonal_sums(const float* block, int lane, floa
 // Persistent: the copy warp takes one unit after the other (the first by
 // blockIdx, the others from a counter, since padding makes them uneven) and
 // hands them to the other warps.  Every barrier and ring runs on across them:
-// G counts the CTA's 64-column tiles, U its units with any.
-template <int KIND, int P, bool BIAS>
+// G counts the CTA's 64-column tiles, U its units with any.  GRAD (kDq): the
+// table's gradient as well.
+template <int KIND, int P, bool BIAS, bool GRAD = false>
 __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     const __grid_constant__ TcArgs c, const __grid_constant__ CUtensorMap out_map,
     const __grid_constant__ CUtensorMap q_map) {
@@ -501,11 +515,11 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
   extern __shared__ unsigned char raw[];
   unsigned char* const smem = raw + (((smem_addr(raw) + 1023u) & ~1023u) - smem_addr(raw));
   unsigned char* const row_bufs = smem + kStages * stage_bytes<P>();
-  TcTail& sm = *reinterpret_cast<TcTail*>(row_bufs + kRowWarpsOf(P) * kRowBuf);
+  TcTail<P>& sm = *reinterpret_cast<TcTail<P>*>(row_bufs + kRowWarpsOf(P) * kRowBuf);
 
   const AttnArgs& a = c.t.a;
   const int tid = threadIdx.x, warp = tid >> 5, d = a.head_dim;
-  const bool with_grad = KIND == kDq && c.t.part != nullptr;
+  static_assert(!GRAD || (KIND == kDq && BIAS), "the table's gradient goes with dq");
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -528,7 +542,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     mbar_init(&sm.far_free, 1);
     for (int s = 0; s < kQueue; ++s) {
       mbar_init(&sm.u_full[s], 1);
-      mbar_init(&sm.u_free[s], kIssueWarp + (with_grad ? 3 : 1));
+      mbar_init(&sm.u_free[s], kIssueWarp + (GRAD ? 3 : 1));
     }
     sm.abort_flag = 0;
     fence_mbar_init();
@@ -673,9 +687,11 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
       }
       return tc16::pow2(-e);
     };
-    // The rest of a unit's rows (its first round is on the way) and what goes
-    // with them.  Called when the scores of the unit before are complete.
-    auto load_rows = [&](const TcUnit& u, Row& r) {
+    // A unit's rows (their first round is on the way) and what goes with them,
+    // in two steps so that something can be done while the second round comes.
+    // Called when the scores of the unit before are complete.
+    static_assert(kRounds <= 2, "rounds of a unit's rows");
+    auto load_first = [&](const TcUnit& u, Row& r) -> bool {
       const long long tile = static_cast<long long>(u.local) * c.tiles + u.r0 / 64 + ((warp & 3) >> 1);
       if constexpr (!kOwnRows) {
         const TileScale& s = c.scales[tile];
@@ -690,12 +706,14 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
         r.norm = c.rows[tile * kRowValues + 192 + (rt & 63)];
       }
       key_range(a, min(u.r0 + rt, u.valid - 1), u.valid, r.lo, r.hi);
-#pragma unroll 1
-      for (int round = 0; round < kRounds; ++round) {
-        if (round > 0) fetch_rows(u, round);
-        if (!place_rows(round)) return false;
-      }
+      if (!place_rows(0)) return false;
+      if constexpr (kRounds == 2) fetch_rows(u, 1);
       if constexpr (kOwnRows) r.qmul = a.qscale * split_row(u.r0 + rt < u.valid);
+      return true;
+    };
+    auto load_rest = [&]() -> bool {
+      if constexpr (kRounds == 2)
+        if (!place_rows(1)) return false;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&sm.a_ready);
@@ -707,11 +725,11 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     int G = 0;
     bool ok = true;  // the same on every lane of the warp
     int units = 0;
-    uint32_t ds_used = 0, ds_phase = 0;  // by block: whether it has been handed over, the parity of its next return
+    uint32_t ds_used = 0, ds_phase = 0;  // GRAD, by block: whether it is with the table's warps, the parity of its next return
     ok = take_unit(u);
     if (u.n > 0) {
       fetch_rows(u, 0);
-      ok = load_rows(u, r);
+      ok = load_first(u, r) && load_rest();
     }
     for (;;) {
       // Warps that meet at barriers of their own leave together.
@@ -720,8 +738,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
       const int row = u.r0 + rt;
       const size_t first_row = static_cast<size_t>(c.slice0 + u.local) * a.seq + u.r0;
       float far_before = 0.f, far_after = 0.f;
-      if (with_grad) {
-        if (ln == 0) tma_store_wait_read();  // the last unit's way out, before the blocks of ds
+      if constexpr (GRAD) {
+        if (ln == 0) tma_store_wait_read();  // the last unit's way out, before the columns of ds
         __syncwarp();
       }
       float o[kOutCols];
@@ -745,7 +763,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
         return true;
       };
       // Block q of the buffer is back from the table's warps.
-      auto ds_return = [&](int q) {
+      auto ds_return = [&](int q) -> bool {
         if (!(ds_used >> q & 1u)) return true;
         if (!warp_wait(&sm.ds_free[warp * kBlocks + q], ds_phase >> q)) return false;
         ds_phase ^= 1u << q;
@@ -768,18 +786,18 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
       };
       auto prepare_next = [&](int t) {
         if (t + 1 < u.n) return;
-        if (with_grad) {
+        if constexpr (GRAD) {
 #pragma unroll
           for (int q = 0; q < kBlocks; ++q) ok = ok && ds_return(q);
           begin_next();
         }
-        if (ok && nu.n > 0) ok = load_rows(nu, nr);
+        if (ok && nu.n > 0) ok = load_first(nu, nr) && (kScores2 || load_rest());
       };
 
       for (int t = 0; t < u.n; ++t, ++G) {
         const int st = G % kStages, c0 = (u.t0 + t) * kTileCols + kW * half;
         const int sb = kScores2 ? 0 : G & 1;
-        if (!with_grad && t + 1 == u.n) begin_next();
+        if (!GRAD && t + 1 == u.n) begin_next();
         if (ok) ok = warp_wait(&sm.full[st], G / kStages) && warp_wait(&sm.s_full[sb], kScores2 ? G : G >> 1);
         if (!kShared && !ok) break;
         tc_fence_after();
@@ -909,27 +927,30 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
               put2(s + i + 2, __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(get2(dp + i + 2), unit2, g1)));
             }
             store_weights(scol + 32 * q, s);
-            if (with_grad) {
+            if constexpr (GRAD) {
               const int base = c0 + 32 * q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
-              if (base - 31 >= c.far || base + 31 <= -c.far) {          // all beyond the last bound
+              if (!near_block(base, c.far)) {
                 float2 x = get2(s), y = get2(s + 2);
 #pragma unroll
                 for (int i = 4; i < 32; i += 4) {
                   x = __fadd2_rn(x, get2(s + i));
                   y = __fadd2_rn(y, get2(s + i + 2));
                 }
-                const float sum = (x.x + x.y) + (y.x + y.y);
+                const float sum = ((x.x + x.y) + (y.x + y.y)) * down;
                 if (base > 0)
-                  far_after = fmaf(sum, down, far_after);
+                  far_after += sum;
                 else
-                  far_before = fmaf(sum, down, far_before);
+                  far_before += sum;
               } else {
                 ok = ok && ds_return(q);
                 if (ok) {
+                  const float2 down2 = make_float2(down, down);
 #pragma unroll
-                  for (int i = 0; i < 32; i += 4)
+                  for (int i = 0; i < 32; i += 4) {
+                    const float2 x = __fmul2_rn(get2(s + i), down2), y = __fmul2_rn(get2(s + i + 2), down2);
                     *reinterpret_cast<float4*>(buf + q * kBlockBytes + ln * 128 + (((i >> 2) ^ (ln & 7)) << 4)) =
-                        make_float4(s[i] * down, s[i + 1] * down, s[i + 2] * down, s[i + 3] * down);
+                        make_float4(x.x, x.y, y.x, y.y);
+                  }
                   __syncwarp();
                   if (ln == 0) mbar_arrive(&sm.ds_ready[warp * kBlocks + q]);
                   ds_used |= 1u << q;
@@ -943,6 +964,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           factor = finite(tc16::pow2(-e) * tc16::pow2(-e1));
           prepare_next(t);
           if (ok) ok = add_partial(G);
+          if (ok && t + 1 == u.n && nu.n > 0) ok = load_rest();
         }
       }
       if constexpr (!kScores2)
@@ -962,21 +984,15 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
                             : make_float2(-INFINITY, 0.f);
         __syncwarp();
       }
-      if (with_grad && ok) {
-        // The warp's sums beyond the last bound, to the table's warps.
-        if (units > 0) ok = warp_wait(&sm.far_free, units - 1);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-          far_before += __shfl_xor_sync(0xffffffffu, far_before, off);
-          far_after += __shfl_xor_sync(0xffffffffu, far_after, off);
+      if constexpr (GRAD) {
+        // The rows' sums beyond the last bound, to the table's warps.
+        if (ok && units > 0) ok = warp_wait(&sm.far_free, units - 1);
+        if (ok) {
+          sm.far[warp][ln] = make_float2(far_before, far_after);
+          __syncwarp();
+          if (ln == 0) mbar_arrive(&sm.far_ready);
+          ++units;
         }
-        if (ln == 0) {
-          sm.far[warp][0] = far_before;
-          sm.far[warp][1] = far_after;
-          mbar_arrive(&sm.far_ready);
-        }
-        __syncwarp();
-        ++units;
       }
       if (ok) {
         const bool live = row < u.valid;
@@ -1105,43 +1121,54 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     }
     // Nothing arrives on a barrier after the CTA has ended.
     for (int g = max(0, committed - kStages); ok && g < committed; ++g) ok = warp_wait(&sm.freed[g % kStages], g / kStages);
-  } else if (with_grad && warp > kIssueWarp + 1) {
+  } else if (GRAD && warp > kIssueWarp + 1) {
     // ---------------- the table's gradient ----------------
     // Two warps, each with the row warps of its parity: their near blocks of
     // ds (some pair below the last bound) by distance, and at the unit's end
     // the distances by bucket, everything in a fixed order.  Beside the row
     // threads, whose own diagonal sums took 1.6k cycles a block and 7k a unit.
     const int me = warp - (kIssueWarp + 2), ln = tid & 31;
-    float* const all = c.dist ? c.dist + static_cast<size_t>(blockIdx.x) * 2 * c.slots : reinterpret_cast<float*>(&sm + 1);
-    float* const dist = all + me * c.slots;
-    const int mid = c.far + 63;  // the slot of distance 0
+    float* const all = c.dist ? c.dist + static_cast<size_t>(blockIdx.x) * 8 * c.slots : reinterpret_cast<float*>(&sm + 1);
+    float* const dist = all + 4 * me * c.slots;
+    const int mid = dist_mid(c.far);
     uint32_t phase = 0;
     bool ok = true;
     TcUnit u;
     for (int units = 0;; ++units) {
       const bool got = take_unit(u);
       if (bar_any(kTableBarrier, 64, !got) || u.n <= 0) break;  // both leave together
-      for (int i = ln; i < c.slots; i += 32) dist[i] = 0.f;
+      for (int i = ln; i < c.slots; i += 32) reinterpret_cast<float4*>(dist)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       __syncwarp();
       for (int t = 0; ok && t < u.n; ++t)
         for (int w = me; ok && w < kIssueWarp; w += 2)
           for (int q = 0; ok && q < kBlocks; ++q) {
             const int base = (u.t0 + t) * kTileCols + kW * (w >> 2) + 32 * q - (u.r0 + (w & 3) * 32);
-            if (base - 31 >= c.far || base + 31 <= -c.far) continue;
+            if (!near_block(base, c.far)) continue;
             const int i = w * kBlocks + q;
             ok = warp_wait(&sm.ds_ready[i], phase >> i);
             if (!ok) break;
             phase ^= 1u << i;
-            float before, after;
-            diagonal_sums(reinterpret_cast<const float*>(row_bufs + w * kRowBuf + q * kBlockBytes), ln, before, after);
+            float2 upper[2], lower[2];
+            diagonal_sums(reinterpret_cast<const float*>(row_bufs + w * kRowBuf + q * kBlockBytes), ln, upper, lower);
             __syncwarp();
             if (ln == 0) mbar_arrive(&sm.ds_free[i]);
-            dist[mid + base + ln - 31] += before;
-            __syncwarp();
-            dist[mid + base + ln + 1] += after;  // lane 31: 0, one slot past the block's distances
+            float4* const at = reinterpret_cast<float4*>(dist + (ln >> 3) * c.slots + mid + base) + (ln & 7);
+            const float4 x = at[0], y = at[-8];
+            at[0] = make_float4(x.x + upper[0].x, x.y + upper[0].y, x.z + upper[1].x, x.w + upper[1].y);
+            at[-8] = make_float4(y.x + lower[0].x, y.y + lower[0].y, y.z + lower[1].x, y.w + lower[1].y);
             __syncwarp();
           }
       if (ok) ok = warp_wait(&sm.far_ready, units);
+      float2 far = make_float2(0.f, 0.f);
+      for (int w = 0; ok && w < kIssueWarp; ++w) {
+        far.x += sm.far[w][ln].x;
+        far.y += sm.far[w][ln].y;
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        far.x += __shfl_xor_sync(0xffffffffu, far.x, off);
+        far.y += __shfl_xor_sync(0xffffffffu, far.y, off);
+      }
       if (bar_any(kTableBarrier, 64, !ok)) break;
       float* partial = c.t.part + (static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets;
       const int sides = c.t.buckets / 2;
@@ -1152,14 +1179,16 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           const bool behind = b >= sides;  // keys after the query
           const int k = behind ? b - sides : b;
           const int from = max(c.bounds.at[k], behind ? 1 : 0);
-          const int to = k + 1 < sides ? min(c.bounds.at[k + 1], c.far + 64) : c.far + 64;
-#pragma unroll 4
+          const int to = k + 1 < sides ? min(c.bounds.at[k + 1], c.far + 62) : c.far + 62;
+#pragma unroll 2
           for (int i = from + (ln & 3); i < to; i += 4) {
-            const int at = mid + (behind ? i : -i);
-            x += all[at] + all[c.slots + at];
+            const float* const at = all + mid + (behind ? i : -i);
+            float y[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) y[p] = at[p * c.slots + (p & 3)];
+            x += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
           }
-          if (k + 1 == sides && (ln & 3) == 0)
-            for (int w = 0; w < kIssueWarp; ++w) x += sm.far[w][behind];
+          if (k + 1 == sides && (ln & 3) == 0) x += behind ? far.y : far.x;
         }
         x += __shfl_xor_sync(0xffffffffu, x, 1);
         x += __shfl_xor_sync(0xffffffffu, x, 2);
