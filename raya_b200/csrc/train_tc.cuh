@@ -1159,40 +1159,39 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
             __syncwarp();
           }
       if (ok) ok = warp_wait(&sm.far_ready, units);
-      float2 far = make_float2(0.f, 0.f);
-      for (int w = 0; ok && w < kIssueWarp; ++w) {
-        far.x += sm.far[w][ln].x;
-        far.y += sm.far[w][ln].y;
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        far.x += __shfl_xor_sync(0xffffffffu, far.x, off);
-        far.y += __shfl_xor_sync(0xffffffffu, far.y, off);
-      }
       if (bar_any(kTableBarrier, 64, !ok)) break;
-      float* partial = c.t.part + (static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets;
-      const int sides = c.t.buckets / 2;
-      for (int b0 = 8 * me; b0 < c.t.buckets; b0 += 16) {  // four lanes to a bucket
-        const int b = b0 + (ln >> 2);
-        float x = 0.f;
-        if (b < c.t.buckets) {
-          const bool behind = b >= sides;  // keys after the query
-          const int k = behind ? b - sides : b;
-          const int from = max(c.bounds.at[k], behind ? 1 : 0);
-          const int to = k + 1 < sides ? min(c.bounds.at[k + 1], c.far + 62) : c.far + 62;
-#pragma unroll 2
-          for (int i = from + (ln & 3); i < to; i += 4) {
-            const float* const at = all + mid + (behind ? i : -i);
-            float y[8];
+      // Warp 0 has the keys up to the query, warp 1 those behind it.  First
+      // each distance's eight copies into one (in its own slot of the first
+      // copy), those from the last bound on into `beyond`.
+      const bool behind = me == 1;
+      float beyond = 0.f;
+      for (int w = 0; w < kIssueWarp; ++w) beyond += behind ? sm.far[w][ln].y : sm.far[w][ln].x;
+      for (int i = me + ln; i < c.far + 62; i += 32) {
+        float* const at = all + mid + (behind ? i : -i);
+        float y[8];
 #pragma unroll
-            for (int p = 0; p < 8; ++p) y[p] = at[p * c.slots + (p & 3)];
-            x += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-          }
-          if (k + 1 == sides && (ln & 3) == 0) x += behind ? far.y : far.x;
+        for (int p = 0; p < 8; ++p) y[p] = at[p * c.slots + (p & 3)];
+        const float x = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+        if (i >= c.far)
+          beyond += x;
+        else
+          at[0] = x;
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) beyond += __shfl_xor_sync(0xffffffffu, beyond, off);
+      __syncwarp();
+      const int sides = c.t.buckets / 2;
+      float* const partial = c.t.part + (static_cast<size_t>(c.slice0 + u.local) * c.t.parts + u.r0 / kTileRows) * c.t.buckets + me * sides;
+      for (int k0 = 0; k0 < sides; k0 += 8) {  // four lanes to a bucket
+        const int k = k0 + (ln >> 2);
+        float x = 0.f;
+        if (k + 1 < sides) {
+          const int to = min(c.bounds.at[k + 1], c.far);
+          for (int i = max(c.bounds.at[k], me) + (ln & 3); i < to; i += 4) x += all[mid + (behind ? i : -i)];
         }
         x += __shfl_xor_sync(0xffffffffu, x, 1);
         x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if (b < c.t.buckets && (ln & 3) == 0) partial[b] = x;
+        if (k < sides && (ln & 3) == 0) partial[k] = k + 1 == sides ? beyond : x;
       }
       if (bar_any(kTableBarrier, 64, false)) break;  // both are done with the distances and the far sums
       if (me == 0 && ln == 0) mbar_arrive(&sm.far_free);
