@@ -217,7 +217,6 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   train::TcArgs c{};
   c.t = t;
   c.tiles = plan.tiles;
-  c.backward = backward;
   c.first_image = !backward && P == 1 ? train::kImgK : train::kImgQ;
   for (int i = c.first_image; i < (backward ? 4 : 3); ++i) c.img[i] = at<uint8_t>(workspace, plan.img[i]);
   c.scales = at<train::TileScale>(workspace, plan.scales);
@@ -242,7 +241,11 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
   for (c.slice0 = 0; c.slice0 < slices; c.slice0 += plan.chunk) {
     const long long n = std::min(plan.chunk, slices - c.slice0) * plan.tiles;
     c.units = static_cast<unsigned>(n / 2);
-    train::split_kernel<P><<<dim3(static_cast<unsigned>(n), (backward ? 4 : 3) - c.first_image + (bias ? 1 : 0)), 256, 0, stream>>>(c);
+    const dim3 split_grid(static_cast<unsigned>(n), (backward ? 4 : 3) - c.first_image + (bias ? 1 : 0));
+    if (backward)
+      train::split_kernel<P, true><<<split_grid, 256, 0, stream>>>(c);
+    else
+      train::split_kernel<P, false><<<split_grid, 256, 0, stream>>>(c);
     raya_attn_status st = check_launch("operand split launch");
     if (st != RAYA_ATTN_OK) return st;
     auto launch_kind = [&](void (*fn)(train::TcArgs, CUtensorMap, CUtensorMap), size_t shared, long long ctas, float* out, const char* what) {

@@ -125,7 +125,6 @@ struct TcArgs {
   const float* table;  // the bias, or nullptr
   float* vec;          // where it goes by distance (t.rel_bias)
   int tiles;           // 64-row tiles per slice (even)
-  bool backward;
   int first_image;     // kImgK where the forward kernel splits q itself, else kImgQ
   long long slice0;
   unsigned units;      // 128-row tiles of the chunk
@@ -158,18 +157,20 @@ __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontro
 
 // 64 rows of one tensor into their image.  256 threads: 16 lanes take a row's
 // 64 columns of a panel (16-byte loads, 8-byte stores), 16 rows at a time.
-// blockIdx.y: the tensor, and behind them the bias by distance.  Tiles of padding write the zeros of the results
-// there instead.  Bound by HBM: 4 bytes read and 4 written per element
-// (dout: 8 read), 75 to 80% of the copy rate (8 x 16 x 8192, backward: 2.0 GB
-// in 388 us).
-template <int P>
-__global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcArgs c) {
+// blockIdx.y: the tensor, and behind them the bias by distance.  Tiles of
+// padding write the zeros of the results there instead.  Bound by HBM: 4 bytes
+// read and 4 written per element (dout: 8 read), 96% of the copy rate forward
+// (8 x 16 x 8192: 0.88 GB in 140 us), 88% backward (64 x 12 x 512, half of it
+// valid: 0.67 GB in 116 us).  With four blocks on an SM, which the registers
+// of all of dout's and out's loads at once allow, it was 176 and 131.
+template <int P, bool BACK>
+__global__ void __launch_bounds__(256, P == 1 ? (BACK ? 5 : 6) : 3) split_kernel(const __grid_constant__ TcArgs c) {
   __shared__ uint32_t red[8];
   __shared__ float norms[8], deltas[8];
   const AttnArgs& a = c.t.a;
   const int tid = threadIdx.x, which = c.first_image + blockIdx.y, d = a.head_dim;
   launch_dependents();
-  if (which == 4 || (which == 3 && !c.backward)) {
+  if (which == 4 || (which == 3 && !BACK)) {
     rel_table(c.table, a.heads, c.t.buckets, c.t.rel_half, c.bounds, c.vec, nullptr, blockIdx.x * 256ll + tid,
               gridDim.x * 256ll);
     return;
@@ -183,62 +184,71 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
   const size_t first = static_cast<size_t>(bh) * a.seq + r0;
   if (r0 >= (valid + 127) / 128 * 128) {  // no 128-row tile reads it: padding, whose results are zero
     float* o = nullptr;
-    if (c.backward)
+    if (BACK)
       o = which == kImgQ ? c.t.dq : which == kImgK ? c.t.dk : which == kImgV ? c.t.dv : nullptr;
     else if (which == kImgV)
       o = a.out;
     const int rows = min(64, a.seq - r0);
     if (o)
       for (int i = tid; i < rows * d / 4; i += 256) st_stream(o + first * d + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f));
-    if (!c.backward && which == kImgV && c.t.stats_out && tid < rows) c.t.stats_out[first + tid] = make_float2(-INFINITY, 0.f);
+    if (!BACK && which == kImgV && c.t.stats_out && tid < rows) c.t.stats_out[first + tid] = make_float2(-INFINITY, 0.f);
     if (c.t.part && which == kImgQ && tile % 2 == 0 && tid < c.t.buckets)
       c.t.part[(static_cast<size_t>(bh) * c.t.parts + tile / 2) * c.t.buckets + tid] = 0.f;
     return;
   }
   const float* __restrict__ src = (which == kImgQ ? a.q : which == kImgK ? a.k : which == kImgV ? a.v : c.t.dout) + first * d;
   const float* __restrict__ out = a.out + first * d;
-  const bool grad = which == kImgG;
+  const bool grad = BACK && which == kImgG;
   const int c4 = (tid & 15) * 4, r = tid >> 4, live = valid - r0;  // rows below `live` are read
-  float4 x[4][P], y[4][P];
-  float2 st[4];
-  float delta = 0.f;
+  float4 x[4][P];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r + 16 * i;
-    st[i] = make_float2(0.f, 0.f);
-    if (grad && row < live) st[i] = __ldg(c.t.stats + first + row);
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const int col = 64 * p + c4;
-      x[i][p] = y[i][p] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < live && col < d) {
-        x[i][p] = __ldcs(reinterpret_cast<const float4*>(src + static_cast<size_t>(row) * d + col));
-        if (grad) y[i][p] = __ldcs(reinterpret_cast<const float4*>(out + static_cast<size_t>(row) * d + col));
-      }
+      const int row = r + 16 * i, col = 64 * p + c4;
+      x[i][p] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < live && col < d) x[i][p] = __ldcs(reinterpret_cast<const float4*>(src + static_cast<size_t>(row) * d + col));
     }
-  }
+  float delta = 0.f;
   if (grad) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float m2, linv, dot = 0.f;
-      row_stats(st[i], m2, linv);
+    for (int half = 0; half < 4; half += 2) {  // two rows of out at a time, for a fifth block on the SM
+      float4 y[2][P];
+      float2 st[2];
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        float4& g = x[i][p];
-        const float4 o = y[i][p];
-        g = make_float4(g.x * linv, g.y * linv, g.z * linv, g.w * linv);
-        dot = fmaf(g.x, o.x, fmaf(g.y, o.y, fmaf(g.z, o.z, fmaf(g.w, o.w, dot))));
+      for (int i = 0; i < 2; ++i) {
+        const int row = r + 16 * (half + i);
+        st[i] = make_float2(0.f, 0.f);
+        if (row < live) st[i] = __ldg(c.t.stats + first + row);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const int col = 64 * p + c4;
+          y[i][p] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (row < live && col < d) y[i][p] = __ldcs(reinterpret_cast<const float4*>(out + static_cast<size_t>(row) * d + col));
+        }
       }
 #pragma unroll
-      for (int off = 8; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-      if ((tid & 15) == 0) {
-        float* rows = c.rows + (static_cast<size_t>(local) * c.tiles + tile) * kRowValues + r + 16 * i;
-        const float off = linv != 0.f ? m2 : INFINITY;  // 2^(x - inf) = 0: no key, or past valid_len
-        rows[0] = off;
-        rows[64] = off - kWeightLog2;
-        rows[128] = dot;
+      for (int i = 0; i < 2; ++i) {
+        float m2, linv, dot = 0.f;
+        row_stats(st[i], m2, linv);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          float4& g = x[half + i][p];
+          const float4 o = y[i][p];
+          g = make_float4(g.x * linv, g.y * linv, g.z * linv, g.w * linv);
+          dot = fmaf(g.x, o.x, fmaf(g.y, o.y, fmaf(g.z, o.z, fmaf(g.w, o.w, dot))));
+        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+        if ((tid & 15) == 0) {
+          float* rows = c.rows + (static_cast<size_t>(local) * c.tiles + tile) * kRowValues + r + 16 * (half + i);
+          const float off = linv != 0.f ? m2 : INFINITY;  // 2^(x - inf) = 0: no key, or past valid_len
+          rows[0] = off;
+          rows[64] = off - kWeightLog2;
+          rows[128] = dot;
+        }
+        if (fabsf(dot) < INFINITY) delta = fmaxf(delta, fabsf(dot));
       }
-      if (fabsf(dot) < INFINITY) delta = fmaxf(delta, fabsf(dot));
     }
   }
   float big = 0.f;
@@ -274,7 +284,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ TcAr
       *reinterpret_cast<uint2*>(img + at) = make_uint2(h[0], h[1]);
       *reinterpret_cast<uint2*>(img + P * kPanelBytes + at) = make_uint2(l[0], l[1]);
     }
-  if (!c.backward || which < kImgV) return;
+  if (!BACK || which < kImgV) return;
   // The rows' lengths, for the bound on ds (kDq, kDk).
   float longest = 0.f;
 #pragma unroll
