@@ -104,15 +104,22 @@ __global__ void __launch_bounds__(256) rel_table_kernel(const float* table, int 
   rel_table(table, heads, buckets, half, b, vec, ids, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
 }
 
+// Programmatic dependent launch.  A kernel that says launch_dependents lets the
+// next one's CTAs start where it leaves room; wait_for_primary returns when
+// the kernel before is complete and its writes are visible.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // dtable[head][b] = the sum of its partials over the batch and the parts of
 // each slice, always in the same order (one block per head and bucket; 256
 // strided sums, then a tree), in 64 bits: thousands of partials of either
-// sign meet here.
+// sign meet here.  Its blocks wait beside the end of the launch before.
 __global__ void __launch_bounds__(256) bias_grad_kernel(const float* __restrict__ part, int batch, int heads, int parts,
                                                         int buckets, float* __restrict__ dtable) {
   __shared__ double sum[256];
   const int h = blockIdx.x, b = blockIdx.y;
   double s = 0.0;
+  wait_for_primary();
   const long long n = static_cast<long long>(batch) * parts;
   for (long long t = threadIdx.x; t < n; t += 256) {
     const long long seq = t / parts, at = (seq * heads + h) * parts + t % parts;

@@ -210,6 +210,14 @@ raya_attn_status encode_rows3d(CUtensorMap* map, const float* base, uint64_t hea
   return RAYA_ATTN_OK;
 }
 
+// A launch that may begin where the one before leaves room (train_common.cuh).
+cudaLaunchAttribute early_launch() {
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  return overlap;
+}
+
 // Chunk by chunk: the images of its slices, then every 128-row tile of them.
 template <int P>
 raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, const float* table, const train::BucketBounds& bounds,
@@ -254,9 +262,7 @@ raya_attn_status launch_tc(const TrainPlan& plan, const train::TrainArgs& t, con
       if (encoded == RAYA_ATTN_OK && c.first_image == train::kImgK)
         encoded = encode_rows3d(&q_map, t.a.q, t.a.head_dim, t.a.seq, slices);
       if (encoded != RAYA_ATTN_OK) return encoded;
-      cudaLaunchAttribute overlap{};  // with the end of the launch before (train_tc.cuh)
-      overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      overlap.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchAttribute overlap = early_launch();
       cudaLaunchConfig_t config{};
       config.gridDim = dim3(static_cast<unsigned>(std::min(n / 2, ctas)));
       config.blockDim = dim3(train::tc_threads(P));
@@ -346,9 +352,16 @@ raya_attn_status train_call(const raya_attn_desc* d, const TrainIo& io, const ra
     st = launch_rowwise(plan, t, bias ? bias->table : nullptr, bounds, workspace, stream, backward);
   if (st != RAYA_ATTN_OK) return st;
   if (io.dtable) {
-    train::bias_grad_kernel<<<dim3(static_cast<unsigned>(d->heads), static_cast<unsigned>(bias->buckets)), 256, 0, stream>>>(
-        t.part, static_cast<int>(d->batch), static_cast<int>(d->heads), plan.parts, bias->buckets, io.dtable);
-    st = check_launch("bias gradient launch");
+    cudaLaunchAttribute overlap = early_launch();
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(d->heads), static_cast<unsigned>(bias->buckets));
+    config.blockDim = dim3(256);
+    config.stream = stream;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    const cudaError_t launched = cudaLaunchKernelEx(&config, train::bias_grad_kernel, static_cast<const float*>(t.part), static_cast<int>(d->batch),
+                                                    static_cast<int>(d->heads), plan.parts, static_cast<int>(bias->buckets), io.dtable);
+    st = launched == cudaSuccess ? check_launch("bias gradient launch") : cuda_fail(launched, "bias gradient launch");
   }
   return st;
 }

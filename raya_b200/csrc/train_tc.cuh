@@ -149,12 +149,6 @@ __device__ __forceinline__ void split_near(float x, float y, uint32_t& h, uint32
   l = tc16::pack_f16x2(x - back.x, y - back.y);
 }
 
-// Programmatic dependent launch.  A kernel that says launch_dependents lets the
-// next one's CTAs start where it leaves room; wait_for_primary returns when
-// the kernel before is complete and its writes are visible.
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // 64 rows of one tensor into their image.  256 threads: 16 lanes take a row's
 // 64 columns of a panel (16-byte loads, 8-byte stores), 16 rows at a time.
 // blockIdx.y: the tensor, and behind them the bias by distance.  Tiles of
@@ -488,8 +482,8 @@ constexpr int dist_slots(int far) { return (dist_mid(far) + far + 68) / 4 * 4; }
 // The launches of a call overlap.  kForward and kDq start while split_kernel
 // ends and wait for it before they read what it wrote; kDk and kDv start
 // where the gradient before leaves room, which is after it waited for
-// split_kernel itself, so they wait for it only before they end (a kernel
-// behind them is to find all three complete).
+// split_kernel itself, so they wait for it only before they end (whatever is
+// behind them, the sum of the partials first, is to find all three complete).
 //
 // Persistent: the copy warp takes one unit after the other (the first by
 // blockIdx, the others from a counter, since padding makes them uneven) and
@@ -1228,7 +1222,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
       }
       if (first) {
         if constexpr (kBehindSplit) wait_for_primary();
-        if constexpr (KIND == kDq || KIND == kDk) launch_dependents();
+        if constexpr (KIND != kForward) launch_dependents();
         first = false;
       }
       if ((tid & 31) == 0) unit = gridDim.x + atomicAdd(c.next + KIND, 1u);  // the next one, used a unit later
