@@ -900,7 +900,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           // |delta| (w <= 1, the column's or the row's longest vector) to
           // [2^13, 2^14): four times that still fit, should rounding bring a
           // weight above 1.  fp16 holds what is 2^-38 of the bound; a pass
-          // for the largest |ds| itself would gain a few bits for 9% of the time.
+          // for the largest |ds| itself would gain a few bits for 4% of the time.
           const float unit = finite(r.unit * tc16::pow2(-e2));
           const float bound = KIND == kDq ? fmaf(r.norm * sm.scales[st].v_norm, unit, fabsf(r.delta))
                                           : fmaf(r.norm * sm.scales[st].g_norm, unit, sm.scales[st].delta);
