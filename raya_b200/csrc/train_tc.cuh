@@ -399,6 +399,30 @@ __device__ __forceinline__ void tmem_ld32x2(uint32_t at0, float* v0, uint32_t at
   }
 }
 
+// Four k-steps (16 each) of D (+)= A B as tc16::mma_f16_ts_e issues one: A
+// from tensor memory, its steps A1, A2 and A3 columns behind the first, B's
+// descriptors STEP apart.
+template <uint32_t IDESC, int STEP, int A1, int A2, int A3>
+__device__ __forceinline__ void mma4_ts_e(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+      "add.u32 a1, %1, %6;\n\t"
+      "add.u32 a2, %1, %7;\n\t"
+      "add.u32 a3, %1, %8;\n\t"
+      "add.u64 b1, %2, %9;\n\t"
+      "add.u64 b2, %2, 2 * %9;\n\t"
+      "add.u64 b3, %2, 3 * %9;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.b32 t, %5, 0;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, {%5, %5, %5, %5}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, {%5, %5, %5, %5}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, {%5, %5, %5, %5}, t;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "n"(IDESC), "r"(accumulate), "r"(0u), "n"(A1), "n"(A2), "n"(A3), "n"(STEP)
+      : "memory");
+}
+
 // Weights w[32] (fp32, already scaled) as fp16 hi and lo over their scores.
 __device__ __forceinline__ void store_weights(uint32_t taddr, const float* w) {
 #pragma unroll
@@ -1044,38 +1068,27 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     // rows x columns^T into dcol: the small products first
     auto scores = [&](uint32_t dcol, uint32_t acol, uint32_t b) {
       const uint32_t ah = tmem + acol, al = ah + 32 * P, bl = b + P * kPanelBytes;
-      uint32_t add = 0;
+      auto four = [&](uint32_t at, uint32_t op, uint32_t add) {
+        mma4_ts_e<tc16::kIdescQK, 2, 8, 16, 24>(tmem + dcol, at, tc16::b_desc(op, 0), add);
+      };
 #pragma unroll
-      for (int p = 0; p < P; ++p)
+      for (int p = 0; p < P; ++p) four(ah + 32 * p, bl + p * kPanelBytes, p > 0 ? 1u : 0u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          tc16::mma_f16_ts_e<tc16::kIdescQK>(tmem + dcol, ah + 32 * p + 8 * k, tc16::b_desc(bl + p * kPanelBytes, k), add);
-          add = 1;
-        }
+      for (int p = 0; p < P; ++p) four(al + 32 * p, b + p * kPanelBytes, 1u);
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc16::mma_f16_ts_e<tc16::kIdescQK>(tmem + dcol, al + 32 * p + 8 * k, tc16::b_desc(b + p * kPanelBytes, k), 1u);
-#pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc16::mma_f16_ts_e<tc16::kIdescQK>(tmem + dcol, ah + 32 * p + 8 * k, tc16::b_desc(b + p * kPanelBytes, k), 1u);
+      for (int p = 0; p < P; ++p) four(ah + 32 * p, b + p * kPanelBytes, 1u);
     };
     // weights x operand (its 64 rows are the inner dimension) into the partial
     auto sums = [&](uint32_t wcol, uint32_t b) {
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const uint32_t dcol = tmem + kColPart + 64 * p, bhi = b + p * kPanelBytes, blo = bhi + P * kPanelBytes;
-        auto hi_at = [&](int k) { return tmem + wcol + 32 * (k >> 1) + 8 * (k & 1); };
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k), tc16::v_desc(blo, k), k > 0 ? 1u : 0u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k) + 16, tc16::v_desc(bhi, k), 1u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tc16::mma_f16_ts_e<tc16::kIdescPV>(dcol, hi_at(k), tc16::v_desc(bhi, k), 1u);
+        const uint32_t w = tmem + wcol, bhi = b + p * kPanelBytes, blo = bhi + P * kPanelBytes;
+        auto four = [&](uint32_t at, uint32_t op, uint32_t add) {
+          mma4_ts_e<tc16::kIdescPV, 128, 8, 32, 40>(tmem + kColPart + 64 * p, at, tc16::v_desc(op, 0), add);
+        };
+        four(w, blo, 0u);
+        four(w + 16, bhi, 1u);
+        four(w, bhi, 1u);
       }
     };
     int G = 0, U = 0;
