@@ -399,27 +399,50 @@ __device__ __forceinline__ void tmem_ld32x2(uint32_t at0, float* v0, uint32_t at
   }
 }
 
-// Four k-steps (16 each) of D (+)= A B as tc16::mma_f16_ts_e issues one: A
-// from tensor memory, its steps A1, A2 and A3 columns behind the first, B's
-// descriptors STEP apart.
+// D (+)= A B over 64 of the inner dimension in split fp16, A from tensor memory:
+// hi lo + lo hi + hi hi, the small products first, each in four k-steps of 16:
+// A's steps A1, A2 and A3 columns behind the first, B's descriptors STEP
+// apart.  As tc16::mma_f16_ts_e, but one statement: with a statement for each
+// of the twelve, 47 cycles apart where the tensor core takes 32, the kernels
+// took 2 to 4% longer.
 template <uint32_t IDESC, int STEP, int A1, int A2, int A3>
-__device__ __forceinline__ void mma4_ts_e(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
+__device__ __forceinline__ void mma12_ts_e(uint32_t d, uint32_t a_hi, uint32_t a_lo, uint64_t b_hi, uint64_t b_lo, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
-      "add.u32 a1, %1, %6;\n\t"
-      "add.u32 a2, %1, %7;\n\t"
-      "add.u32 a3, %1, %8;\n\t"
-      "add.u64 b1, %2, %9;\n\t"
-      "add.u64 b2, %2, 2 * %9;\n\t"
-      "add.u64 b3, %2, 3 * %9;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.eq.b32 t, %5, 0;\n\t"
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r;\n\t.reg .b32 h0, h1, h2, h3, l0, l1, l2, l3;\n\t"
+      ".reg .b64 x0, x1, x2, x3, y0, y1, y2, y3;\n\t"
+      "mov.b32 h0, %1;\n\t"
+      "add.u32 h1, %1, %8;\n\t"
+      "add.u32 h2, %1, %9;\n\t"
+      "add.u32 h3, %1, %10;\n\t"
+      "mov.b32 l0, %2;\n\t"
+      "add.u32 l1, %2, %8;\n\t"
+      "add.u32 l2, %2, %9;\n\t"
+      "add.u32 l3, %2, %10;\n\t"
+      "mov.b64 x0, %3;\n\t"
+      "add.u64 x1, %3, 1 * %11;\n\t"
+      "add.u64 x2, %3, 2 * %11;\n\t"
+      "add.u64 x3, %3, 3 * %11;\n\t"
+      "mov.b64 y0, %4;\n\t"
+      "add.u64 y1, %4, 1 * %11;\n\t"
+      "add.u64 y2, %4, 2 * %11;\n\t"
+      "add.u64 y3, %4, 3 * %11;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.eq.b32 t, %7, 0;\n\t"
       "elect.sync r|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, {%5, %5, %5, %5}, t;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, {%5, %5, %5, %5}, t;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, {%5, %5, %5, %5}, t;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "n"(IDESC), "r"(accumulate), "r"(0u), "n"(A1), "n"(A2), "n"(A3), "n"(STEP)
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h0], y0, %5, {%7, %7, %7, %7}, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h1], y1, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h2], y2, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h3], y3, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [l0], x0, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [l1], x1, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [l2], x2, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [l3], x3, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h0], x0, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h1], x1, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h2], x2, %5, {%7, %7, %7, %7}, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [h3], x3, %5, {%7, %7, %7, %7}, t;\n\t"
+      "}" ::"r"(d),
+      "r"(a_hi), "r"(a_lo), "l"(b_hi), "l"(b_lo), "n"(IDESC), "r"(accumulate), "r"(0u), "n"(A1), "n"(A2), "n"(A3), "n"(STEP)
       : "memory");
 }
 
@@ -1065,30 +1088,22 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     auto operand = [&](int g, int which) {
       return ops + static_cast<uint32_t>((g % kStages) * stage_bytes<P>() + which * kOp);
     };
-    // rows x columns^T into dcol: the small products first
+    // rows x columns^T into dcol
     auto scores = [&](uint32_t dcol, uint32_t acol, uint32_t b) {
-      const uint32_t ah = tmem + acol, al = ah + 32 * P, bl = b + P * kPanelBytes;
-      auto four = [&](uint32_t at, uint32_t op, uint32_t add) {
-        mma4_ts_e<tc16::kIdescQK, 2, 8, 16, 24>(tmem + dcol, at, tc16::b_desc(op, 0), add);
-      };
 #pragma unroll
-      for (int p = 0; p < P; ++p) four(ah + 32 * p, bl + p * kPanelBytes, p > 0 ? 1u : 0u);
-#pragma unroll
-      for (int p = 0; p < P; ++p) four(al + 32 * p, b + p * kPanelBytes, 1u);
-#pragma unroll
-      for (int p = 0; p < P; ++p) four(ah + 32 * p, b + p * kPanelBytes, 1u);
+      for (int p = 0; p < P; ++p) {
+        const uint32_t hi = tmem + acol + 32 * p, bhi = b + p * kPanelBytes;
+        mma12_ts_e<tc16::kIdescQK, 2, 8, 16, 24>(tmem + dcol, hi, hi + 32 * P, tc16::b_desc(bhi, 0),
+                                                 tc16::b_desc(bhi + P * kPanelBytes, 0), p > 0 ? 1u : 0u);
+      }
     };
     // weights x operand (its 64 rows are the inner dimension) into the partial
     auto sums = [&](uint32_t wcol, uint32_t b) {
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const uint32_t w = tmem + wcol, bhi = b + p * kPanelBytes, blo = bhi + P * kPanelBytes;
-        auto four = [&](uint32_t at, uint32_t op, uint32_t add) {
-          mma4_ts_e<tc16::kIdescPV, 128, 8, 32, 40>(tmem + kColPart + 64 * p, at, tc16::v_desc(op, 0), add);
-        };
-        four(w, blo, 0u);
-        four(w + 16, bhi, 1u);
-        four(w, bhi, 1u);
+        const uint32_t hi = tmem + wcol, bhi = b + p * kPanelBytes;
+        mma12_ts_e<tc16::kIdescPV, 128, 8, 32, 40>(tmem + kColPart + 64 * p, hi, hi + 16, tc16::v_desc(bhi, 0),
+                                                   tc16::v_desc(bhi + P * kPanelBytes, 0), 0u);
       }
     };
     int G = 0, U = 0;
