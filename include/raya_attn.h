@@ -256,7 +256,9 @@ raya_attn_status raya_attn_forward_packed_noalloc(const raya_attn_desc* desc, co
  * element, and absolutely to 2^-40 of the largest of its 64 rows).  An
  * infinity or NaN at or past valid_len is never read; one in a valid row
  * spoils what the plain formulas spoil, where a weight of 0 times it counts
- * as NaN, also for pairs that the mask or the bias excludes.
+ * as NaN, also for pairs that the mask or the bias excludes.  Scores are
+ * recomputed backward: beyond about 10^6 in magnitude, where fp32 leaves p no
+ * digit, gradients may be infinite.
  *
  * raya_attn_backward takes q, k, v, out and stats of such a forward pass
  * with the same descriptor, valid_len and bias, and dout, the gradient of
