@@ -353,7 +353,9 @@ constexpr size_t stage_bytes() { return 2ull * 2 * P * kPanelBytes; }
 // swizzle.  The next unit's rows come in through it by bulk copies, the
 // output leaves through it by tensor stores (which clip rows past seq and
 // columns past head_dim), and neither holds the row threads up: with loads
-// and stores of their own these took 5 to 7k of a unit's 30k cycles.
+// and stores of their own these took 5 to 7k of a unit's 30k cycles.  Whatever
+// writes into the buffer (rows coming in, ds for the table's gradient, the
+// output) first waits for the store that reads it.
 constexpr int kBlockBytes = 32 * 128, kRowBuf = 2 * kBlockBytes;
 template <int P>
 constexpr size_t tc_smem() {
@@ -1070,6 +1072,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
       if (ok) {
         const bool live = row < u.valid;
         const int wr0 = u.r0 + (warp & 3) * 32;
+        if (ln == 0) tma_store_wait_read();  // a last unit fetches no rows: the one before may still be on its way out
+        __syncwarp();
 #pragma unroll
         for (int q = 0; q < kOutCols; q += 32) {
 #pragma unroll

@@ -1,0 +1,88 @@
+"""The training operators where every CTA takes several units of work: the
+persistent kernels run two CTAs on an SM for head_dim up to 64 and one for 72
+to 128, so these calls have at least twice as many 128-row units as CTAs.
+Compared with the plain form in 64 bits (tests/_train.py), and with
+themselves: a row of one unit that got a value of another would show in both."""
+import numpy as np
+import pytest
+
+import raya_b200 as rb
+from _train import close
+from test_train_gpu import Call, make
+
+pytestmark = pytest.mark.gpu
+
+OWN, WINDOW, FULL = rb.Mask.block(0), rb.Mask.sliding(40), rb.Mask.FULL
+SMS = 148
+
+
+def lengths(batch, seq, seed):
+    """Uneven, most of them past the last unit's first row; the first ones whole, empty and of one row."""
+    rng = np.random.default_rng(seed)
+    valid = rng.integers((seq - 1) // 128 * 128 + 1, seq + 1, batch)
+    valid[:3] = seq, 0, 1
+    return valid
+
+
+def units(valid, heads):
+    return int(((valid + 127) // 128).sum()) * heads
+
+
+CASES = [
+    # batch, heads, seq, head_dim, mask, block, buckets, whether the table's gradient is asked for
+    (80, 8, 64, 64, OWN, 64, 0, False),  # one 64-column tile a unit
+    (80, 8, 64, 64, OWN, 64, 32, True),
+    (80, 8, 200, 64, OWN, 64, 32, False),
+    (80, 8, 150, 64, WINDOW, 128, 0, False),
+    (80, 8, 150, 64, WINDOW, 128, 32, True),
+    (80, 8, 150, 64, FULL, 128, 0, False),
+    (80, 8, 150, 64, FULL, 128, 32, False),
+    (80, 8, 150, 64, FULL, 128, 32, True),
+    (40, 8, 300, 64, rb.Mask.block(1), 64, 32, True),
+    (80, 8, 140, 40, WINDOW, 128, 16, True),
+    (80, 8, 70, 8, FULL, 128, 0, False),
+    (40, 8, 64, 96, OWN, 64, 0, False),
+    (40, 8, 64, 96, OWN, 64, 32, True),
+    (40, 8, 150, 96, WINDOW, 128, 32, False),
+    (40, 8, 150, 96, FULL, 128, 0, False),
+    (40, 8, 150, 72, FULL, 128, 64, True),
+    (40, 8, 64, 128, OWN, 64, 0, False),
+    (40, 8, 64, 128, OWN, 64, 32, True),
+    (40, 8, 150, 128, WINDOW, 128, 0, False),
+    (40, 8, 150, 128, WINDOW, 128, 32, True),
+    (40, 8, 150, 128, FULL, 128, 32, False),
+    (20, 8, 300, 128, rb.Mask.block(1), 64, 32, True),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x) for x in c[:4] + (c[4].name(),) + c[5:]))
+def test_several_units_per_cta(cuda_device, case):
+    import torch
+
+    batch, heads, seq, d, mask, block, buckets, grad = case
+    assert torch.cuda.get_device_properties(0).multi_processor_count == SMS
+    valid = lengths(batch, seq, seq + d)
+    assert units(valid, heads) >= 2 * SMS * (2 if d <= 64 else 1)
+    x, valid = make(batch, heads, seq, d, valid, seq + d + 1, buckets)
+    c = Call(x, valid, mask, block)
+    if not grad:
+        c.dtable = None
+    c.forward()
+    first = c.results()
+    c.poison()
+    c.backward()
+    got = {**c.results(), **{n: first[n] for n in ("out", "m", "l")}}
+    want = c.want()
+    for n in ("out", "m", "l", "dq", "dk", "dv") + (("dtable",) if grad else ()):
+        close(got[n], want[n], n)
+    pad = np.broadcast_to(np.arange(seq)[None, None, :] >= valid[:, None, None], (batch, heads, seq))
+    for n in ("out", "dq", "dk", "dv"):
+        assert (got[n][pad] == 0).all() and not np.signbit(got[n][pad]).any(), f"{n}: padded rows are not +0"
+    for _ in range(3):
+        for n in ("out", "dq", "dk", "dv"):
+            c.t[n].fill_(7.0)
+        c.forward()
+        c.backward()
+        again = c.results()
+        for n in ("out", "dq", "dk", "dv") + (("dtable",) if grad else ()):
+            assert np.array_equal(again[n], got[n]), n
