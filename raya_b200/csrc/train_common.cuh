@@ -113,9 +113,11 @@ __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontro
 // dtable[head][b] = the sum of its partials over the batch and the parts of
 // each slice, always in the same order (one block per head and bucket; 256
 // strided sums, then a tree), in 64 bits: thousands of partials of either
-// sign meet here.  Its blocks wait beside the end of the launch before.
-__global__ void __launch_bounds__(256) bias_grad_kernel(const float* __restrict__ part, int batch, int heads, int parts,
-                                                        int buckets, float* __restrict__ dtable) {
+// sign meet here.  Its blocks wait beside the end of the launch before, while
+// the partials are still being written: they are no read-only data, and are
+// read from L2.
+__global__ void __launch_bounds__(256) bias_grad_kernel(const float* part, int batch, int heads, int parts, int buckets,
+                                                        float* dtable) {
   __shared__ double sum[256];
   const int h = blockIdx.x, b = blockIdx.y;
   double s = 0.0;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(256) bias_grad_kernel(const float* __restrict_
   const long long n = static_cast<long long>(batch) * parts;
   for (long long t = threadIdx.x; t < n; t += 256) {
     const long long seq = t / parts, at = (seq * heads + h) * parts + t % parts;
-    s += static_cast<double>(part[at * buckets + b]);
+    s += static_cast<double>(__ldcg(part + at * buckets + b));
   }
   sum[threadIdx.x] = s;
   __syncthreads();

@@ -86,3 +86,30 @@ def test_several_units_per_cta(cuda_device, case):
         again = c.results()
         for n in ("out", "dq", "dk", "dv") + (("dtable",) if grad else ()):
             assert np.array_equal(again[n], got[n]), n
+
+
+@pytest.mark.parametrize("batch,heads,seq,d", [(1, 12, 512, 64), (40, 8, 150, 64), (2, 8, 300, 96), (1, 2, 90, 136)])
+def test_the_tables_gradient_in_a_workspace_with_old_contents(cuda_device, batch, heads, seq, d):
+    """Calls on different inputs one behind the other in one workspace, which first holds NaN: the last sum, which is
+    launched before the partials are complete, finds those of its own call."""
+    import torch
+
+    calls, want = [], []
+    for seed in (41, 42):
+        x, valid = make(batch, heads, seq, d, None, seed, 32)
+        c = Call(x, valid, rb.Mask.block(1), 64)
+        c.forward()
+        c.backward()
+        want.append(c.results())
+        close(want[-1]["dtable"], c.want()["dtable"], "dtable")
+        calls.append(c)
+    ws = torch.full((rb.train_workspace(c.shape, c.params, c.bias, backward=True),), 255, dtype=torch.uint8, device="cuda")
+    sums = []
+    for turn in range(20):
+        c = calls[turn % 2]
+        c.dtable.fill_(7.0)
+        c.backward(ws)
+        sums.append(c.dtable.clone())
+    rb.sync_status()
+    for turn, y in enumerate(sums):
+        assert np.array_equal(y.cpu().numpy(), want[turn % 2]["dtable"]), turn
