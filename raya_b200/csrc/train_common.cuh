@@ -109,6 +109,19 @@ __global__ void __launch_bounds__(256) rel_table_kernel(const float* table, int 
 // the kernel before is complete and its writes are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// What a kernel learned by that wait, passed on to the kernels behind it that
+// do not wait themselves: one lane of a warp that has waited says so, a whole
+// warp of the later kernel asks.  Where the word is not (yet) to be seen, that
+// warp waits for the launch before it to be complete, which is always enough.
+__device__ __forceinline__ void publish_primary(unsigned* word) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(word), "r"(1u) : "memory");
+}
+__device__ __forceinline__ void see_primary(const unsigned* word) {
+  unsigned seen;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(word) : "memory");
+  if (!__all_sync(0xffffffffu, seen == 1u)) wait_for_primary();
+  fence_proxy_async_global();
+}
 
 // dtable[head][b] = the sum of its partials over the batch and the parts of
 // each slice, always in the same order (one block per head and bucket; 256

@@ -128,7 +128,8 @@ struct TcArgs {
   int first_image;     // kImgK where the forward kernel splits q itself, else kImgQ
   long long slice0;
   unsigned units;      // 128-row tiles of the chunk
-  unsigned* next;      // [4] by kind: units handed out beyond the first one of each CTA; split_kernel clears them
+  unsigned* next;      // [4] by kind: units handed out beyond the first one of each CTA; split_kernel clears them.
+                       // Backward, [kForward]: 1 once kDq has seen split_kernel complete
   BucketBounds bounds;
   int far;             // the last bucket's first distance
   // With t.part, the table's gradient by distance:
@@ -552,9 +553,15 @@ constexpr int dist_slots(int far) { return (dist_mid(far) + far + 68) / 4 * 4; }
 
 // The launches of a call overlap.  kForward and kDq start while split_kernel
 // ends and wait for it before they read what it wrote; kDk and kDv start
-// where the gradient before leaves room, which is after it waited for
-// split_kernel itself, so they wait for it only before they end (whatever is
-// behind them, the sum of the partials first, is to find all three complete).
+// where the gradient before leaves room, which is after every CTA of kDq has
+// waited for split_kernel, published that and said launch_dependents.  They
+// acquire the published word before they read an image, so that its writes are
+// ordered before their loads and bulk copies, and wait for the launch before
+// them only at their end (whatever is behind them, the sum of the partials
+// first, is to find all three complete).  The word alone cannot tell this
+// call's 1 from one that was in the workspace before: split_kernel has cleared
+// it long before a kDk can exist, and atomics and acquiring loads read L2,
+// where that is the only copy.
 //
 // Persistent: the copy warp takes one unit after the other (the first by
 // blockIdx, the others from a counter, since padding makes them uneven) and
@@ -802,6 +809,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
     int units = 0;
     uint32_t ds_used = 0, ds_phase = 0;  // GRAD, by block: whether it is with the table's warps, the parity of its next return
     ok = take_unit(u);
+    if constexpr (kByKey) fence_proxy_async_global();  // behind the copy warp's see_primary: the images, before the copies
     if (u.n > 0) {
       fetch_rows(u, 0);
       ok = load_first(u, r) && load_rest();
@@ -1285,7 +1293,14 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
         u.n = hi > lo ? (hi + kTileCols - 1) / kTileCols - u.t0 : 0;
       }
       if (first) {
-        if constexpr (kBehindSplit) wait_for_primary();
+        if constexpr (kBehindSplit)
+          wait_for_primary();
+        else
+          see_primary(c.next + kForward);
+        if constexpr (KIND == kDq) {
+          if ((tid & 31) == 0) publish_primary(c.next + kForward);
+          __syncwarp();
+        }
         if constexpr (KIND != kForward) launch_dependents();
         first = false;
       }
