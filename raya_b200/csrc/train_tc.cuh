@@ -7,7 +7,9 @@
 // lo*hi + hi*hi into fp32, and the softmax threads take the exponents off
 // with the factor that they multiply by anyway.  An operand is good to 2^-22
 // of its value, and absolutely to 2^-40 of its tile's largest.  The weights
-// that meet the second operand (w, ds) are scaled too: w by a constant, ds by
+// that meet the second operand (w, ds) are scaled too: w by a constant, and
+// for dv, where a key may have nothing but small ones, by an exponent of its
+// own where the constant would leave them to fp16's smallest steps; ds by
 // an exponent from a bound for each row and tile.  Every tile's product
 // is added into fp32 registers with rounding to nearest, since the tensor
 // core's accumulation truncates.
@@ -99,8 +101,8 @@ constexpr int kPairBarrier = 1, kTableBarrier = 5;
 constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
-constexpr float kWeightLog2 = 14.f;                // kDv: w enters as w * 2^14, so that small ones keep their bits
-constexpr int kRowValues = 4 * 64;                 // values per 64 rows of dout; kDk and kDv read the first three of each
+constexpr float kWeightScale = 16384.f;            // kDv: w <= 1 enters as w * 2^14, fp16's last power of two with room above it
+constexpr int kRowValues = 3 * 64;                 // values per 64 rows of dout; kDk and kDv read the first two of each
 constexpr float kRescale = 8.f, kForwardLog2 = 7.f;  // kForward: p <= 2^8 of the kept maximum, times 2^7
 
 enum TcKind { kForward = 0, kDq = 1, kDk = 2, kDv = 3 };
@@ -121,7 +123,7 @@ struct TcArgs {
   TrainArgs t;
   uint8_t* img[4];     // [chunk slices][tiles][2 P panels]: q, k, v, dout
   TileScale* scales;   // [chunk slices][tiles]
-  float* rows;         // [chunk slices][tiles][4][64]: m * log2(e) (inf: no key), that - kWeightLog2, delta = g . out, |g| 2^e
+  float* rows;         // [chunk slices][tiles][3][64]: m * log2(e) (inf: no key), delta = g . out, |g| 2^e
   const float* table;  // the bias, or nullptr
   float* vec;          // where it goes by distance (t.rel_bias)
   int tiles;           // 64-row tiles per slice (even)
@@ -239,8 +241,7 @@ __global__ void __launch_bounds__(256, P == 1 ? (BACK ? 5 : 6) : 3) split_kernel
           float* rows = c.rows + (static_cast<size_t>(local) * c.tiles + tile) * kRowValues + r + 16 * (half + i);
           const float off = linv != 0.f ? m2 : INFINITY;  // 2^(x - inf) = 0: no key, or past valid_len
           rows[0] = off;
-          rows[64] = off - kWeightLog2;
-          rows[128] = dot;
+          rows[64] = dot;
         }
         if (fabsf(dot) < INFINITY) delta = fmaxf(delta, fabsf(dot));
       }
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(256, P == 1 ? (BACK ? 5 : 6) : 3) split_kernel
     for (int off = 8; off > 0; off >>= 1) square += __shfl_xor_sync(0xffffffffu, square, off);
     const float norm = square < INFINITY ? sqrtf(square) : 0.f;
     longest = fmaxf(longest, norm);
-    if (grad && (tid & 15) == 0) c.rows[at_tile * kRowValues + 192 + r + 16 * i] = norm;
+    if (grad && (tid & 15) == 0) c.rows[at_tile * kRowValues + 128 + r + 16 * i] = norm;
   }
   longest = fmaxf(longest, __shfl_xor_sync(0xffffffffu, longest, 16));
   delta = fmaxf(delta, __shfl_xor_sync(0xffffffffu, delta, 16));
@@ -331,7 +332,7 @@ constexpr int kQueue = 2;
 template <int P>
 struct alignas(16) TcTail {
   float vec[kStages][kVec];       // bias * log2(e) by distance
-  float rows[kStages][192];       // kDk, kDv: the columns' exponents and delta
+  float rows[kStages][128];       // kDk, kDv: the columns' exponents and delta
   TileScale scales[kStages];      // of the columns' 64 rows
   int flat[kStages];              // the tile's pairs all lie in one distance bucket
   float red[2][2][P == 2 ? kTileRows : 1];  // [tile parity][half]: what a row's threads exchange
@@ -472,14 +473,50 @@ __device__ __forceinline__ void mma4_ts_e(uint32_t d, uint32_t a, uint64_t b, ui
 }
 
 // Weights w[32] (fp32, already scaled) as fp16 hi and lo over their scores.
-__device__ __forceinline__ void store_weights(uint32_t taddr, const float* w) {
+// Returns the OR of the hi halves.
+__device__ __forceinline__ uint32_t store_weights(uint32_t taddr, const float* w) {
+  uint32_t all = 0;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     uint32_t h[8], l[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) tc16::split2(w[16 * s + 2 * k], w[16 * s + 2 * k + 1], h[k], l[k]);
+    for (int k = 0; k < 8; ++k) {
+      tc16::split2(w[16 * s + 2 * k], w[16 * s + 2 * k + 1], h[k], l[k]);
+      all |= h[k];
+    }
     tc16::tmem_st8u(taddr + 8 * s, h);
     tc16::tmem_st8u(taddr + 8 * s + 16, l);
+  }
+  return all;
+}
+
+// The largest magnitude of a row's weights, as they are, in those of its two
+// blocks of 32 columns that the bits of `blocks` name.  Both functions are for
+// the rare tile, and no part of the loops that call them.
+__device__ __noinline__ float largest_weight(uint32_t taddr, uint32_t blocks) {
+  float big = 0.f;
+  tc32::tmem_wait_st();
+#pragma unroll 1
+  for (int i = 0; i < 64; i += 16) {
+    if (!(blocks >> (i >> 5) & 1u)) continue;
+    float x[16];
+    tc16::tmem_ld16(taddr + i, x);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) big = fmaxf(big, fabsf(x[k]));
+  }
+  return big;
+}
+
+// These blocks, times f, split in their place.
+__device__ __noinline__ void split_again(uint32_t taddr, uint32_t blocks, float f) {
+#pragma unroll 1
+  for (int q = 0; q < 2; ++q) {
+    if (!(blocks >> q & 1u)) continue;
+    float w[32];
+    tc32::tmem_ld32(taddr + 32 * q, w);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) w[i] *= f;
+    store_weights(taddr + 32 * q, w);
   }
 }
 
@@ -580,7 +617,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
   constexpr int kHalves = P;                                 // threads per row
   constexpr int kW = 64 / kHalves;                           // score columns of a thread
   constexpr int kBlocks = kW / 32;
-  constexpr bool kShared = KIND == kForward && kHalves == 2; // a row's threads share a maximum
+  constexpr bool kShared = (KIND == kForward || KIND == kDv) && kHalves == 2; // a row's threads share a maximum
   constexpr int kRowThreadsTc = 128 * kHalves;
   constexpr int kIssueWarp = kRowWarpsOf(P);                 // then the copy warp and two for the table's gradient
   constexpr uint32_t kCols = 256 * P;
@@ -784,8 +821,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
       r.off = r.delta = 0.f;
       if constexpr (KIND == kDq) {
         r.off = c.rows[tile * kRowValues + (rt & 63)];
-        r.delta = c.rows[tile * kRowValues + 128 + (rt & 63)];
-        r.norm = c.rows[tile * kRowValues + 192 + (rt & 63)];
+        r.delta = c.rows[tile * kRowValues + 64 + (rt & 63)];
+        r.norm = c.rows[tile * kRowValues + 128 + (rt & 63)];
       }
       key_range(a, min(u.r0 + rt, u.valid - 1), u.valid, r.lo, r.hi);
       if (!place_rows(0)) return false;
@@ -861,6 +898,40 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
         x = fmaxf(x, sm.red[g & 1][half ^ 1][rt]);
         return true;
       };
+      // A tile's weights in fp16.  A row with a weight of 2 or more (the top bit
+      // of its hi part's exponent) holds them all to 2^-24, 2^-25 of that one.
+      // The weights of a row without one are scaled by 2^e more, which brings
+      // the largest to 2^14.  A block with such rows is put over its scores
+      // once more as it is (`raw`), and split when the row is known.  Few tiles
+      // have any; the others pay an OR of the halves and a vote (what is behind
+      // the vote, written in line, cost every tile 4%: instruction fetch).
+      struct SmallWeights {
+        int e = 0;
+        bool fits = false, seen = false;
+        uint32_t raw = 0;  // the same on every lane of the warp
+      };
+      // Behind the store of block q; bits: the OR of its hi parts, seen: some of
+      // the row's weights in it may not be zero.
+      auto weigh = [&](SmallWeights& sw, int q, uint32_t scol, const float* w, uint32_t bits, bool seen) {
+        sw.fits |= (bits & 0x40004000u) != 0;
+        sw.seen |= seen;
+        if (__any_sync(0xffffffffu, !sw.fits && sw.seen)) {
+          tmem_wait_st();
+          tmem_st32(scol + 32 * q, w);
+          sw.raw |= 1u << q;
+        }
+      };
+      // Behind the last block.  False if a pair's other warp gave up.
+      auto settle = [&](SmallWeights& sw, uint32_t scol, int g) -> bool {
+        if (kHalves == 2 || sw.raw) {
+          float big = sw.fits ? 2.f : 0.f;
+          if (sw.raw) big = fmaxf(big, largest_weight(scol, sw.raw));
+          if (!share_max(g, big)) return ok = false;
+          if (big < 2.f) sw.e = tc16::scale_exp(__float_as_uint(big));
+          if (sw.raw) split_again(scol, sw.raw, tc16::pow2(sw.e));
+        }
+        return true;
+      };
       nu.n = -1;
       // The next unit's rows: begun before the last tile (with the table's
       // gradient behind it, when the buffer is back), placed behind it.
@@ -891,6 +962,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
         const float mult = finite(r.qmul * tc16::pow2(-e1));
         const bool flat = BIAS && sm.flat[st] != 0;
         const float* const vec = &sm.vec[st][vec_at];
+        const bool some = !flat || vec[0] != -INFINITY;  // the bias leaves the tile
         // 32 columns at a time, in rolled loops (the loop over the tiles is to
         // fit the instruction cache nearest to the scheduler): block q's masked
         // scores, and back into tensor memory until the row's maximum is known.
@@ -954,25 +1026,29 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           factor = tc16::pow2(-e2);
           prepare_next(t);
         } else if constexpr (KIND == kDv) {
+          SmallWeights sw;
 #pragma unroll 1
           for (int q = 0; q < kBlocks; ++q) {
-            const float* off = sm.rows[st] + 64 + kW * half + 32 * q;
+            const float* off = sm.rows[st] + kW * half + 32 * q;
             float s[32];
             block_scores(q, s, nullptr);
+            const float2 up = make_float2(kWeightScale, kWeightScale);
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               const float4 f = *reinterpret_cast<const float4*>(off + i);
               const float2 x = sub2(get2(s + i), make_float2(f.x, f.y)), y = sub2(get2(s + i + 2), make_float2(f.z, f.w));
-              put2(s + i, make_float2(ex2(x.x), ex2(x.y)));
-              put2(s + i + 2, make_float2(ex2(y.x), ex2(y.y)));
+              put2(s + i, __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)), up));
+              put2(s + i + 2, __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), up));
             }
-            store_weights(scol + 32 * q, s);
+            const uint32_t bits = store_weights(scol + 32 * q, s);
+            weigh(sw, q, scol, s, bits, some && mlo < 32 * q + 32 && mhi > 32 * q);
           }
+          if (!settle(sw, scol, G)) break;
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&sm.w_ready[sb]);
           if (t > 0) ok = add_partial(G - 1);
-          factor = tc16::pow2(-e2) * 6.103515625e-05f;  // 2^-14
+          factor = tc16::pow2(-e2) * (1.f / kWeightScale) * tc16::pow2(-sw.e);
           prepare_next(t);
         } else {
           // ds = w (g . v - delta) times 2^e, which brings the bound |g| |v| +
@@ -998,7 +1074,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
               float2 g0 = minus2, g1 = minus2;
               if constexpr (KIND == kDk) {
                 f = *reinterpret_cast<const float4*>(off + i);
-                const float4 g = *reinterpret_cast<const float4*>(off + 128 + i);
+                const float4 g = *reinterpret_cast<const float4*>(off + 64 + i);
                 g0 = __fmul2_rn(make_float2(g.x, g.y), minus2);
                 g1 = __fmul2_rn(make_float2(g.z, g.w), minus2);
               } else {
@@ -1336,7 +1412,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           unsigned char* op = smem + st * stage_bytes<P>();
           uint64_t* bar = &sm.full[st];
           if constexpr (BIAS) sm.flat[st] = rel + 1 >= c.far || rel + kVec - 1 <= -c.far;
-          constexpr uint32_t kScaleBytes = sizeof(TileScale), kRowBytes = 192 * 4;
+          constexpr uint32_t kScaleBytes = sizeof(TileScale), kRowBytes = 128 * 4;
           mbar_arrive_expect_tx(bar, 2 * kOp + kScaleBytes + (BIAS ? kVec * 4u : 0u) + (kByKey ? kRowBytes : 0u));
           tma_load_1d(op, c.img[kB1] + tile * static_cast<long long>(kOp), kOp, bar);
           tma_load_1d(op + kOp, c.img[kB2] + tile * static_cast<long long>(kOp), kOp, bar);

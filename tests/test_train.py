@@ -174,3 +174,22 @@ def test_reference_gradients_against_differences(mask):
             x[i] = was
             # the central difference is off by step^2 / 6 times a third derivative of order 10, and by rounding / step
             assert abs((up - down) / (2 * step) - grad[i]) < 1e-8 + 1e-9 * abs(grad[i]), (name, i)
+
+
+@pytest.mark.parametrize("mask,buckets", [(rb.Mask.block(1), 8), (rb.Mask.sliding(30), 0), (rb.Mask.FULL, 8)])
+def test_tight_bounds_have_the_references_values(mask, buckets):
+    from _train_tight import small, tight
+
+    rng = np.random.default_rng(4)
+    valid = np.array([140, 77])
+    q, k, v, g = (rng.standard_normal((2, 2, 140, 16)) for _ in range(4))
+    k[:, :, 5] *= 30
+    table = rng.standard_normal((2, buckets)) if buckets else None
+    have, want = (f(mask, 32, 0.25, valid, q, k, v, g, table, 6) for f in (tight, reference))
+    for n in want:
+        assert np.array_equal(have[n][0], want[n][0]), n
+        bound = np.broadcast_to(have[n][1], want[n][0].shape)
+        assert np.isfinite(bound).all() and (bound >= 0).all(), n
+    x = small(k)
+    for r in range(140):
+        assert (x[:, :, r, 0] == 2.0 ** -40 * np.abs(k[:, :, r // 64 * 64 : r // 64 * 64 + 64]).max((2, 3))).all()
