@@ -253,9 +253,11 @@ raya_attn_status raya_attn_forward_packed_noalloc(const raya_attn_desc* desc, co
  * without keys.  `stats` is a DEVICE array of batch*heads*seq pairs of
  * floats, and log(l) + m is the row's log-sum-exp.  Products are as good as
  * fp32's (3xFP16 on the tensor cores for head_dim <= 128: to 2^-22 of an
- * element, and absolutely to 2^-40 of the largest of its 64 rows; a weight to
- * 2^-21 of itself, and absolutely to 2^-31 of its row's largest in out and to
- * 2^-25 of the largest of its key and 64 queries in dv, however small).  An
+ * element, and absolutely to 2^-40 of the largest of its 64 rows; the weights
+ * to 2^-21 of themselves, and absolutely to 2^-31 of their row's largest in
+ * out, to 2^-21 of their key's largest in dv and dk, however small that is,
+ * each with the largest dout of its 64 queries in dv and times dout . v - delta
+ * in dk, and to 2^-37 of the bound |dout| |v| + |delta| over l in dq).  An
  * infinity or NaN at or past valid_len is never read; one in a valid row
  * spoils what the plain formulas spoil, where a weight of 0 times it counts
  * as NaN, also for pairs that the mask or the bias excludes.  Scores are

@@ -7,10 +7,10 @@
 // lo*hi + hi*hi into fp32, and the softmax threads take the exponents off
 // with the factor that they multiply by anyway.  An operand is good to 2^-22
 // of its value, and absolutely to 2^-40 of its tile's largest.  The weights
-// that meet the second operand (w, ds) are scaled too: w by a constant, and
-// for dv, where a key may have nothing but small ones, by an exponent of its
-// own where the constant would leave them to fp16's smallest steps; ds by
-// an exponent from a bound for each row and tile.  Every tile's product
+// that meet the second operand (w, ds) are scaled too: w by a constant, ds by
+// an exponent from a bound for each row and tile, and for dv and dk, where a
+// key may have nothing but small ones, by a second exponent where the first
+// would leave them to fp16's smallest steps.  Every tile's product
 // is added into fp32 registers with rounding to nearest, since the tensor
 // core's accumulation truncates.
 //
@@ -102,6 +102,7 @@ constexpr int kStages = 2;
 constexpr int kPanelBytes = 64 * 128;              // 64 rows of 64 fp16
 constexpr int kVec = 192;                          // distances that a 128x64 tile covers (191, and one for alignment)
 constexpr float kWeightScale = 16384.f;            // kDv: w <= 1 enters as w * 2^14, fp16's last power of two with room above it
+constexpr float kSmallWeight = 0.25f;              // kDk, kDv: what is scaled once more where a row has nothing larger
 constexpr int kRowValues = 3 * 64;                 // values per 64 rows of dout; kDk and kDv read the first two of each
 constexpr float kRescale = 8.f, kForwardLog2 = 7.f;  // kForward: p <= 2^8 of the kept maximum, times 2^7
 
@@ -371,6 +372,12 @@ static_assert(tc_smem<1>() <= kHalfSm && tc_smem<1>() > 233472 / 3 && tc_smem<2>
 // A product of scales that would be infinite, as the largest float: 0 times it is 0.
 __device__ __forceinline__ float finite(float x) { return fmaxf(fminf(x, 3.4028235e38f), -3.4028235e38f); }
 
+// 2^e, of two factors: the sum of some exponents may be beyond one float's.
+__device__ __forceinline__ float two_to(int e) {
+  const int a = e >> 1, b = e - a;
+  return tc16::pow2(max(-126, min(127, a))) * tc16::pow2(max(-126, min(127, b)));
+}
+
 // One tensor-map tile into shared memory, completing on `bar`; zeros outside the tensor.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -490,34 +497,43 @@ __device__ __forceinline__ uint32_t store_weights(uint32_t taddr, const float* w
   return all;
 }
 
-// The largest magnitude of a row's weights, as they are, in those of its two
-// blocks of 32 columns that the bits of `blocks` name.  Both functions are for
-// the rare tile, and no part of the loops that call them.
-__device__ __noinline__ float largest_weight(uint32_t taddr, uint32_t blocks) {
-  float big = 0.f;
-  tc32::tmem_wait_st();
-#pragma unroll 1
-  for (int i = 0; i < 64; i += 16) {
-    if (!(blocks >> (i >> 5) & 1u)) continue;
-    float x[16];
-    tc16::tmem_ld16(taddr + i, x);
+// What is left to do for a tile with small weights (see SmallWeights): no part of
+// the loops that call it.  A row's blocks of 32 columns that the bits of `blocks`
+// name are in their places as they are, in fp32.  settle_rows scales and splits
+// them and returns their largest magnitude, or `big`; the two threads of a row
+// do it in two steps, with an exchange between.
+__device__ __forceinline__ float largest(float big, const float* w) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) big = fmaxf(big, fabsf(x[k]));
-  }
+  for (int i = 0; i < 32; i += 2) big = tc32::fmax3(big, fabsf(w[i]), fabsf(w[i + 1]));
   return big;
 }
-
-// These blocks, times f, split in their place.
-__device__ __noinline__ void split_again(uint32_t taddr, uint32_t blocks, float f) {
-#pragma unroll 1
-  for (int q = 0; q < 2; ++q) {
-    if (!(blocks >> q & 1u)) continue;
-    float w[32];
-    tc32::tmem_ld32(taddr + 32 * q, w);
+__device__ __forceinline__ void scale_and_store(uint32_t taddr, float* w, float f) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) w[i] *= f;
-    store_weights(taddr + 32 * q, w);
-  }
+  for (int i = 0; i < 32; ++i) w[i] *= f;
+  store_weights(taddr, w);
+}
+__device__ __forceinline__ int small_exp(float big) { return big < kSmallWeight ? tc16::scale_exp(__float_as_uint(big)) : 0; }
+__device__ __noinline__ float settle_rows(uint32_t taddr, uint32_t blocks, float big) {
+  float w[32], x[32];
+  tc32::tmem_wait_st();
+  tmem_ld32x2(taddr, w, taddr + 32, x);
+  if (blocks & 1u) big = largest(big, w);
+  if (blocks & 2u) big = largest(big, x);
+  const float f = tc16::pow2(small_exp(big));
+  if (blocks & 1u) scale_and_store(taddr, w, f);
+  if (blocks & 2u) scale_and_store(taddr + 32, x, f);
+  return big;
+}
+__device__ __noinline__ float largest_weight(uint32_t taddr, float big) {
+  float w[32];
+  tc32::tmem_wait_st();
+  tc32::tmem_ld32(taddr, w);
+  return largest(big, w);
+}
+__device__ __noinline__ void split_again(uint32_t taddr, float big) {
+  float w[32];
+  tc32::tmem_ld32(taddr, w);
+  scale_and_store(taddr, w, tc16::pow2(small_exp(big)));
 }
 
 // Two neighbouring values for the packed operations.
@@ -617,7 +633,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
   constexpr int kHalves = P;                                 // threads per row
   constexpr int kW = 64 / kHalves;                           // score columns of a thread
   constexpr int kBlocks = kW / 32;
-  constexpr bool kShared = (KIND == kForward || KIND == kDv) && kHalves == 2; // a row's threads share a maximum
+  constexpr bool kShared = KIND != kDq && kHalves == 2;      // a row's threads share a maximum
   constexpr int kRowThreadsTc = 128 * kHalves;
   constexpr int kIssueWarp = kRowWarpsOf(P);                 // then the copy warp and two for the table's gradient
   constexpr uint32_t kCols = 256 * P;
@@ -898,38 +914,45 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
         x = fmaxf(x, sm.red[g & 1][half ^ 1][rt]);
         return true;
       };
-      // A tile's weights in fp16.  A row with a weight of 2 or more (the top bit
-      // of its hi part's exponent) holds them all to 2^-24, 2^-25 of that one.
-      // The weights of a row without one are scaled by 2^e more, which brings
-      // the largest to 2^14.  A block with such rows is put over its scores
-      // once more as it is (`raw`), and split when the row is known.  Few tiles
-      // have any; the others pay an OR of the halves and a vote (what is behind
-      // the vote, written in line, cost every tile 4%: instruction fetch).
+      // kDk and kDv: a key may have nothing but small weights.  Where its largest
+      // so far, in this tile's scale, is kSmallWeight or more, fp16 holds the
+      // tile's to 2^-24 (half a step of hi and of lo), 2^-22 of that one.  The
+      // weights of a row that has had none are scaled by 2^e more, which brings
+      // the largest to 2^14.  A block with such rows is put over its scores once
+      // more as it is (`raw`), and split when the row is known.  The loops pay an
+      // OR of the hi parts, whose exponents have their top bit from 2 on, and a
+      // vote, both behind the stores: a branch before them, or the rest in line,
+      // cost every tile 4%.  With it: every key 478 to 502 us, window 233 to 242.
+      float top = 0.f;  // the row's largest in the unit, unscaled, or less where it is large enough
       struct SmallWeights {
+        float big;        // that in the tile's scale, with the tile's own
         int e = 0;
-        bool fits = false, seen = false;
+        bool seen = false;
         uint32_t raw = 0;  // the same on every lane of the warp
       };
-      // Behind the store of block q; bits: the OR of its hi parts, seen: some of
-      // the row's weights in it may not be zero.
+      // Behind the store of block q, which gave `bits`; seen: some of the row's
+      // weights in it may not be zero.
       auto weigh = [&](SmallWeights& sw, int q, uint32_t scol, const float* w, uint32_t bits, bool seen) {
-        sw.fits |= (bits & 0x40004000u) != 0;
+        if (bits & 0x40004000u) sw.big = fmaxf(sw.big, 2.f);
         sw.seen |= seen;
-        if (__any_sync(0xffffffffu, !sw.fits && sw.seen)) {
+        if (__any_sync(0xffffffffu, sw.seen && !(sw.big >= kSmallWeight))) {
           tmem_wait_st();
           tmem_st32(scol + 32 * q, w);
           sw.raw |= 1u << q;
         }
       };
-      // Behind the last block.  False if a pair's other warp gave up.
-      auto settle = [&](SmallWeights& sw, uint32_t scol, int g) -> bool {
-        if (kHalves == 2 || sw.raw) {
-          float big = sw.fits ? 2.f : 0.f;
-          if (sw.raw) big = fmaxf(big, largest_weight(scol, sw.raw));
-          if (!share_max(g, big)) return ok = false;
-          if (big < 2.f) sw.e = tc16::scale_exp(__float_as_uint(big));
-          if (sw.raw) split_again(scol, sw.raw, tc16::pow2(sw.e));
+      // Behind the last block; down: one over the tile's scale.  False if a
+      // pair's other warp gave up.
+      auto settle = [&](SmallWeights& sw, uint32_t scol, float down, int g) -> bool {
+        if constexpr (kHalves == 1) {
+          if (sw.raw) sw.big = settle_rows(scol, sw.raw, sw.big);
+        } else {
+          if (sw.raw) sw.big = largest_weight(scol, sw.big);
+          if (!share_max(g, sw.big)) return ok = false;
+          if (sw.raw) split_again(scol, sw.big);
         }
+        sw.e = small_exp(sw.big);
+        top = fmaxf(top, fminf(sw.big, 32768.f) * down);
         return true;
       };
       nu.n = -1;
@@ -1027,6 +1050,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           prepare_next(t);
         } else if constexpr (KIND == kDv) {
           SmallWeights sw;
+          sw.big = top * tc16::pow2(e2) * kWeightScale;
 #pragma unroll 1
           for (int q = 0; q < kBlocks; ++q) {
             const float* off = sm.rows[st] + kW * half + 32 * q;
@@ -1043,7 +1067,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
             const uint32_t bits = store_weights(scol + 32 * q, s);
             weigh(sw, q, scol, s, bits, some && mlo < 32 * q + 32 && mhi > 32 * q);
           }
-          if (!settle(sw, scol, G)) break;
+          if (!settle(sw, scol, tc16::pow2(-e2) * (1.f / kWeightScale), G)) break;
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&sm.w_ready[sb]);
@@ -1054,8 +1078,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           // ds = w (g . v - delta) times 2^e, which brings the bound |g| |v| +
           // |delta| (w <= 1, the column's or the row's longest vector) to
           // [2^13, 2^14): four times that still fit, should rounding bring a
-          // weight above 1.  fp16 holds what is 2^-38 of the bound; a pass
-          // for the largest |ds| itself would gain a few bits for 4% of the time.
+          // weight above 1.  fp16 holds what is 2^-37 of the bound.  That will
+          // do for dq, where some weight of the row is of the size of 1.
           const float unit = finite(r.unit * tc16::pow2(-e2));
           const float bound = KIND == kDq ? fmaf(r.norm * sm.scales[st].v_norm, unit, fabsf(r.delta))
                                           : fmaf(r.norm * sm.scales[st].g_norm, unit, sm.scales[st].delta);
@@ -1063,6 +1087,8 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
           const float up = tc16::pow2(e), down = tc16::pow2(-e);
           const float unit_up = finite(unit * up), minus_up = KIND == kDq ? -r.delta * up : -up;
           const float2 unit2 = make_float2(unit_up, unit_up), minus2 = make_float2(minus_up, minus_up);
+          SmallWeights sw;
+          sw.big = top * up;
 #pragma unroll 1
           for (int q = 0; q < kBlocks; ++q) {
             const float* off = sm.rows[st] + kW * half + 32 * q;
@@ -1085,7 +1111,9 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
               put2(s + i, __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)), __ffma2_rn(get2(dp + i), unit2, g0)));
               put2(s + i + 2, __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(get2(dp + i + 2), unit2, g1)));
             }
-            store_weights(scol + 32 * q, s);
+            const uint32_t bits = store_weights(scol + 32 * q, s);
+            if constexpr (KIND == kDk)
+              weigh(sw, q, scol, s, bits, some && bound > 0.f && mlo < 32 * q + 32 && mhi > 32 * q);
             if constexpr (GRAD) {
               const int base = c0 + 32 * q - (u.r0 + (warp & 3) * 32);  // column - row of the block's first pair
               if (!near_block(base, c.far)) {
@@ -1117,10 +1145,13 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
               }
             }
           }
+          if constexpr (KIND == kDk) {
+            if (!settle(sw, scol, down, G)) break;
+          }
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&sm.w_ready[sb]);
-          factor = finite(tc16::pow2(-e) * tc16::pow2(-e1));
+          factor = finite(KIND == kDk ? two_to(-(e + e1 + sw.e)) : tc16::pow2(-e) * tc16::pow2(-e1));
           prepare_next(t);
           if (ok) ok = add_partial(G);
           if (ok && t + 1 == u.n && nu.n > 0) ok = load_rest();

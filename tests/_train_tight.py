@@ -11,13 +11,15 @@ since w is off by its own score's error and the exponential's 2^-22, and l by
 its terms'; nothing in it is absolute, so a weight of 2^-60 is as good as one
 of 1.
 
-What meets the second operand on the tensor cores is held in two fp16 numbers:
-w of dv and ds of dk each to 2^-21 of itself (counted in EPS), or to 2^-24
-after scaling (half a step of hi and of lo), where the largest of a key's 64
-queries is 2 at least: so absolutely to 2^-25 of that largest one.  ds of dq is scaled by the bound
-|g_i| |v_j| + |delta_i| instead and held to 2^-38 of it: dq sums over a row's
-keys, of which one has a weight of the row's size.  The table's gradient takes
-ds in fp32.
+What meets the second operand on the tensor cores is held in two fp16 numbers,
+to 2^-21 of itself (counted in EPS), or after scaling to 2^-24 (half a step of
+hi and of lo).  For dk that is at most 2^-22 of the largest |ds| that the key
+has.  For dv it is 2^-22 of the largest w that the key has had, each one in the
+scale of its 64 queries' dout / l, whose exponents are known to a factor of 2:
+2^-21 of w_s G_s / G with G the largest dout / l of 64 queries.  ds of dq is
+scaled by the bound |g_i| |v_j| + |delta_i| instead and held to 2^-37 of it: dq
+sums over a row's keys, of which one has a weight of the row's size.  The
+table's gradient takes ds in fp32.
 """
 from __future__ import annotations
 
@@ -79,13 +81,18 @@ def tight(mask, block, scale, valid, q, k, v, dout, table=None, max_distance=128
     dse = p * (e * (ga @ va.swapaxes(-1, -2)) + ddelta + 4 * U * (np.abs(dp) + np.abs(delta))) + p * off * np.abs(dp - delta)
     held = e + (s + 8) * U
     t = lambda y: y.swapaxes(-1, -2)  # noqa: E731
-    floor = lambda y, z: 2.0 ** -25 * (t(tops(y, -2)) @ tiles(np.abs(z), -2))  # noqa: E731
+    gl = np.abs(g / some)
+    most_g = tops(gl.max(-1, keepdims=True, initial=0), -2)  # [b, h, tiles, 1]
+    largest = (tops(w * (1 + off), -2) * most_g).max(-2)[..., None]  # [b, h, keys, 1]
+    lost = 2.0 ** -21 * largest * (tiles(gl, -2) / np.where(most_g > 0, most_g, 1)).sum(-2, keepdims=True)
     got = dict(full)
-    got["dv"] = (full["dv"][0], t(p * (off + held)) @ ga + floor(w * (1 + off), g / some))
-    got["dk"] = (full["dk"][0], abs(scale) * (t(dse + held * np.abs(ds)) @ (np.abs(q) + small(q)) + floor(np.abs(ds) + dse, q)))
+    got["dv"] = (full["dv"][0], t(p * (off + held)) @ ga + lost)
+    dsm = (np.abs(ds) + dse).max(-2)[..., None]
+    got["dk"] = (full["dk"][0], abs(scale) * (t(dse + held * np.abs(ds)) @ (np.abs(q) + small(q))
+                                              + 2.0 ** -22 * dsm * np.abs(q).sum(-2, keepdims=True)))
     most = np.where(n > 0, (np.sqrt((g * g).sum(-1, keepdims=True)) * np.sqrt((v * v).sum(-1)).max(-1, initial=0)[..., None, None]
                             + np.abs(delta)) / some, 0.0)
-    got["dq"] = (full["dq"][0], abs(scale) * ((dse + held * np.abs(ds) + 2.0 ** -38 * most * see) @ (np.abs(k) + small(k))))
+    got["dq"] = (full["dq"][0], abs(scale) * ((dse + held * np.abs(ds) + 2.0 ** -37 * most * see) @ (np.abs(k) + small(k))))
     if table is not None:
         tb = np.zeros(table.shape)
         for c in range(table.shape[1]):

@@ -55,3 +55,84 @@ def test_value_gradients_of_small_weights_under_masks(cuda_device, mask, block, 
     x, valid, weak = weak_keys(d, 50, 52, seq=330, amount=6)
     c, got = run(x, valid, mask, block)
     close(got["dv"], want_of(c)["dv"], "dv")
+
+
+@pytest.mark.parametrize("d", [64, 40, 96, 128, 136])
+@pytest.mark.parametrize("bits", [20, 28, 36, 60, 100])
+def test_the_key_gradient_of_keys_with_small_weights(cuda_device, d, bits):
+    x, valid, weak = weak_keys(d, bits, 53, buckets=32 if bits == 36 else 0)
+    c, got = run(x, valid, rb.Mask.FULL, 128)
+    value, bound = want_of(c)["dk"]
+    size = np.abs(value[:, :, weak]).max(-1, keepdims=True)
+    assert (size > 0).all() and (bound[:, :, weak] < 0.25 * size).all()
+    close(got["dk"], (value, bound), "dk")
+
+
+@pytest.mark.parametrize("mask,block", [(rb.Mask.sliding(40), 128), (BLOCK3, 64), (rb.Mask.block(0), 64)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_key_gradients_of_small_weights_under_masks(cuda_device, mask, block, d):
+    x, valid, weak = weak_keys(d, 50, 54, seq=330, amount=6)
+    c, got = run(x, valid, mask, block)
+    close(got["dk"], want_of(c)["dk"], "dk")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_weak_keys_of_units_behind_the_first(cuda_device, d):
+    """The same where each CTA takes several units, some with weak keys and some without."""
+    batch, seq = (80, 150) if d == 64 else (40, 150)
+    x, valid = make(batch, 8, seq, d, None, 55)
+    x["q"][..., 0], x["k"][..., 0] = 4.0, 0.0
+    x["k"][1::3, :, [3, 70, 140], 0] = -45 * np.log(2.0) * np.sqrt(d) / 4.0
+    c, got = run(x, valid, rb.Mask.FULL, 128)
+    want = want_of(c)
+    for n in GRADIENTS:
+        close(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("d", [64, 96, 136])
+def test_gradients_that_are_zero_but_for_a_few_rows(cuda_device, d):
+    """dout of one row only, and of none: keys whose queries have no gradient, next to some that do."""
+    x, valid = make(2, 2, 300, d, [300, 170], 56, 32)
+    for rows in ([7], [], [69, 150]):
+        dout = np.zeros_like(x["dout"])
+        dout[:, :, rows] = x["dout"][:, :, rows]
+        y = dict(x, dout=dout)
+        c, got = run(y, valid, BLOCK3, 64)
+        want = want_of(c)
+        for n in GRADIENTS + ("dtable",):
+            close(got[n], want[n], n)
+            assert rows or (got[n] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_masked_buckets_beside_weak_keys(cuda_device, d):
+    """A bias that masks every key behind the query, and keys with small weights."""
+    x, valid, weak = weak_keys(d, 40, 57, seq=300, buckets=32)
+    x["table"][:, 16:] = -np.inf
+    c, got = run(x, valid, rb.Mask.FULL, 128)
+    want = want_of(c)
+    for n in GRADIENTS + ("dtable",):
+        close(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x) for x in (c[:4] + (c[5].name(), c[6], c[7]))))
+def test_tight_bounds_on_ordinary_inputs(cuda_device, case):
+    batch, heads, seq, d, valid, mask, block, buckets, far = case
+    x, valid = make(batch, heads, seq, d, valid, seq + d, buckets)
+    c, got = run(x, valid, mask, block, max_distance=far or 128)
+    want = want_of(c)
+    for n in GRADIENTS + (("dtable",) if buckets else ()):
+        close(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("d", [64, 96])
+def test_rows_far_smaller_than_their_neighbours(cuda_device, d):
+    """Operands that change by 2^20 from tile to tile, and by 2^12 within one."""
+    x, valid = make(1, 2, 320, d, None, 58)
+    at = np.arange(320)
+    for n in ("v", "dout"):
+        x[n] *= (2.0 ** (20 * (at // 64 % 2) - 10 - 12 * (at % 5 == 3)))[None, None, :, None].astype(np.float32)
+    c, got = run(x, valid, rb.Mask.FULL, 128)
+    want = want_of(c)
+    for n in GRADIENTS:
+        close(got[n], want[n], n)
