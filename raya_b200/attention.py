@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import abc
 import ctypes
+import operator
 from dataclasses import dataclass, field
 from typing import Sequence, Union
 
@@ -211,11 +212,17 @@ class RelativeBias:
     def buckets(self) -> int:
         return int(self.table.shape[-1])
 
+    def sizes(self) -> tuple[int, int]:
+        """(buckets, max_distance) as the library's 32-bit integers: what does
+        not fit becomes the largest one, which it refuses."""
+        n, far = self.buckets, operator.index(self.max_distance)
+        return min(n, 2**31 - 1), far if -2**31 <= far < 2**31 else 2**31 - 1
+
     def bounds(self) -> np.ndarray:
         """The smallest distance of each bucket of one side (host-only)."""
-        n = self.buckets
-        out = np.zeros(max(n // 2, 1), dtype=np.int32)
-        _check(lib.raya_attn_bias_bounds(n, self.max_distance, _i32p(out)))
+        n, far = self.sizes()
+        out = np.zeros(max(min(n, 64) // 2, 1), dtype=np.int32)
+        _check(lib.raya_attn_bias_bounds(n, far, _i32p(out)))
         return out
 
     def bucket(self, rel) -> np.ndarray:
@@ -453,7 +460,7 @@ class Cuda(AttentionKernel):
 def train_workspace(shape: AttnShape, params: AttnParams, bias: RelativeBias | None = None,
                     backward: bool = False) -> int:
     """Workspace bytes of attend_bias, or of attend_backward (host-only)."""
-    b = None if bias is None else _lib.Bias(None, bias.buckets, bias.max_distance)
+    b = None if bias is None else _lib.Bias(None, *bias.sizes())
     return _train_bytes(make_desc(shape, params), b, backward)
 
 
@@ -493,7 +500,7 @@ def _train_call(call, backward, shape, params, tensors, stats, more, bias, dtabl
     b = dtable_ptr = None
     if bias is not None:
         entries = shape.heads * bias.buckets
-        b = _lib.Bias(ptr("table", bias.table, entries), bias.buckets, bias.max_distance)
+        b = _lib.Bias(ptr("table", bias.table, entries), *bias.sizes())
         if dtable is not None:
             dtable_ptr = ptr("dtable", dtable, entries)
     elif dtable is not None:

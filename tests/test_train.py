@@ -193,3 +193,26 @@ def test_tight_bounds_have_the_references_values(mask, buckets):
     x = small(k)
     for r in range(140):
         assert (x[:, :, r, 0] == 2.0 ** -40 * np.abs(k[:, :, r // 64 * 64 : r // 64 * 64 + 64]).max((2, 3))).all()
+
+
+@pytest.mark.parametrize("buckets,max_distance", [(32, 2 ** 32 + 128), (32, 2 ** 31), (32, -(2 ** 32) + 128), (32, 2 ** 64 + 128), (2 ** 32 + 32, 128)])
+def test_sizes_beyond_32_bits_are_refused_in_python(buckets, max_distance):
+    """The library takes 32-bit integers: what does not fit is refused, not cut to one that does."""
+    class Table:
+        shape = (3, buckets)
+
+    bias = rb.RelativeBias(Table(), max_distance)
+    shape, params = rb.AttnShape(heads=3, seq=70, head_dim=64), rb.AttnParams.new(rb.Mask.FULL, 70, 64)
+    refused = rb.ShapeError if buckets == 32 else rb.UnsupportedError
+    for call in (bias.bounds, lambda: bias.bucket(5), lambda: rb.train_workspace(shape, params, bias)):
+        with pytest.raises(refused):
+            call()
+
+
+def test_sizes_may_be_numpy_integers():
+    class Table:
+        shape = (3, np.int64(32))
+
+    assert np.array_equal(rb.RelativeBias(Table(), np.int64(128)).bounds(), bounds(32, 128)[1])
+    with pytest.raises(TypeError):
+        rb.RelativeBias(Table(), 128.5).bounds()
