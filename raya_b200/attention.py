@@ -434,7 +434,8 @@ class Cuda(AttentionKernel):
         Both are optional.  Contiguous CUDA float32 tensors on one device;
         asynchronous on ``stream`` (the current one of that device if None),
         except that uploading ``params.valid_len`` (``valid_len`` None, and
-        some sequence padded) waits for the call.  A caller's ``workspace``
+        some sequence padded) waits for the call; a captured call takes the
+        lengths as a tensor.  A caller's ``workspace``
         (a CUDA tensor of at least train_workspace bytes) must not be used by
         another call meanwhile; without one the call takes it from torch's
         caching allocator."""
@@ -505,13 +506,14 @@ def _train_call(call, backward, shape, params, tensors, stats, more, bias, dtabl
             dtable_ptr = ptr("dtable", dtable, entries)
     elif dtable is not None:
         raise TypeError("dtable without a bias")
-    keep = None
+    host = None
     if valid_len is None:
         host = params.valid_array(shape.batch)
         if (host < 0).any() or (host > shape.seq).any():
             raise ShapeError(f"invalid shape: valid_len outside [0, {shape.seq}]")
-        if (host != shape.seq).any():
-            keep = valid_len = torch.from_numpy(host).to(q.device)
+        if not (host != shape.seq).any():
+            host = None
+    lengths_at = len(args)
     args.append(None if valid_len is None else ptr("valid_len", valid_len, shape.batch, torch.int32))
     args.append(b)
     if backward:
@@ -525,10 +527,15 @@ def _train_call(call, backward, shape, params, tensors, stats, more, bias, dtabl
         ws = workspace
         if ws is None:
             ws = torch.empty(_train_bytes(d, b, backward), dtype=torch.uint8, device=q.device)
+        if host is not None:
+            if torch.cuda.is_current_stream_capturing():
+                raise UnsupportedError("unsupported: padded lengths of params in a captured call (give valid_len as a CUDA tensor)")
+            lengths = torch.from_numpy(host).to(q.device)
+            args[lengths_at] = lengths.data_ptr()
         status = call(d, *args, ws.data_ptr() or None, ws.numel() * ws.element_size(), handle)
         if status != _lib.OK:
             _check(status)
-        if keep is not None:  # keep the uploaded lengths alive until the kernels have run
+        if host is not None:  # the uploaded lengths live until the kernels have run
             _sync(handle)
 
     if stream is None and at == torch.cuda.current_device():
