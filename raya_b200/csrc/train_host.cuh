@@ -116,7 +116,7 @@ raya_attn_status train_plan(const raya_attn_desc* d, const raya_attn_bias* bias,
     plan->tiles = static_cast<int>((d->seq + 127) / 128 * 2);
     plan->parts = plan->tiles / 2;
     const size_t image = static_cast<size_t>(plan->tiles) * 2 * plan->panels * train::kPanelBytes;
-    // The grid of a chunk: three CTAs per 128-row tile and at most 2^31 in all.
+    // The split's grid: one block per 64-row tile (and tensor), below 2^31; the kernels behind it have a CTA per resident one.
     plan->chunk = std::max<long long>(1, std::min<long long>({slices, static_cast<long long>(kMaxImageBytes / ((last - first) * image)),
                                                               0x7fffffffll / (2ll * plan->tiles)}));
     for (int i = first; i < last; ++i) plan->img[i] = take(plan->chunk * image);
