@@ -256,8 +256,8 @@ raya_attn_status raya_attn_forward_packed_noalloc(const raya_attn_desc* desc, co
  * element, and absolutely to 2^-40 of the largest of its 64 rows; the weights
  * to 2^-21 of themselves, and absolutely to 2^-31 of their row's largest in
  * out, to 2^-21 of their key's largest in dv and dk, however small that is,
- * each with the largest dout of its 64 queries in dv and times dout . v - delta
- * in dk, and to 2^-37 of the bound |dout| |v| + |delta| over l in dq).  An
+ * each with the largest dout of its 64 queries in dv (queries without a dout do
+ * not count) and times dout . v - delta in dk, and to 2^-37 of the bound |dout| |v| + |delta| over l in dq).  An
  * infinity or NaN at or past valid_len is never read; one in a valid row
  * spoils what the plain formulas spoil, where a weight of 0 times it counts
  * as NaN, also for pairs that the mask or the bias excludes.  Scores are

@@ -124,7 +124,7 @@ struct TcArgs {
   TrainArgs t;
   uint8_t* img[4];     // [chunk slices][tiles][2 P panels]: q, k, v, dout
   TileScale* scales;   // [chunk slices][tiles]
-  float* rows;         // [chunk slices][tiles][3][64]: m * log2(e) (inf: no key), delta = g . out, |g| 2^e
+  float* rows;         // [chunk slices][tiles][3][64]: m * log2(e) (inf: no key, no dout), delta = g . out, |g| 2^e
   const float* table;  // the bias, or nullptr
   float* vec;          // where it goes by distance (t.rel_bias)
   int tiles;           // 64-row tiles per slice (even)
@@ -296,7 +296,13 @@ __global__ void __launch_bounds__(256, P == 1 ? (BACK ? 5 : 6) : 3) split_kernel
     for (int off = 8; off > 0; off >>= 1) square += __shfl_xor_sync(0xffffffffu, square, off);
     const float norm = square < INFINITY ? sqrtf(square) : 0.f;
     longest = fmaxf(longest, norm);
-    if (grad && (tid & 15) == 0) c.rows[at_tile * kRowValues + 128 + r + 16 * i] = norm;
+    if (grad && (tid & 15) == 0) {
+      float* rows = c.rows + at_tile * kRowValues + r + 16 * i;
+      rows[128] = norm;
+      // A row without a dout adds nothing to any gradient.  Its weights become 0
+      // too, so that they do not hide how small those of the other rows are.
+      if (square == 0.f) rows[0] = INFINITY;
+    }
   }
   longest = fmaxf(longest, __shfl_xor_sync(0xffffffffu, longest, 16));
   delta = fmaxf(delta, __shfl_xor_sync(0xffffffffu, delta, 16));
@@ -1065,7 +1071,7 @@ __global__ void __launch_bounds__(tc_threads(P), P == 1 ? 2 : 1) tc_train(
               put2(s + i + 2, __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), up));
             }
             const uint32_t bits = store_weights(scol + 32 * q, s);
-            weigh(sw, q, scol, s, bits, some && mlo < 32 * q + 32 && mhi > 32 * q);
+            weigh(sw, q, scol, s, bits, some && sm.scales[st].g_norm > 0.f && mlo < 32 * q + 32 && mhi > 32 * q);
           }
           if (!settle(sw, scol, tc16::pow2(-e2) * (1.f / kWeightScale), G)) break;
           tmem_wait_st();

@@ -16,7 +16,8 @@ to 2^-21 of itself (counted in EPS), or after scaling to 2^-24 (half a step of
 hi and of lo).  For dk that is at most 2^-22 of the largest |ds| that the key
 has.  For dv it is 2^-22 of the largest w that the key has had, each one in the
 scale of its 64 queries' dout / l, whose exponents are known to a factor of 2:
-2^-21 of w_s G_s / G with G the largest dout / l of 64 queries.  ds of dq is
+2^-21 of w_s G_s / G with G the largest dout / l of 64 queries; queries without
+a dout do not count.  ds of dq is
 scaled by the bound |g_i| |v_j| + |delta_i| instead and held to 2^-37 of it: dq
 sums over a row's keys, of which one has a weight of the row's size.  The
 table's gradient takes ds in fp32.
@@ -31,6 +32,11 @@ from _train import U, allowed, buckets_of, eps, reference
 def small(x):
     """2^-40 of the largest value of each element's 64 rows, [b, h, s, 1]."""
     return 2.0 ** -40 * spread(np.abs(x).max(-1, keepdims=True, initial=0), -2, np.max)
+
+
+def magnitude(x):
+    """|x| with what its representation may add to it; a zero is exact."""
+    return np.where(x != 0, np.abs(x) + small(x), 0.0)
 
 
 def spread(x, axis, join):
@@ -70,11 +76,11 @@ def tight(mask, block, scale, valid, q, k, v, dout, table=None, max_distance=128
     l = w.sum(-1, keepdims=True)
     some = np.where(l > 0, l, 1)
     p, n = w / some, see.sum(-1, keepdims=True)
-    a = abs(scale) * ((np.abs(q) + small(q)) @ (np.abs(k) + small(k)).swapaxes(-1, -2))
+    a = abs(scale) * (magnitude(q) @ magnitude(k).swapaxes(-1, -2))
     dx = np.where(see, e * a + 4 * U * (a + np.abs(bias) + np.abs(m0)), 0.0)
     # 1.01: the second order
     off = 1.01 * (dx + (p * dx).sum(-1, keepdims=True) + 2.0 ** -21 + (n + 8) * U)
-    ga, va = np.abs(g) + some * small(g / some), np.abs(v) + small(v)
+    ga, va = some * magnitude(g / some), magnitude(v)
     dp, delta = g @ v.swapaxes(-1, -2), (g * full["out"][0]).sum(-1, keepdims=True)
     ddelta = (np.abs(g) * (full["out"][1] + (d + 2) * U * np.abs(full["out"][0]))).sum(-1, keepdims=True)
     ds = p * (dp - delta)
@@ -83,16 +89,17 @@ def tight(mask, block, scale, valid, q, k, v, dout, table=None, max_distance=128
     t = lambda y: y.swapaxes(-1, -2)  # noqa: E731
     gl = np.abs(g / some)
     most_g = tops(gl.max(-1, keepdims=True, initial=0), -2)  # [b, h, tiles, 1]
-    largest = (tops(w * (1 + off), -2) * most_g).max(-2)[..., None]  # [b, h, keys, 1]
+    live = np.abs(g).max(-1, keepdims=True, initial=0) > 0
+    largest = (tops(w * (1 + off) * live, -2) * most_g).max(-2)[..., None]  # [b, h, keys, 1]
     lost = 2.0 ** -21 * largest * (tiles(gl, -2) / np.where(most_g > 0, most_g, 1)).sum(-2, keepdims=True)
     got = dict(full)
     got["dv"] = (full["dv"][0], t(p * (off + held)) @ ga + lost)
     dsm = (np.abs(ds) + dse).max(-2)[..., None]
-    got["dk"] = (full["dk"][0], abs(scale) * (t(dse + held * np.abs(ds)) @ (np.abs(q) + small(q))
+    got["dk"] = (full["dk"][0], abs(scale) * (t(dse + held * np.abs(ds)) @ magnitude(q)
                                               + 2.0 ** -22 * dsm * np.abs(q).sum(-2, keepdims=True)))
     most = np.where(n > 0, (np.sqrt((g * g).sum(-1, keepdims=True)) * np.sqrt((v * v).sum(-1)).max(-1, initial=0)[..., None, None]
                             + np.abs(delta)) / some, 0.0)
-    got["dq"] = (full["dq"][0], abs(scale) * ((dse + held * np.abs(ds) + 2.0 ** -37 * most * see) @ (np.abs(k) + small(k))))
+    got["dq"] = (full["dq"][0], abs(scale) * ((dse + held * np.abs(ds) + 2.0 ** -37 * most * see) @ magnitude(k)))
     if table is not None:
         tb = np.zeros(table.shape)
         for c in range(table.shape[1]):

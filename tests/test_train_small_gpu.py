@@ -104,6 +104,26 @@ def test_gradients_that_are_zero_but_for_a_few_rows(cuda_device, d):
             assert rows or (got[n] == 0).all()
 
 
+@pytest.mark.parametrize("d", [64, 40, 128, 136])
+@pytest.mark.parametrize("live", [[7, 69, 150], [70, 71], [3]])
+def test_weak_keys_of_the_rows_that_have_a_gradient(cuda_device, d, live):
+    """As in training on some tokens only: the other rows' dout is zero, and it is they that weigh the keys highly."""
+    x, valid = make(2, 2, 200, d, [200, 155], 59)
+    weak = [5, 77, 130]
+    x["q"][..., 0], x["k"][..., 0] = 0.0, 0.0
+    x["q"][:, :, live, 0] = 4.0
+    x["k"][:, :, weak, 0] = -45 * np.log(2.0) * np.sqrt(d) / 4.0
+    dout = np.zeros_like(x["dout"])
+    dout[:, :, live] = x["dout"][:, :, live]
+    x["dout"] = dout
+    c, got = run(x, valid, rb.Mask.FULL, 128)
+    want = want_of(c)
+    size = np.abs(want["dv"][0][:, :, weak]).max(-1, keepdims=True)
+    assert (size[0] > 0).all() and (want["dv"][1][0][:, weak] < 4e-3 * size[0]).all()
+    for n in GRADIENTS:
+        close(got[n], want[n], n)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_masked_buckets_beside_weak_keys(cuda_device, d):
     """A bias that masks every key behind the query, and keys with small weights."""
